@@ -46,6 +46,16 @@ SIGNATURES = {
                                      f32, vp, vp]),
     "dcg_qk_norm_rope_kv_append_tokens": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, f32, f32,
                                                 vp, vp, vp, vp, vp, i32, i32, vp, i32, vp]),
+    "dcg_paged_attn_tree_scratch_size": (sz, [i32, i32, i32, i32, i32, i32]),
+    "dcg_paged_attn_tree": (i32, [vp, vp, vp, i64, i32, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
+                                  i32, f32, vp, vp, sz, vp]),
+    "dcg_kv_fork_scratch_size": (sz, [i32, i32, i64]),
+    "dcg_kv_fork": (i32, [vp, vp, i64, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, sz, vp]),
+    "dcg_kv_compact": (i32, [vp, vp, i64, i32, i32, i32, vp, i32, vp, vp, i32, vp, i32, vp, vp]),
+    "dcg_beam_select_scratch_size": (sz, [i32, i32, i64, i32]),
+    "dcg_beam_select": (i32, [vp, i64, i32, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, sz, vp]),
+    "dcg_qk_norm_rope_kv_append_tree": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, f32, f32,
+                                              vp, vp, vp, vp, vp, vp, i32, i32, vp, i32, vp]),
     "dcg_kv_append": (i32, [vp, vp, vp, vp, i32, i32, vp, i32, vp, vp, i32, i32, i32, vp]),
     "dcg_add_rmsnorm_quantize": (i32, [vp, vp, vp, f32, i64, i64, i32, vp, vp]),
     "dcg_swiglu_quantize": (i32, [vp, vp, i64, i64, i64, i32, vp, vp]),

@@ -255,14 +255,16 @@ int dcg_mul_mat(int type, const void* w, int64_t n, int64_t k, const float* x, i
 
 int dcg_device_error(int* code, int clear) {
     if (!code) return fail(DCG_EINVAL, "null pointer");
-    int a = 0, b = 0, c = 0, d = 0, f = 0, g = 0;
+    int a = 0, b = 0, c = 0, d = 0, f = 0, g = 0, h = 0, i = 0;
+    DCG_CUDA(dcg::tree_device_error(&h, clear != 0), "read device error flag");
+    DCG_CUDA(dcg::pages_device_error(&i, clear != 0), "read device error flag");
     DCG_CUDA(dcg::qmm_q8tc_device_error(&f, clear != 0), "read device error flag");
     DCG_CUDA(dcg::m1s_device_error(&g, clear != 0), "read device error flag");
     DCG_CUDA(dcg::gemv_device_error(&a, clear != 0), "read device error flag");
     DCG_CUDA(dcg::qmm_device_error(&b, clear != 0), "read device error flag");
     DCG_CUDA(dcg::attn_device_error(&c, clear != 0), "read device error flag");
     DCG_CUDA(dcg::qmm_tc_device_error(&d, clear != 0), "read device error flag");
-    *code = a ? a : (b ? b : (c ? c : (d ? d : (f ? f : g))));
+    *code = a ? a : (b ? b : (c ? c : (d ? d : (f ? f : (g ? g : (h ? h : i))))));
     return DCG_OK;
 }
 
@@ -324,6 +326,136 @@ int dcg_paged_attn_prefill(const float* q, const void* k_arena, const void* v_ar
     return DCG_OK;
 }
 
+size_t dcg_paged_attn_tree_scratch_size(int n_seqs, int hq, int hkv, int head_dim, int max_seq_tokens, int max_ctx) {
+    if (n_seqs <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || head_dim != 128 || max_seq_tokens <= 0 || max_ctx < 0) return 0;
+    return dcg::tree_scratch_bytes(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
+}
+
+int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena, int64_t n_arena_blocks,
+                        int n_layer, int layer, const int32_t* block_tables, int max_blocks_per_seq,
+                        const int32_t* seq_starts, const int32_t* ctx_lens, const int64_t* tree_mask,
+                        int mask_words, int n_tok, int n_seqs, int max_seq_tokens, int hq, int hkv,
+                        int head_dim, int max_ctx, float scale, float* out, void* scratch,
+                        size_t scratch_bytes, void* stream) {
+    if (n_seqs < 0 || max_seq_tokens < 0 || n_tok < 0) return fail(DCG_EINVAL, "n_seqs, n_tok and max_seq_tokens must be >= 0");
+    if (n_seqs == 0 || max_seq_tokens == 0 || n_tok == 0) return DCG_OK;
+    if (!q || !k_arena || !v_arena || !block_tables || !seq_starts || !ctx_lens || !tree_mask || !out)
+        return fail(DCG_EINVAL, "null pointer");
+    if (head_dim != 128) return fail(DCG_EINVAL, "head_dim must be 128");
+    if (hkv <= 0 || hq <= 0 || hq % hkv) return fail(DCG_EINVAL, "hq must be a multiple of hkv");
+    if (n_layer <= 0 || layer < 0 || layer >= n_layer) return fail(DCG_EINVAL, "bad layer");
+    if (n_arena_blocks <= 0 || n_arena_blocks * n_layer > (int64_t)INT32_MAX / 16)
+        return fail(DCG_EINVAL, "n_arena_blocks * n_layer must be in 1 .. 2^27 - 1");
+    if (max_blocks_per_seq <= 0 || max_blocks_per_seq > INT32_MAX / 16) return fail(DCG_EINVAL, "bad max_blocks_per_seq");
+    if (max_ctx < 0 || max_ctx > 16 * max_blocks_per_seq) return fail(DCG_EINVAL, "max_ctx exceeds the block table");
+    if (mask_words <= 0 || max_seq_tokens > (int64_t)64 * mask_words)
+        return fail(DCG_EINVAL, "tree_mask has too few words for max_seq_tokens");
+    if (n_seqs > 65535 || hq > 65535) return fail(DCG_EINVAL, "n_seqs and hq must be <= 65535");
+    if ((int64_t)max_seq_tokens * (hq / hkv) > INT32_MAX / 2) return fail(DCG_EINVAL, "max_seq_tokens too large");
+    if (!aligned(k_arena, 16) || !aligned(v_arena, 16) || !aligned(q, 16) || !aligned(out, 16) || !aligned(tree_mask, 8))
+        return fail(DCG_EINVAL, "q, out and the arenas must be 16-byte aligned, tree_mask 8-byte");
+    const size_t need = dcg::tree_scratch_bytes(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
+    if (scratch_bytes < need || (need && !scratch))
+        return fail(DCG_ESCRATCH, "tree attention scratch needs " + std::to_string(need) + " bytes");
+    if (need && !aligned(scratch, 256)) return fail(DCG_EINVAL, "scratch must be 256-byte aligned");
+    DCG_CUDA(dcg::launch_paged_attn_tree(q, k_arena, v_arena, n_arena_blocks, n_layer, layer, block_tables,
+                                         max_blocks_per_seq, seq_starts, ctx_lens, tree_mask, mask_words, n_tok,
+                                         n_seqs, max_seq_tokens, hq, hkv, max_ctx, scale, out, scratch,
+                                         (cudaStream_t)stream), "paged_attn_tree");
+    return DCG_OK;
+}
+
+static int pages_common(const void* k_arena, const void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv,
+                        int head_dim, int max_blocks_per_seq) {
+    if (n_layer <= 0 || hkv <= 0 || head_dim <= 0 || n_arena_blocks <= 0 || max_blocks_per_seq <= 0)
+        return fail(DCG_EINVAL, "bad shape");
+    if (n_arena_blocks > INT32_MAX || max_blocks_per_seq > INT32_MAX / 16) return fail(DCG_EINVAL, "too many blocks");
+    if ((int64_t)hkv * head_dim % 8 || (int64_t)hkv * head_dim > INT32_MAX / 32)
+        return fail(DCG_EINVAL, "hkv * head_dim must be a multiple of 8");
+    if (!aligned(k_arena, 16) || !aligned(v_arena, 16)) return fail(DCG_EINVAL, "arenas must be 16-byte aligned");
+    return DCG_OK;
+}
+
+size_t dcg_kv_fork_scratch_size(int n_seqs, int max_blocks_per_seq, int64_t n_arena_blocks) {
+    if (n_seqs <= 0 || max_blocks_per_seq <= 0 || n_arena_blocks <= 0) return 0;
+    return dcg::kv_fork_scratch_bytes(n_seqs, max_blocks_per_seq, n_arena_blocks);
+}
+
+int dcg_kv_fork(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv, int head_dim,
+                int32_t* block_tables, int max_blocks_per_seq, int32_t* ctx_lens, int32_t* n_pages,
+                int32_t* ref_counts, const int32_t* parents, const int32_t* reserve, int n_seqs,
+                int fill_block, int32_t* status, void* scratch, size_t scratch_bytes, void* stream) {
+    if (n_seqs < 0) return fail(DCG_EINVAL, "n_seqs < 0");
+    if (!status) return fail(DCG_EINVAL, "null pointer");
+    if (n_seqs > dcg::kv_fork_max_rows()) return fail(DCG_EINVAL, "n_seqs must be <= " + std::to_string(dcg::kv_fork_max_rows()));
+    if (n_seqs == 0) {
+        DCG_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), (cudaStream_t)stream), "kv_fork");
+        return DCG_OK;
+    }
+    if (!k_arena || !v_arena || !block_tables || !ctx_lens || !n_pages || !ref_counts || !parents || !scratch)
+        return fail(DCG_EINVAL, "null pointer");
+    const int rc = pages_common(k_arena, v_arena, n_arena_blocks, n_layer, hkv, head_dim, max_blocks_per_seq);
+    if (rc) return rc;
+    if (fill_block < 0 || fill_block >= n_arena_blocks) return fail(DCG_EINVAL, "fill_block out of range");
+    if ((int64_t)n_seqs * ((int64_t)max_blocks_per_seq + 1) > INT32_MAX) return fail(DCG_EINVAL, "block table too large");
+    const size_t need = dcg::kv_fork_scratch_bytes(n_seqs, max_blocks_per_seq, n_arena_blocks);
+    if (scratch_bytes < need) return fail(DCG_ESCRATCH, "kv_fork scratch needs " + std::to_string(need) + " bytes");
+    if (!aligned(scratch, 256)) return fail(DCG_EINVAL, "scratch must be 256-byte aligned");
+    DCG_CUDA(dcg::launch_kv_fork(k_arena, v_arena, n_arena_blocks, n_layer, (int64_t)hkv * head_dim * 2, block_tables,
+                                 max_blocks_per_seq, ctx_lens, n_pages, ref_counts, parents, reserve, n_seqs,
+                                 fill_block, status, scratch, (cudaStream_t)stream), "kv_fork");
+    return DCG_OK;
+}
+
+int dcg_kv_compact(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv, int head_dim,
+                   const int32_t* block_tables, int max_blocks_per_seq, const int32_t* base_lens,
+                   const int32_t* path, int max_path, const int32_t* path_lens, int n_seqs,
+                   int32_t* ctx_lens, void* stream) {
+    if (n_seqs < 0) return fail(DCG_EINVAL, "n_seqs < 0");
+    if (n_seqs == 0) return DCG_OK;
+    if (n_seqs > 65535) return fail(DCG_EINVAL, "n_seqs must be <= 65535");
+    if (!k_arena || !v_arena || !block_tables || !base_lens || !path || !path_lens || !ctx_lens)
+        return fail(DCG_EINVAL, "null pointer");
+    const int rc = pages_common(k_arena, v_arena, n_arena_blocks, n_layer, hkv, head_dim, max_blocks_per_seq);
+    if (rc) return rc;
+    if (max_path <= 0 || max_path > dcg::kv_compact_max_path())
+        return fail(DCG_EINVAL, "max_path must be in 1 .. " + std::to_string(dcg::kv_compact_max_path()));
+    if (ctx_lens < base_lens + n_seqs && base_lens < ctx_lens + n_seqs)
+        return fail(DCG_EINVAL, "ctx_lens must not overlap base_lens");
+    DCG_CUDA(dcg::launch_kv_compact(k_arena, v_arena, n_arena_blocks, n_layer, (int64_t)hkv * head_dim * 2,
+                                    block_tables, max_blocks_per_seq, base_lens, path, max_path, path_lens, n_seqs,
+                                    ctx_lens, (cudaStream_t)stream), "kv_compact");
+    return DCG_OK;
+}
+
+static bool beam_shape_ok(int n_groups, int n_beams, int64_t vocab, int k) {
+    return n_groups > 0 && n_beams > 0 && vocab > 0 && vocab <= INT32_MAX && k > 0 && k <= dcg::BEAM_MAX_K &&
+           (int64_t)n_groups * n_beams <= INT32_MAX / dcg::BEAM_MAX_K;
+}
+size_t dcg_beam_select_scratch_size(int n_groups, int n_beams, int64_t vocab, int k) {
+    return beam_shape_ok(n_groups, n_beams, vocab, k) ? dcg::beam_scratch_bytes(n_groups, n_beams, vocab, k) : 0;
+}
+
+int dcg_beam_select(const float* logits, int64_t ld, int n_groups, int n_beams, int64_t vocab,
+                    const float* scores, const uint8_t* finished, int32_t eos, int k, float* out_scores,
+                    int32_t* out_rows, int32_t* out_tokens, void* scratch, size_t scratch_bytes,
+                    void* stream) {
+    if (n_groups < 0) return fail(DCG_EINVAL, "n_groups < 0");
+    if (n_groups == 0) return DCG_OK;
+    if (!beam_shape_ok(n_groups, n_beams, vocab, k))
+        return fail(DCG_EINVAL, "n_beams and vocab must be > 0, k in 1 .. " + std::to_string(dcg::BEAM_MAX_K));
+    if (ld < vocab) return fail(DCG_EINVAL, "ld smaller than a row");
+    if (!logits || !scores || !out_scores || !out_rows || !out_tokens) return fail(DCG_EINVAL, "null pointer");
+    if (!aligned(logits, 4)) return fail(DCG_EINVAL, "logits must be 4-byte aligned");
+    const size_t need = dcg::beam_scratch_bytes(n_groups, n_beams, vocab, k);
+    if (scratch_bytes < need || !scratch)
+        return fail(DCG_ESCRATCH, "beam_select scratch needs " + std::to_string(need) + " bytes");
+    if (!aligned(scratch, 256)) return fail(DCG_EINVAL, "scratch must be 256-byte aligned");
+    DCG_CUDA(dcg::launch_beam_select(logits, ld, n_groups, n_beams, vocab, scores, finished, eos, k, out_scores,
+                                     out_rows, out_tokens, scratch, (cudaStream_t)stream), "beam_select");
+    return DCG_OK;
+}
+
 int dcg_kv_append(const float* k, const float* v, void* k_arena, void* v_arena, int n_layer,
                   int layer, const int32_t* block_tables, int max_blocks_per_seq,
                   const int32_t* seq_ids, const int32_t* positions, int n_tok, int hkv,
@@ -371,7 +503,8 @@ static int qk_rope_common(const float* q, int64_t ldq, const float* k, int64_t l
                                const float* q_norm_w, const float* k_norm_w, float eps, float rope_theta,
                                const int32_t* positions, float* q_out, void* k_arena, void* v_arena,
                                int n_layer, int layer, const int32_t* block_tables,
-                               int max_blocks_per_seq, void* stream, const int32_t* seq_ids) {
+                               int max_blocks_per_seq, void* stream, const int32_t* seq_ids,
+                               const int32_t* slots = nullptr) {
     if (!q || !k || !v || !positions || !q_out || !k_arena || !v_arena || !block_tables)
         return fail(DCG_EINVAL, "null pointer");
     if (!q_norm_w != !k_norm_w) return fail(DCG_EINVAL, "give both QK-norm weights or neither");
@@ -381,7 +514,7 @@ static int qk_rope_common(const float* q, int64_t ldq, const float* k, int64_t l
     if (n_seqs == 0) return DCG_OK;
     DCG_CUDA(dcg::launch_qk_rope_append(q, ldq, k, ldk, v, ldv, n_seqs, hq, hkv, q_norm_w, k_norm_w, eps,
                                         rope_theta, positions, q_out, k_arena, v_arena, n_layer, layer,
-                                        block_tables, max_blocks_per_seq, (cudaStream_t)stream, seq_ids),
+                                        block_tables, max_blocks_per_seq, (cudaStream_t)stream, seq_ids, slots),
              "qk_norm_rope_kv_append");
     return DCG_OK;
 }
@@ -407,6 +540,18 @@ int dcg_qk_norm_rope_kv_append_tokens(const float* q, int64_t ldq, const float* 
     return qk_rope_common(q, ldq, k, ldk, v, ldv, n_tok, hq, hkv, head_dim, q_norm_w, k_norm_w, eps, rope_theta,
                           positions, q_out, k_arena, v_arena, n_layer, layer, block_tables, max_blocks_per_seq,
                           stream, seq_ids);
+}
+
+int dcg_qk_norm_rope_kv_append_tree(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v,
+                                    int64_t ldv, int n_tok, int hq, int hkv, int head_dim,
+                                    const float* q_norm_w, const float* k_norm_w, float eps, float rope_theta,
+                                    const int32_t* seq_ids, const int32_t* positions, const int32_t* slots,
+                                    float* q_out, void* k_arena, void* v_arena, int n_layer, int layer,
+                                    const int32_t* block_tables, int max_blocks_per_seq, void* stream) {
+    if (!seq_ids || !slots) return fail(DCG_EINVAL, "null pointer");
+    return qk_rope_common(q, ldq, k, ldk, v, ldv, n_tok, hq, hkv, head_dim, q_norm_w, k_norm_w, eps, rope_theta,
+                          positions, q_out, k_arena, v_arena, n_layer, layer, block_tables, max_blocks_per_seq,
+                          stream, seq_ids, slots);
 }
 
 size_t dcg_act_size(int act_type, int64_t m, int64_t k) {

@@ -75,6 +75,34 @@ cudaError_t launch_kv_append(const float* k, const float* v, void* karena, void*
                              int layer, const int* bt, int mbs, const int* seq_ids, const int* pos,
                              int n_tok, int hkv, int hd, cudaStream_t st);
 
+// attention of a drafted token tree over the paged cache (attn_tree.cu); words = 64-bit mask words per token
+cudaError_t tree_device_error(int* out, bool clear);
+size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx);
+cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const void* varena, int64_t n_arena_blocks,
+                                   int n_layer, int layer, const int* bt, int mbs, const int* seq_starts,
+                                   const int* ctx, const int64_t* mask, int words, int n_tok, int n_seqs,
+                                   int max_seq_tokens, int hq, int hkv, int max_ctx, float scale, float* out,
+                                   void* scratch, cudaStream_t st);
+
+// forking and compacting of cache pages (kv_pages.cu); slot_bytes = one token's K of one layer
+cudaError_t pages_device_error(int* out, bool clear);
+int kv_fork_max_rows();
+size_t kv_fork_scratch_bytes(int n, int mbs, int64_t n_arena_blocks);
+cudaError_t launch_kv_fork(void* k, void* v, int64_t n_arena_blocks, int n_layer, int64_t slot_bytes, int* bt,
+                           int mbs, int* lens, int* held, int* refs, const int* parents, const int* reserve,
+                           int n, int fill, int* status, void* scratch, cudaStream_t st);
+int kv_compact_max_path();
+cudaError_t launch_kv_compact(void* k, void* v, int64_t n_arena_blocks, int n_layer, int64_t slot_bytes,
+                              const int* bt, int mbs, const int* base_lens, const int* path, int max_path,
+                              const int* path_lens, int n_seqs, int* ctx_lens, cudaStream_t st);
+
+// beam search's selection (beam.cu)
+constexpr int BEAM_MAX_K = 64;
+size_t beam_scratch_bytes(int n_groups, int n_beams, int64_t vocab, int k);
+cudaError_t launch_beam_select(const float* logits, int64_t ld, int n_groups, int n_beams, int64_t vocab,
+                               const float* scores, const uint8_t* finished, int eos, int k, float* out_scores,
+                               int* out_rows, int* out_tokens, void* scratch, cudaStream_t st);
+
 // fused pre-matmul element-wise kernels (fused.cu)
 cudaError_t launch_add_rmsnorm_quant(float* x, const float* delta, const float* w, float eps, int64_t m,
                                      int64_t k, int act_type, void* act, cudaStream_t st);
@@ -84,7 +112,7 @@ cudaError_t launch_qk_rope_append(const float* q, int64_t ldq, const float* k, i
                                   int64_t ldv, int n_seqs, int hq, int hkv, const float* qw, const float* kw,
                                   float eps, float theta, const int* pos, float* q_out, void* karena,
                                   void* varena, int n_layer, int layer, const int* bt, int mbs,
-                                  cudaStream_t st, const int* seq_ids = nullptr);
+                                  cudaStream_t st, const int* seq_ids = nullptr, const int* slots = nullptr);
 
 // error flag of the bounded waits of the GEMV kernels (0 = none); optionally cleared
 cudaError_t gemv_device_error(int* out, bool clear);

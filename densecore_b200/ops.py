@@ -230,6 +230,213 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_arena: torch.Tensor, v_arena: 
         "dcg_kv_append")
 
 
+def _check_all(dev: torch.device, *named):
+    """(tensor, name, dtype) triples: contiguous CUDA tensors of that type on device `dev`."""
+    for t, name, dtype in named:
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.device != dev:
+            _check_cuda(t, name, dtype)
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _call(dev: torch.device, fn: str, *args):
+    """Call a device entry point on `dev` and its current stream (whatever device is current)."""
+    if dev.index == torch.cuda.current_device():
+        rc = getattr(_lib.load(), fn)(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_lib.load(), fn)(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc, fn)
+
+
+def _arena_shape(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int):
+    """(blocks, hkv, head_dim) of a pair of arenas [blocks * n_layer, 16, hkv, head_dim]."""
+    if k_arena.dim() != 4 or k_arena.shape[1] != 16 or n_layer < 1 or k_arena.shape[0] % n_layer:
+        raise ValueError(f"arenas must be [blocks * n_layer, 16, hkv, head_dim], got {tuple(k_arena.shape)}")
+    if v_arena.shape != k_arena.shape:
+        raise ValueError("k_arena and v_arena differ in shape")
+    return k_arena.shape[0] // n_layer, k_arena.shape[2], k_arena.shape[3]
+
+
+def tree_masks(parents) -> torch.Tensor:
+    """Mask rows of a drafted tree: parents[i] < i is the parent of token i (-1: the history), and
+    every token sees its ancestors and itself.  int64 [n, ceil(n / 64)] (CPU), for paged_attn_tree."""
+    n = len(parents)
+    words = max(1, (n + 63) // 64)
+    bits = []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"parents[{i}] = {p}: a token's parent comes before it (or is -1)")
+        bits.append((bits[p] if p >= 0 else 0) | (1 << i))
+    rows = np.array([[(b >> (64 * w)) & 0xFFFFFFFFFFFFFFFF for w in range(words)] for b in bits], dtype=np.uint64)
+    return torch.from_numpy(rows.reshape(n, words).view(np.int64))
+
+
+def paged_attn_tree_scratch_size(n_seqs: int, hq: int, hkv: int, max_seq_tokens: int, max_ctx: int,
+                                 head_dim: int = 128) -> int:
+    return int(_lib.load().dcg_paged_attn_tree_scratch_size(n_seqs, hq, hkv, head_dim, max_seq_tokens, max_ctx))
+
+
+def paged_attn_tree(q: torch.Tensor, k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int, layer: int,
+                    block_tables: torch.Tensor, seq_starts: torch.Tensor, ctx_lens: torch.Tensor,
+                    tree_mask: torch.Tensor, hkv: int, max_seq_tokens: int, max_ctx: int,
+                    scale: float | None = None, out: torch.Tensor | None = None,
+                    scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted token trees over the paged fp16 KV arena.
+
+    q [n_tok, hq, 128] f32, sequence s's drafted tokens are rows seq_starts[s] .. seq_starts[s+1]-1;
+    token t's K/V sit in slot ctx_lens[s] - n_s + t (already appended).  Row i sees the history and
+    drafted token t of its sequence where bit t % 64 of tree_mask[i, t // 64] (int64) is set; a row
+    that sees nothing is zeros (see dcg_paged_attn_tree)."""
+    dev = q.device
+    _check_all(dev, (q, "q", torch.float32), (k_arena, "k_arena", torch.float16), (v_arena, "v_arena", torch.float16),
+               (block_tables, "block_tables", torch.int32), (seq_starts, "seq_starts", torch.int32),
+               (ctx_lens, "ctx_lens", torch.int32), (tree_mask, "tree_mask", torch.int64))
+    if q.dim() != 3 or block_tables.dim() != 2 or tree_mask.dim() != 2:
+        raise ValueError("q must be [n_tok, hq, head_dim], block_tables and tree_mask two-dimensional")
+    n_tok, hq, hd = q.shape
+    n_seqs = ctx_lens.numel()
+    if seq_starts.numel() != n_seqs + 1 or block_tables.shape[0] != n_seqs:
+        raise ValueError("seq_starts needs one entry more than ctx_lens, block_tables as many rows")
+    if tree_mask.shape[0] != n_tok:
+        raise ValueError("tree_mask needs a row for each row of q")
+    per_block = 16 * hkv * hd * n_layer
+    if per_block <= 0 or k_arena.numel() % per_block or v_arena.numel() != k_arena.numel():
+        raise ValueError("arenas are not whole blocks of n_layer x 16 x hkv x head_dim")
+    if scale is None:
+        scale = 1.0 / float(hd) ** 0.5
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_all(dev, (out, "out", torch.float32))
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    if scratch is None:
+        scratch = torch.empty(max(1, paged_attn_tree_scratch_size(n_seqs, hq, hkv, max_seq_tokens, max_ctx, hd)), dtype=torch.uint8, device=dev)
+    else:
+        _check_all(dev, (scratch, "scratch", torch.uint8))
+    _call(dev, "dcg_paged_attn_tree", q.data_ptr(), k_arena.data_ptr(), v_arena.data_ptr(),
+          k_arena.numel() // per_block, n_layer, layer, block_tables.data_ptr(), block_tables.shape[1],
+          seq_starts.data_ptr(), ctx_lens.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], n_tok, n_seqs,
+          max_seq_tokens, hq, hkv, hd, max_ctx, scale, out.data_ptr(), scratch.data_ptr(), scratch.numel())
+    return out
+
+
+def kv_fork_scratch_size(n_seqs: int, max_blocks_per_seq: int, n_arena_blocks: int) -> int:
+    return int(_lib.load().dcg_kv_fork_scratch_size(n_seqs, max_blocks_per_seq, n_arena_blocks))
+
+
+def kv_fork(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int, block_tables: torch.Tensor,
+            ctx_lens: torch.Tensor, n_pages: torch.Tensor, ref_counts: torch.Tensor, parents: torch.Tensor,
+            reserve: torch.Tensor | None = None, fill_page: int = 0, status: torch.Tensor | None = None,
+            scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Row i of the table becomes a child of row parents[i] (-1: empty), in place: it shares the
+    parent's blocks, gets a copy of a partly filled last block that others hold too, and the blocks
+    that ctx_len + reserve[i] tokens need; blocks nobody holds any more are free.  All of
+    block_tables, ctx_lens, n_pages, ref_counts are int32 and updated in place; the arenas are
+    [blocks * n_layer, 16, hkv, head_dim] fp16.  Returns status (int32): 0, or the number of blocks
+    that were missing, or -1 for bad input; unless 0 nothing was changed (see dcg_kv_fork)."""
+    dev = k_arena.device
+    i32 = torch.int32
+    _check_all(dev, (k_arena, "k_arena", torch.float16), (v_arena, "v_arena", torch.float16),
+               (block_tables, "block_tables", i32), (ctx_lens, "ctx_lens", i32), (n_pages, "n_pages", i32),
+               (ref_counts, "ref_counts", i32), (parents, "parents", i32))
+    blocks, hkv, hd = _arena_shape(k_arena, v_arena, n_layer)
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be two-dimensional")
+    n, mbs = block_tables.shape
+    if ctx_lens.numel() != n or n_pages.numel() != n or parents.numel() != n:
+        raise ValueError("ctx_lens, n_pages and parents need an entry for each row of block_tables")
+    if ref_counts.numel() != blocks:
+        raise ValueError(f"ref_counts has {ref_counts.numel()} entries, the arenas hold {blocks} blocks")
+    if reserve is not None:
+        _check_all(dev, (reserve, "reserve", i32))
+        if reserve.numel() != n:
+            raise ValueError("reserve needs an entry for each row of block_tables")
+    if status is None:
+        status = torch.empty((), dtype=i32, device=dev)
+    else:
+        _check_all(dev, (status, "status", i32))
+        if status.numel() < 1:
+            raise ValueError("status must hold one int32")
+    if scratch is None:
+        scratch = torch.empty(max(1, kv_fork_scratch_size(n, mbs, blocks)), dtype=torch.uint8, device=dev)
+    else:
+        _check_all(dev, (scratch, "scratch", torch.uint8))
+    _call(dev, "dcg_kv_fork", k_arena.data_ptr(), v_arena.data_ptr(), blocks, n_layer, hkv, hd,
+          block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), n_pages.data_ptr(), ref_counts.data_ptr(),
+          parents.data_ptr(), reserve.data_ptr() if reserve is not None else None, n, fill_page,
+          status.data_ptr(), scratch.data_ptr(), scratch.numel())
+    return status
+
+
+def kv_compact(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int, block_tables: torch.Tensor,
+               base_lens: torch.Tensor, path: torch.Tensor, path_lens: torch.Tensor, ctx_lens: torch.Tensor) -> None:
+    """Move accepted drafted tokens together: slot base_lens[s] + path[s, j] of sequence s goes to
+    slot base_lens[s] + j for j < path_lens[s], in every layer, and ctx_lens[s] becomes
+    base_lens[s] + path_lens[s] (in place; int32; see dcg_kv_compact)."""
+    dev = k_arena.device
+    i32 = torch.int32
+    _check_all(dev, (k_arena, "k_arena", torch.float16), (v_arena, "v_arena", torch.float16),
+               (block_tables, "block_tables", i32), (base_lens, "base_lens", i32), (path, "path", i32),
+               (path_lens, "path_lens", i32), (ctx_lens, "ctx_lens", i32))
+    blocks, hkv, hd = _arena_shape(k_arena, v_arena, n_layer)
+    if block_tables.dim() != 2 or path.dim() != 2:
+        raise ValueError("block_tables and path must be two-dimensional")
+    n = block_tables.shape[0]
+    if base_lens.numel() != n or path.shape[0] != n or path_lens.numel() != n or ctx_lens.numel() != n:
+        raise ValueError("base_lens, path, path_lens and ctx_lens need an entry for each row of block_tables")
+    _call(dev, "dcg_kv_compact", k_arena.data_ptr(), v_arena.data_ptr(), blocks, n_layer, hkv, hd,
+          block_tables.data_ptr(), block_tables.shape[1], base_lens.data_ptr(), path.data_ptr(), path.shape[1],
+          path_lens.data_ptr(), n, ctx_lens.data_ptr())
+
+
+def beam_select_scratch_size(n_groups: int, n_beams: int, vocab: int, k: int) -> int:
+    return int(_lib.load().dcg_beam_select_scratch_size(n_groups, n_beams, vocab, k))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, k: int,
+                finished: torch.Tensor | None = None, eos: int = -1, out: tuple | None = None,
+                scratch: torch.Tensor | None = None):
+    """The k best continuations of each group of n_beams beams.
+
+    logits [n_groups * n_beams, vocab] f32 (rows may be strided), scores [n_groups * n_beams] f32;
+    candidates score scores[row] + log_softmax(logits[row])[token].  Returns (scores [n_groups, k]
+    f32, rows int32, tokens int32), best first; rows index `logits` (the parents for kv_fork).
+    finished (uint8): a finished row offers itself alone, as token eos (see dcg_beam_select)."""
+    dev = logits.device
+    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be a two-dimensional CUDA tensor of float32 with contiguous rows")
+    rows, vocab = logits.shape
+    if n_beams < 1 or rows % n_beams:
+        raise ValueError(f"{rows} rows of logits are not whole groups of {n_beams} beams")
+    groups = rows // n_beams
+    _check_all(dev, (scores, "scores", torch.float32))
+    if scores.numel() != rows:
+        raise ValueError("scores needs an entry for each row of logits")
+    if finished is not None:
+        _check_all(dev, (finished, "finished", torch.uint8))
+        if finished.numel() != rows:
+            raise ValueError("finished needs an entry for each row of logits")
+    if out is None:
+        out = (torch.empty((groups, k), dtype=torch.float32, device=dev),
+               torch.empty((groups, k), dtype=torch.int32, device=dev),
+               torch.empty((groups, k), dtype=torch.int32, device=dev))
+    else:
+        _check_all(dev, (out[0], "out scores", torch.float32), (out[1], "out rows", torch.int32),
+                   (out[2], "out tokens", torch.int32))
+        if any(t.numel() != groups * k for t in out):
+            raise ValueError("out tensors must hold n_groups * k values")
+    if scratch is None:
+        scratch = torch.empty(max(1, beam_select_scratch_size(groups, n_beams, vocab, k)), dtype=torch.uint8, device=dev)
+    else:
+        _check_all(dev, (scratch, "scratch", torch.uint8))
+    _call(dev, "dcg_beam_select", logits.data_ptr(), logits.stride(0) if rows > 1 else max(vocab, logits.stride(0)),
+          groups, n_beams, vocab, scores.data_ptr(), finished.data_ptr() if finished is not None else None, eos, k,
+          out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), scratch.data_ptr(), scratch.numel())
+    return out
+
+
 def add_rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, act_type: int,
                          act: torch.Tensor, delta: torch.Tensor | None = None) -> torch.Tensor:
     """x += delta (in place, optional); act = quantize(rmsnorm(x) * weight)."""
@@ -268,6 +475,17 @@ def qk_norm_rope_kv_append_tokens(q, ldq, k, ldk, v, ldv, n_tok, hq, hkv, q_norm
         _ptr(k_norm_w) if k_norm_w is not None else None,
         eps, theta, _ptr(seq_ids), _ptr(positions), _ptr(q_out), _ptr(k_arena), _ptr(v_arena), n_layer, layer,
         _ptr(block_tables), block_tables.shape[1], _stream()), "dcg_qk_norm_rope_kv_append_tokens")
+
+
+def qk_norm_rope_kv_append_tree(q, ldq, k, ldk, v, ldv, n_tok, hq, hkv, q_norm_w, k_norm_w, eps, theta,
+                                seq_ids, positions, slots, q_out, k_arena, v_arena, n_layer, layer, block_tables):
+    """qk_norm_rope_kv_append_tokens with the cache slot of each row apart from its position."""
+    _lib.check(_lib.load().dcg_qk_norm_rope_kv_append_tree(
+        _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, n_tok, hq, hkv, 128,
+        _ptr(q_norm_w) if q_norm_w is not None else None,
+        _ptr(k_norm_w) if k_norm_w is not None else None,
+        eps, theta, _ptr(seq_ids), _ptr(positions), _ptr(slots), _ptr(q_out), _ptr(k_arena), _ptr(v_arena), n_layer,
+        layer, _ptr(block_tables), block_tables.shape[1], _stream()), "dcg_qk_norm_rope_kv_append_tree")
 
 
 class HostContext:

@@ -54,10 +54,14 @@ int dcg_set_programmatic_launch(int enable);
 const char* dcg_strerror(int code);
 const char* dcg_last_error(void);
 
-/* Status of the kernels' bounded waits: *code = 0, or DCG_DEVERR_TIMEOUT when a kernel gave up
- * waiting for a bulk copy and returned early (its outputs are then invalid).  clear != 0 resets
- * it.  The flag is read with a blocking copy, so call it between steps. */
+/* Status of the kernels' bounded waits and of the indexes that they read from device memory:
+ * *code = 0, or DCG_DEVERR_TIMEOUT when a kernel gave up waiting for a bulk copy and returned early
+ * (its outputs are then invalid), or DCG_DEVERR_INDEX when dcg_paged_attn_tree or dcg_kv_compact met
+ * a block id, length or path that is out of range and left that access out (a block id that
+ * attention cannot read counts as zeros; a row that kv_compact cannot move stays as it was).
+ * clear != 0 resets it.  The flag is read with a blocking copy, so call it between steps. */
 #define DCG_DEVERR_TIMEOUT 1
+#define DCG_DEVERR_INDEX 2
 int dcg_device_error(int* code, int clear);
 
 /* ---------------------------------------------------------------------------------------------
@@ -169,6 +173,76 @@ int dcg_paged_attn_prefill(const float* q, const void* k_arena, const void* v_ar
                            const int32_t* seq_starts, const int32_t* ctx_lens, int n_seqs, int max_seq_tokens,
                            int hq, int hkv, int head_dim, int max_ctx, float scale, float* out, void* stream);
 
+/* Attention of a drafted token tree over the same cache (speculative decoding: several guesses of the
+ * next tokens verified in one pass; the reference's attention selector, inference.cpp:1506-1573,
+ * knows causal masks only).  Sequence s's drafted tokens are rows seq_starts[s] .. seq_starts[s+1]-1
+ * of q / out ([n_tok][hq][head_dim] f32); drafted token t's K/V sit in slot ctx_lens[s] - n_s + t
+ * (already appended).  Token i sees every key of the history (0 .. ctx_lens[s] - n_s - 1) and
+ * drafted token t of its own sequence when bit t % 64 of tree_mask[i * mask_words + t / 64] is set
+ * (i: row of q).  A token that sees no key gets zeros.  K may hold anything in slots that no token
+ * sees; a non-finite V of a drafted token makes NaN of the rows (token, head) that see it and of no
+ * other; slots at and past ctx_lens[s] may hold anything.  Rows of q outside all sequences are
+ * neither read nor written.  Each n_s must be <= max_seq_tokens and <= 64 * mask_words, each
+ * ctx_lens[s] in [n_s, max_ctx].  hq / hkv: any whole number.  head_dim must be 128.  scratch:
+ * dcg_paged_attn_tree_scratch_size bytes, 256-B aligned, not shared by calls that may overlap. */
+size_t dcg_paged_attn_tree_scratch_size(int n_seqs, int hq, int hkv, int head_dim, int max_seq_tokens, int max_ctx);
+int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena, int64_t n_arena_blocks,
+                        int n_layer, int layer, const int32_t* block_tables, int max_blocks_per_seq,
+                        const int32_t* seq_starts, const int32_t* ctx_lens, const int64_t* tree_mask,
+                        int mask_words, int n_tok, int n_seqs, int max_seq_tokens, int hq, int hkv,
+                        int head_dim, int max_ctx, float scale, float* out, void* scratch,
+                        size_t scratch_bytes, void* stream);
+
+/* Fork rows of a block table (beam search, sampling several continuations, growing and freeing
+ * sequences), on the device and in place.  Row i of the n_seqs rows becomes a child of row
+ * parents[i]: it takes the parent's length and shares its first ceil(len / 16) blocks; -1 empties
+ * it.  n_pages[i] is the number of blocks that row i holds, ref_counts[b] how often block b is held
+ * (by rows of this table or anyone else).  Then, rows in ascending order: a row whose last block is
+ * partly filled (len % 16 != 0) and has another holder gets a block of its own, into which the first
+ * len % 16 slots of every layer are copied; and every row that is not emptied gets the blocks that
+ * len + reserve[i] tokens need (reserve NULL: none beyond len).  New blocks are the lowest ones whose
+ * reference count is 0, in that order; blocks of the old table that no row needs any more fall to 0.
+ * parents[i] = i for all i grows, and frees what lies past the lengths.  Entries of a row from its
+ * new to its old n_pages are set to fill_block, which should hold a reference of its own.
+ * *status (device) is 0; > 0: so many blocks were missing; < 0: a parent, length, block count or
+ * block id was out of range.  In the last two cases nothing is changed.  n_seqs <= 4096;
+ * hkv * head_dim a multiple of 8; arenas 16-B aligned; scratch: dcg_kv_fork_scratch_size bytes,
+ * 256-B aligned, not shared by calls that may overlap. */
+size_t dcg_kv_fork_scratch_size(int n_seqs, int max_blocks_per_seq, int64_t n_arena_blocks);
+int dcg_kv_fork(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv, int head_dim,
+                int32_t* block_tables, int max_blocks_per_seq, int32_t* ctx_lens, int32_t* n_pages,
+                int32_t* ref_counts, const int32_t* parents, const int32_t* reserve, int n_seqs,
+                int fill_block, int32_t* status, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Move an accepted path of drafted tokens together: for every layer and j < path_lens[s], slot
+ * base_lens[s] + path[s][j] of sequence s goes to slot base_lens[s] + j, and ctx_lens[s] becomes
+ * base_lens[s] + path_lens[s].  path [n_seqs][max_path] must ascend strictly within path_lens[s]
+ * (ancestors are drafted before their descendants).  Blocks that are written must not be shared
+ * with other rows (dcg_kv_fork gives every row its own last blocks); blocks past the new length stay
+ * held until the next dcg_kv_fork.  ctx_lens must not overlap base_lens.  A row with a bad path,
+ * length or block id is left as it was (DCG_DEVERR_INDEX).  max_path <= 1024, n_seqs <= 65535;
+ * hkv * head_dim a multiple of 8; arenas 16-B aligned. */
+int dcg_kv_compact(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv, int head_dim,
+                   const int32_t* block_tables, int max_blocks_per_seq, const int32_t* base_lens,
+                   const int32_t* path, int max_path, const int32_t* path_lens, int n_seqs,
+                   int32_t* ctx_lens, void* stream);
+
+/* Beam search's selection.  Rows g * n_beams .. of logits (row stride ld floats) are the beams of
+ * group g; candidate (row, token) scores scores[row] + logits[row][token] - log sum exp logits[row].
+ * Per group, the k best candidates, best first: out_scores / out_rows (row, the parent for
+ * dcg_kv_fork) / out_tokens, each [n_groups][k].  Scores are compared in 64 bits; equal ones go to
+ * the lower row, in a row to the larger logit, then to the lower token.  A row with finished[row]
+ * != 0 (finished may be NULL) offers one candidate, token eos at its own score.  -inf logits are no
+ * candidates; a row whose score is not finite, or whose logits hold a NaN or +inf or are all -inf,
+ * offers none.  Places without a candidate get score -inf, row -1 and token -1.  k <= 64;
+ * vocab < 2^31; scratch: dcg_beam_select_scratch_size bytes, 256-B aligned, not shared by calls
+ * that may overlap. */
+size_t dcg_beam_select_scratch_size(int n_groups, int n_beams, int64_t vocab, int k);
+int dcg_beam_select(const float* logits, int64_t ld, int n_groups, int n_beams, int64_t vocab,
+                    const float* scores, const uint8_t* finished, int32_t eos, int k, float* out_scores,
+                    int32_t* out_rows, int32_t* out_tokens, void* scratch, size_t scratch_bytes,
+                    void* stream);
+
 /* KV append -- PagedKVCache::WriteKSlot / WriteVSlot (kv_cache.cpp:566-598) for n_tok tokens at
  * once: token i (k, v: [n_tok][hkv][head_dim] f32) goes to slot positions[i] of sequence
  * seq_ids[i] through its block table, converted to fp16 (round to nearest even). */
@@ -200,6 +274,14 @@ int dcg_qk_norm_rope_kv_append_tokens(const float* q, int64_t ldq, const float* 
                                       const int32_t* seq_ids, const int32_t* positions, float* q_out,
                                       void* k_arena, void* v_arena, int n_layer, int layer,
                                       const int32_t* block_tables, int max_blocks_per_seq, void* stream);
+/* The same for the tokens of drafted trees: row i is rotated to positions[i] (its depth in the text)
+ * and its K/V go to cache slot slots[i] of its sequence (siblings share a position, not a slot). */
+int dcg_qk_norm_rope_kv_append_tree(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v,
+                                    int64_t ldv, int n_tok, int hq, int hkv, int head_dim,
+                                    const float* q_norm_w, const float* k_norm_w, float eps, float rope_theta,
+                                    const int32_t* seq_ids, const int32_t* positions, const int32_t* slots,
+                                    float* q_out, void* k_arena, void* v_arena, int n_layer, int layer,
+                                    const int32_t* block_tables, int max_blocks_per_seq, void* stream);
 int dcg_add_rmsnorm_quantize(float* x, const float* delta, const float* weight, float eps, int64_t m,
                              int64_t k, int act_type, void* act, void* stream);
 int dcg_swiglu_quantize(const float* gate, const float* up, int64_t ld, int64_t m, int64_t ffn,
