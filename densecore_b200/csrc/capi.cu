@@ -429,7 +429,7 @@ int dcg_kv_compact(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_l
 }
 
 static bool beam_shape_ok(int n_groups, int n_beams, int64_t vocab, int k) {
-    return n_groups > 0 && n_beams > 0 && vocab > 0 && vocab <= INT32_MAX && k > 0 && k <= dcg::BEAM_MAX_K &&
+    return n_groups > 0 && n_beams > 0 && n_beams <= dcg::BEAM_MAX_BEAMS && vocab > 0 && vocab <= (1 << 30) && k > 0 && k <= dcg::BEAM_MAX_K &&
            (int64_t)n_groups * n_beams <= INT32_MAX / dcg::BEAM_MAX_K;
 }
 size_t dcg_beam_select_scratch_size(int n_groups, int n_beams, int64_t vocab, int k) {
@@ -443,7 +443,8 @@ int dcg_beam_select(const float* logits, int64_t ld, int n_groups, int n_beams, 
     if (n_groups < 0) return fail(DCG_EINVAL, "n_groups < 0");
     if (n_groups == 0) return DCG_OK;
     if (!beam_shape_ok(n_groups, n_beams, vocab, k))
-        return fail(DCG_EINVAL, "n_beams and vocab must be > 0, k in 1 .. " + std::to_string(dcg::BEAM_MAX_K));
+        return fail(DCG_EINVAL, "vocab must be in 1 .. 2^30, n_beams in 1 .. " + std::to_string(dcg::BEAM_MAX_BEAMS) + " and k in 1 .. " +
+                                std::to_string(dcg::BEAM_MAX_K));
     if (ld < vocab) return fail(DCG_EINVAL, "ld smaller than a row");
     if (!logits || !scores || !out_scores || !out_rows || !out_tokens) return fail(DCG_EINVAL, "null pointer");
     if (!aligned(logits, 4)) return fail(DCG_EINVAL, "logits must be 4-byte aligned");
