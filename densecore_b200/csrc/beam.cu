@@ -9,7 +9,8 @@
 //
 // beam_rows_kernel reads every logit once, in tiles of BEAM_TILE, cut into equal ranges of tiles per
 // CTA whatever row they lie in.  Per part of a row that a CTA meets it leaves the part's k largest
-// logits and its (max, sum of exp).  beam_merge_kernel, one CTA per group, joins the parts.
+// logits, and per tile and warp the max and the sum of exp(x - max) over the others: sums that do not
+// depend on how the rows were cut, so that rows with the same logits tie exactly.  beam_merge_kernel, one CTA per group, joins them.
 #include <math.h>
 
 #include "../../include/dcgpu.h"
@@ -22,16 +23,39 @@ constexpr int BEAM_THREADS = 256;
 constexpr int BEAM_WARPS = BEAM_THREADS / 32;
 constexpr int BEAM_PER = 16;                             // logits per thread and tile
 constexpr int BEAM_TILE = BEAM_THREADS * BEAM_PER;
-constexpr int BEAM_CTAS = 5;                             // resident CTAs per SM (33 KB of keys each)
+constexpr int BEAM_CTAS = 4;                             // resident CTAs per SM (36 KB of keys each)
 constexpr int BEAM_RANK = 256;                           // lists up to this long are sorted by counting
-constexpr int BEAM_LIMIT = BEAM_RANK - 64;               // a list that grew this long is pruned
-constexpr int BEAM_CAP = BEAM_LIMIT + BEAM_TILE;         // a whole tile always fits
+constexpr int BEAM_FEW = 64;                             // longer ones after a threshold
+constexpr int BEAM_CAP = 2 * BEAM_MAX_K + 32 + BEAM_TILE;   // pruned beyond 2 k + 32: a whole tile always fits
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));   // NaN only if all are
+    return y;
+}
+// (x0, x1) * a + b, and sums, two at a time
+__device__ __forceinline__ uint64_t pack2(float x0, float x1) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x0), "f"(x1));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& x0, float& x1) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
 }
 
 // order-preserving key of a logit and its token: larger logit first, then the lower token; 0 = none
@@ -44,63 +68,92 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
     return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u);
 }
 __device__ __forceinline__ uint32_t key_token(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
-// order-preserving map of a finite double, never 0
-__device__ __forceinline__ uint64_t score_key(double s) {
-    const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);
-    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+__device__ __forceinline__ uint64_t umax64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// order-preserving map of a float (NaN apart), never 0
+__device__ __forceinline__ uint32_t float_key(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ uint64_t umax64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t umin64(uint64_t a, uint64_t b) { return a < b ? a : b; }
-
 // the warp's 32 values in descending order of lane (bitonic network)
-__device__ __forceinline__ uint64_t warp_sort(uint64_t v) {
+__device__ __forceinline__ uint32_t warp_sort(uint32_t v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int d = size >> 1; d; d >>= 1) {
-            const uint64_t w = __shfl_xor_sync(0xffffffffu, v, d);
-            const bool down = (lane & size) == 0, low = (lane & d) == 0;
-            v = down == low ? umax64(v, w) : umin64(v, w);
+            const uint32_t w = __shfl_xor_sync(0xffffffffu, v, d);
+            v = ((lane & size) == 0) == ((lane & d) == 0) ? max(v, w) : min(v, w);
         }
     return v;
 }
 
-// A value that at least k (<= 64) of the CTA's 256 values reach, near the k-th largest of them: of
-// the 4 largest of each warp the k-th, beyond 32 the least of the warps' 8-th largest.
-__device__ uint64_t block_threshold(uint64_t mine, int k, uint64_t* sh /* 32 */) {
+// A value that at least k (<= 64) of the CTA's 256 values reach, near the k-th largest of them: the
+// k-th of the warps' 4 (k > 16: 8) largest.  sh[64]: where warp 0 finds them; the result is left in
+// sh[0].  Starts and ends with a barrier.
+__device__ uint32_t block_threshold(uint32_t mine, int k, uint32_t* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint64_t v = warp_sort(mine);
+    const int each = k <= 16 ? 4 : 8;
+    const uint32_t v = warp_sort(mine);
     __syncthreads();                      // sh free
-    if (k <= 32) {
-        if (lane < 4) sh[warp * 4 + lane] = v;
-    } else if (lane == 7) {
-        sh[warp] = v;
+    if (lane < each) sh[warp * each + lane] = v;
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t a = warp_sort(sh[lane]);
+        if (each == 8) {
+            // two sorted halves, one of them reversed: their maxima are the 32 largest, their minima the rest
+            const uint32_t b = __shfl_xor_sync(0xffffffffu, warp_sort(sh[32 + lane]), 31);
+            a = warp_sort(k <= 32 ? max(a, b) : min(a, b));
+        }
+        a = __shfl_sync(0xffffffffu, a, (k - 1) & 31);
+        if (lane == 0) sh[0] = a;
     }
     __syncthreads();
-    if (k <= 32) return __shfl_sync(0xffffffffu, warp_sort(sh[lane]), k - 1);
-    uint64_t t = sh[0];
-#pragma unroll
-    for (int w = 1; w < BEAM_WARPS; w++) t = umin64(t, sh[w]);
-    return t;
+    return sh[0];
 }
 
-// list[0 .. n) -> its min(n, k) largest, sorted, in list[0 ..); all threads call it after a barrier
-// that completed the list; ends with a barrier
-__device__ int prune_keys(uint64_t* list, int n, int k, uint64_t* sh) {
+// shared memory of the selection
+struct Select {
+    uint32_t sh[64];
+    uint64_t top[BEAM_WARPS];
+    int count;                            // of the growing list
+    int kept;                             // of the list that a pruning makes
+};
+
+// list[0 .. n) -> its min(n, k) largest, sorted, in list[0 ..); tmp[BEAM_RANK]: room of its own.
+// All threads call it after a barrier that completed the list; ends with a barrier.
+__device__ int prune_keys(uint64_t* list, uint64_t* tmp, int n, int k, Select& S) {
     const int keep = n < k ? n : k;
-    if (n <= BEAM_RANK) {                 // rank by counting: the keys are distinct
-        const uint64_t mine = threadIdx.x < n ? list[threadIdx.x] : 0;
-        int rank = 0;
-        if (threadIdx.x < n)
-            for (int i = 0; i < n; i++) rank += list[i] > mine;
+    int m = n;
+    const uint64_t* from = list;
+    if (n > BEAM_FEW) {                   // first those that reach a threshold, from each thread's largest
+        uint32_t best = 0;
+        for (int i = threadIdx.x; i < n; i += BEAM_THREADS) best = max(best, (uint32_t)(list[i] >> 32));
+        if (threadIdx.x == 0) S.kept = 0;
+        const uint32_t th = block_threshold(best, k, S.sh);
+        for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
+            const uint64_t x = list[i];
+            if ((uint32_t)(x >> 32) >= th) {
+                const int slot = atomicAdd(&S.kept, 1);
+                if (slot < BEAM_RANK) tmp[slot] = x;
+            }
+        }
         __syncthreads();
-        if (threadIdx.x < n && rank < keep) list[rank] = mine;
+        m = S.kept;
+        from = tmp;
+    }
+    if (m <= BEAM_RANK) {                 // rank by counting: the keys are distinct
+        const uint64_t mine = threadIdx.x < m ? from[threadIdx.x] : 0;
+        int rank = 0;
+        if (threadIdx.x < m)
+            for (int i = 0; i < m; i++) rank += from[i] > mine;
+        __syncthreads();
+        if (threadIdx.x < m && rank < keep) list[rank] = mine;
         __syncthreads();
         return keep;
     }
-    // long lists (an adverse order of the logits): one maximum after the other, each below the last
+    // many equal logits: one maximum after the other, each below the last
     uint64_t below = ~0ull;
     uint64_t found = 0;                   // thread r < keep remembers the r-th
     for (int r = 0; r < keep; r++) {
@@ -111,11 +164,11 @@ __device__ int prune_keys(uint64_t* list, int n, int k, uint64_t* sh) {
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) best = umax64(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = best;
+        if ((threadIdx.x & 31) == 0) S.top[threadIdx.x >> 5] = best;
         __syncthreads();
-        best = sh[0];
+        best = S.top[0];
 #pragma unroll
-        for (int w = 1; w < BEAM_WARPS; w++) best = umax64(best, sh[w]);
+        for (int w = 1; w < BEAM_WARPS; w++) best = umax64(best, S.top[w]);
         __syncthreads();
         below = best;
         if (threadIdx.x == r) found = best;
@@ -129,115 +182,137 @@ __device__ int prune_keys(uint64_t* list, int n, int k, uint64_t* sh) {
 __host__ __device__ __forceinline__ int64_t beam_begin(int64_t c, int64_t T, int64_t G) { return c * T / G; }
 __device__ __forceinline__ int64_t beam_owner(int64_t u, int64_t T, int64_t G) { return ((u + 1) * G - 1) / T; }
 
-struct BeamPart {
-    double m, s;      // max (0 if there is none) and sum exp(x - m) of the part; s NaN: a NaN or +inf
-};
-
-__global__ void __launch_bounds__(BEAM_THREADS, BEAM_CTAS) beam_rows_kernel(
-    const float* __restrict__ x, int64_t ld, int vocab, int k, int tpr, int64_t T, int max_parts,
-    uint64_t* __restrict__ keys, BeamPart* __restrict__ parts) {
-    __shared__ uint64_t list[BEAM_CAP];
-    __shared__ uint64_t sh[32];
-    __shared__ float wm[BEAM_WARPS];
-    __shared__ double ws[BEAM_WARPS];
-    __shared__ int count;
-    pdl_wait();
-    pdl_trigger();
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int64_t G = gridDim.x, u0 = beam_begin(blockIdx.x, T, G), u1 = beam_begin(blockIdx.x + 1, T, G);
-    float m = -INFINITY;
-    double s = 0.0;
-    int n = 0;                             // keys in the list after it was last pruned
-    float tv = -INFINITY;                  // logits below (tv, ti) cannot be among the part's k largest
-    uint32_t ti = 0;
-    bool seeded = false;
-    if (t == 0) count = 0;
-    for (int64_t u = u0; u < u1; u++) {
-        const int64_t row = u / tpr;
-        const int base = (int)(u % tpr) * BEAM_TILE + t;
-        const float* p = x + row * ld;
-        float v[BEAM_PER];
+// a tile of a row: logits base, base + 256, ... below vocab, -inf beyond
+__device__ __forceinline__ void load_tile(float (&v)[BEAM_PER], const float* __restrict__ p, int base, int vocab, bool whole) {
+    if (whole) {
+#pragma unroll
+        for (int j = 0; j < BEAM_PER; j++) v[j] = __ldcs(p + base + j * BEAM_THREADS);
+    } else {
 #pragma unroll
         for (int j = 0; j < BEAM_PER; j++) {
             const int i = base + j * BEAM_THREADS;
             v[j] = i < vocab ? __ldcs(p + i) : -INFINITY;
         }
-        // max and sum of exp: 16 terms in fp32, then on in 64 bits
-        float mt = v[0];
+    }
+}
+
+// One part of a row: tiles u0 .. u1 - 1 of the whole, all of row `row`.  The list takes the logits
+// that reach (tv, ti).  The first tile sets the threshold, at its r-th largest logit:
+//   CHECKED = false: r may be below k when the part is long (about 4 k logits of the part are then
+//     expected to reach it), and no thread waits for another until the part is read.  Returns false
+//     if fewer than k logits came, or more than the list holds.
+//   CHECKED = true: r = k, which at least k logits reach whatever the order of the logits; the list
+//     is pruned, and the threshold raised, whenever it has grown.
+template <bool CHECKED>
+__device__ bool read_part(const float* __restrict__ p, int64_t u0, int64_t u1, int tile0, int vocab, int k, int tpr,
+                          float2* __restrict__ sums, uint64_t* list, uint64_t* tmp, Select& S) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int tiles = (int)(u1 - u0);
+    const int r = CHECKED ? k : min(k, max(8, (4 * k + tiles - 1) / tiles));
+    float tv = -INFINITY;
+    uint32_t ti = 0xFFFFFFFFu;
+    if (t == 0) S.count = 0;
+    float next[BEAM_PER];
+    load_tile(next, p, tile0 * BEAM_TILE + t, vocab, tile0 + 1 < tpr);
+    for (int i = 0; i < tiles; i++) {
+        const int base = (tile0 + i) * BEAM_TILE + t;
+        float v[BEAM_PER];
 #pragma unroll
-        for (int j = 1; j < BEAM_PER; j++) mt = fmaxf(mt, v[j]);
-        if (mt > m) {
-            s *= (double)ex2((m - mt) * LOG2E);
-            m = mt;
+        for (int j = 0; j < BEAM_PER; j++) v[j] = next[j];
+        if (i + 1 < tiles) load_tile(next, p, base + BEAM_TILE, vocab, tile0 + i + 2 < tpr);
+        float m4[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) m4[j] = fmaxf(fmaxf(v[j], v[j + 4]), fmaxf(v[j + 8], v[j + 12]));
+        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float mw = warp_max(mt);
+        const float me = mw == -INFINITY ? 0.0f : mw;
+        // s = sum 2^(v c - me c), c = log2 e in fp32, as fma(v, c, -h) with h = me c rounded; what that
+        // rounding lost is one factor for the whole warp
+        const float h = me * LOG2E, l = fmaf(me, LOG2E, -h);
+        const uint64_t c2 = pack2(LOG2E, LOG2E), h2 = pack2(-h, -h);
+        uint64_t a0 = 0, a1 = 0;
+#pragma unroll
+        for (int j = 0; j < BEAM_PER; j += 4) {
+            float e0, e1, e2, e3;
+            unpack2(fma2(pack2(v[j], v[j + 1]), c2, h2), e0, e1);
+            unpack2(fma2(pack2(v[j + 2], v[j + 3]), c2, h2), e2, e3);
+            a0 = add2(a0, pack2(ex2(e0), ex2(e1)));
+            a1 = add2(a1, pack2(ex2(e2), ex2(e3)));
         }
-        const float me = m == -INFINITY ? 0.0f : m;
-        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        float s, s1;
+        unpack2(add2(a0, a1), s, s1);
+        s = (s + s1) * ex2(-l);
 #pragma unroll
-        for (int j = 0; j < BEAM_PER; j++) a[j & 3] += ex2((v[j] - me) * LOG2E);
-        s += (double)((a[0] + a[1]) + (a[2] + a[3]));
-        if (!seeded) {                     // the first tile of a part
-            uint64_t best = 0;
-            if (mt > -INFINITY) {
-#pragma unroll
-                for (int j = BEAM_PER - 1; j >= 0; j--)
-                    if (v[j] == mt) best = beam_key(mt, (uint32_t)(base + j * BEAM_THREADS));
-            }
-            const uint64_t th = block_threshold(best, k, sh);
-            tv = th ? key_logit(th) : -INFINITY;
-            ti = key_token(th);
-            seeded = true;
-        }
-        bool over = false;
-        if (mt >= tv && mt > -INFINITY) {
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        float r1 = s - 1.0f;               // the sum without the largest logit's own 1
+        if (s < 1.015625f || !(fabsf(me) < 1e38f)) {
+            // one logit far above the rest (lse - max would be lost next to 1), or me c overflows: the
+            // rest alone.  +inf makes it NaN, as a NaN does
+            bool skip = lane == __ffs(__ballot_sync(0xffffffffu, mt == mw)) - 1;
+            r1 = me == INFINITY ? NAN : 0.0f;
 #pragma unroll
             for (int j = 0; j < BEAM_PER; j++) {
-                const uint32_t i = (uint32_t)(base + j * BEAM_THREADS);
-                if (v[j] > tv || (v[j] == tv && i <= ti && v[j] > -INFINITY)) {
-                    const int slot = atomicAdd(&count, 1);
-                    list[slot] = beam_key(v[j], i);
-                    over |= slot >= BEAM_LIMIT;
+                if (skip && v[j] == mw) skip = false;
+                else r1 += ex2((v[j] - me) * LOG2E);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) r1 += __shfl_xor_sync(0xffffffffu, r1, o);
+        }
+        if (lane == 0) sums[(u0 + i) * BEAM_WARPS + warp] = make_float2(mw, r1);
+        if (i == 0) tv = key_logit((uint64_t)block_threshold(float_key(mt), r, S.sh) << 32);
+        bool over = false;
+        if (mw >= tv && mw > -INFINITY) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                if (!__any_sync(0xffffffffu, m4[g] >= tv)) continue;
+#pragma unroll
+                for (int j = g; j < BEAM_PER; j += 4) {
+                    const uint32_t at = (uint32_t)(base + j * BEAM_THREADS);
+                    if (v[j] > tv || (v[j] == tv && at <= ti && v[j] > -INFINITY)) {
+                        const int slot = atomicAdd(&S.count, 1);
+                        if (CHECKED || slot < BEAM_CAP) list[slot] = beam_key(v[j], at);
+                        if (CHECKED) over |= slot >= 2 * k + 32;
+                    }
                 }
             }
         }
-        const bool last = u + 1 == u1 || (u + 1) % tpr == 0;
-        // one barrier a tile; `count` is only read where every thread then waits before adding again
-        if (__syncthreads_or(over || last)) {
-            n = prune_keys(list, count, k, sh);
-            if (t == 0) count = n;
+        // the count is only read where every thread then waits before adding again
+        if (CHECKED && __syncthreads_or(over)) {
+            const int n = prune_keys(list, tmp, S.count, k, S);
+            if (t == 0) S.count = n;
             if (n == k) {
                 tv = key_logit(list[k - 1]);
                 ti = key_token(list[k - 1]);
             }
             __syncthreads();
         }
-        if (last) {
-            const int64_t part = blockIdx.x - beam_owner(row * tpr, T, G);
-            uint64_t* out = keys + (row * max_parts + part) * k;
-            if (t < k) out[t] = t < n ? list[t] : 0;
-            // join the threads' sums at the CTA's maximum
-            float M = m;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            if (lane == 0) wm[warp] = M;
+    }
+    __syncthreads();
+    return S.count <= BEAM_CAP && (S.count >= k || r == k);
+}
+
+__global__ void __launch_bounds__(BEAM_THREADS, BEAM_CTAS) beam_rows_kernel(
+    const float* __restrict__ x, int64_t ld, int vocab, int k, int tpr, int64_t T, int max_parts,
+    uint64_t* __restrict__ keys, float2* __restrict__ sums) {
+    __shared__ uint64_t list[BEAM_CAP];
+    __shared__ uint64_t tmp[BEAM_RANK];
+    __shared__ Select S;
+    pdl_wait();
+    pdl_trigger();
+    const int64_t G = gridDim.x, end = beam_begin(blockIdx.x + 1, T, G);
+    for (int64_t u0 = beam_begin(blockIdx.x, T, G), u1; u0 < end; u0 = u1) {
+        const int64_t row = u0 / tpr;
+        const int tile0 = (int)(u0 % tpr);
+        u1 = u0 + tpr - tile0 < end ? u0 + tpr - tile0 : end;
+        const float* p = x + row * ld;
+        if (!read_part<false>(p, u0, u1, tile0, vocab, k, tpr, sums, list, tmp, S)) {
             __syncthreads();
-            M = wm[0];
-#pragma unroll
-            for (int w = 1; w < BEAM_WARPS; w++) M = fmaxf(M, wm[w]);
-            if (M == -INFINITY) M = 0.0f;
-            s *= (double)ex2((m - M) * LOG2E);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (lane == 0) ws[warp] = s;
-            if (t == 0) count = 0;
-            __syncthreads();
-            if (t == 0) {
-                for (int w = 1; w < BEAM_WARPS; w++) s += ws[w];
-                parts[row * max_parts + part] = {(double)M, s};
-            }
-            m = -INFINITY;
-            s = 0.0;
-            seeded = false;
+            read_part<true>(p, u0, u1, tile0, vocab, k, tpr, sums, list, tmp, S);
         }
+        const int n = prune_keys(list, tmp, S.count, k, S);
+        const int64_t part = blockIdx.x - beam_owner(row * tpr, T, G);
+        if (threadIdx.x < k) keys[(row * max_parts + part) * k + threadIdx.x] = threadIdx.x < n ? list[threadIdx.x] : 0;
+        __syncthreads();
     }
 }
 
@@ -255,39 +330,35 @@ constexpr int MERGE_TILE = BEAM_THREADS * MERGE_PER;
 
 // one CTA per group; candidate c = (rank c / lists in part-list c % lists): the heads come first
 __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
-    const uint64_t* __restrict__ keys, const BeamPart* __restrict__ parts, int tpr, int64_t T, int64_t G, int max_parts,
+    const uint64_t* __restrict__ keys, const float2* __restrict__ sums, int tpr, int64_t T, int64_t G, int max_parts,
     const float* __restrict__ scores, const uint8_t* __restrict__ finished, int eos, int n_beams, int k,
     float* __restrict__ out_scores, int* __restrict__ out_rows, int* __restrict__ out_tokens) {
     __shared__ Cand list[BEAM_RANK + MERGE_TILE];
     __shared__ double lse[BEAM_MAX_BEAMS];
-    __shared__ uint64_t sh[32];
+    __shared__ Cand tmp[BEAM_RANK];
+    __shared__ Select S;
     __shared__ Cand best_of[BEAM_WARPS];
-    __shared__ int count;
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t row0 = (int64_t)blockIdx.x * n_beams;
-    // lse of each live beam; NaN: the beam offers no candidate; finished beams: 0 parts
+    // lse of each beam, not finite where the beam offers no candidate
     for (int b = warp; b < n_beams; b += BEAM_WARPS) {
-        const int64_t row = row0 + b;
-        const int np = (int)(beam_owner(row * tpr + tpr - 1, T, G) - beam_owner(row * tpr, T, G)) + 1;
-        double M = -INFINITY;
-        for (int i = lane; i < np; i += 32) {
-            const BeamPart p = parts[row * max_parts + i];
-            if (p.s > 0.0) M = fmax(M, p.m);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmax(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const int64_t first = (row0 + b) * tpr * BEAM_WARPS;
+        const int np = tpr * BEAM_WARPS;
+        float M = -INFINITY;
+        for (int i = lane; i < np; i += 32) M = fmaxf(M, sums[first + i].x);
+        M = warp_max(M);
         double s = 0.0;
         for (int i = lane; i < np; i += 32) {
-            const BeamPart p = parts[row * max_parts + i];
-            if (p.s != 0.0) s += p.s * exp(p.m - M);
+            const float2 p = sums[first + i];
+            if (p.x > -INFINITY || p.y != 0.0f) s += (1.0 + (double)p.y) * (double)ex2((p.x - M) * LOG2E);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) lse[b] = M + log(s);
+        if (lane == 0) lse[b] = (double)M + log(s);
     }
-    if (t == 0) count = 0;
+    if (t == 0) S.count = 0;
     __syncthreads();
     const int64_t lists = (int64_t)n_beams * max_parts, N = lists * k;
     int n = 0;
@@ -295,7 +366,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
     Cand bound = {-INFINITY, 0, 0};
     for (int64_t c0 = 0; c0 < N; c0 += MERGE_TILE) {
         Cand v[MERGE_PER];
-        uint64_t best = 0;
+        uint32_t best = 0;
 #pragma unroll
         for (int j = 0; j < MERGE_PER; j++) {
             const int64_t c = c0 + j * BEAM_THREADS + t;
@@ -312,30 +383,47 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
                     if (key) v[j] = {sc + ((double)key_logit(key) - lse[b]), key, b};
                 }
                 if (!isfinite(sc) || !isfinite(v[j].score)) v[j].row = -1;
-                if (v[j].row >= 0) best = umax64(best, score_key(v[j].score));
+                if (v[j].row >= 0) best = max(best, float_key(__double2float_rd(v[j].score)));
             }
         }
-        const uint64_t th = c0 == 0 ? block_threshold(best, k, sh) : 0;
+        // scores rounded down keep their order
+        const uint32_t th = c0 == 0 ? block_threshold(best, k, S.sh) : 0;
         bool over = false;
 #pragma unroll
         for (int j = 0; j < MERGE_PER; j++)
-            if (v[j].row >= 0 && (full ? better(v[j], bound) : score_key(v[j].score) >= th)) {
-                const int slot = atomicAdd(&count, 1);
+            if (v[j].row >= 0 && (full ? better(v[j], bound) : float_key(__double2float_rd(v[j].score)) >= th)) {
+                const int slot = atomicAdd(&S.count, 1);
                 list[slot] = v[j];
                 over |= slot >= BEAM_RANK;
             }
         if (__syncthreads_or(over || c0 + MERGE_TILE >= N)) {
-            n = count;
+            n = S.count;
             const int keep = n < k ? n : k;
-            if (n <= BEAM_RANK) {
+            int m = n;
+            const Cand* from = list;
+            if (n > BEAM_FEW) {            // as prune_keys, by score alone
+                uint32_t top = 0;
+                for (int i = t; i < n; i += BEAM_THREADS) top = max(top, float_key(__double2float_rd(list[i].score)));
+                if (t == 0) S.kept = 0;
+                const uint32_t reach = block_threshold(top, k, S.sh);
+                for (int i = t; i < n; i += BEAM_THREADS)
+                    if (float_key(__double2float_rd(list[i].score)) >= reach) {
+                        const int slot = atomicAdd(&S.kept, 1);
+                        if (slot < BEAM_RANK) tmp[slot] = list[i];
+                    }
+                __syncthreads();
+                m = S.kept;
+                from = tmp;
+            }
+            if (m <= BEAM_RANK) {
                 Cand mine = {0, 0, 0};
                 int rank = 0;
-                if (t < n) {
-                    mine = list[t];
-                    for (int i = 0; i < n; i++) rank += better(list[i], mine);
+                if (t < m) {
+                    mine = from[t];
+                    for (int i = 0; i < m; i++) rank += better(from[i], mine);
                 }
                 __syncthreads();
-                if (t < n && rank < keep) list[rank] = mine;
+                if (t < m && rank < keep) list[rank] = mine;
             } else {
                 Cand found = {0, 0, 0}, below = {INFINITY, 0, 0};
                 for (int r = 0; r < keep; r++) {
@@ -366,7 +454,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
             }
             __syncthreads();
             n = keep;
-            if (t == 0) count = n;
+            if (t == 0) S.count = n;
             __syncthreads();
             full = n == k;
             if (full) bound = list[k - 1];
@@ -401,7 +489,7 @@ static BeamPlan beam_plan(int n_groups, int n_beams, int64_t vocab, int k) {
     p.max_parts = (int)((p.tpr + least - 1) / least + 1);
     if (p.max_parts > p.tpr) p.max_parts = p.tpr;
     p.keys_bytes = align256((size_t)rows * p.max_parts * k * 8);
-    p.bytes = p.keys_bytes + align256((size_t)rows * p.max_parts * sizeof(BeamPart));
+    p.bytes = p.keys_bytes + align256((size_t)p.T * BEAM_WARPS * sizeof(float2));
     return p;
 }
 
@@ -414,12 +502,12 @@ cudaError_t launch_beam_select(const float* logits, int64_t ld, int n_groups, in
                                int* out_rows, int* out_tokens, void* scratch, cudaStream_t st) {
     const BeamPlan p = beam_plan(n_groups, n_beams, vocab, k);
     uint64_t* keys = (uint64_t*)scratch;
-    BeamPart* parts = (BeamPart*)((uint8_t*)scratch + p.keys_bytes);
+    float2* sums = (float2*)((uint8_t*)scratch + p.keys_bytes);
     cudaError_t e = launch_pdl(beam_rows_kernel, dim3((unsigned)p.G), dim3(BEAM_THREADS), 0, st, logits, ld, (int)vocab, k,
-                               p.tpr, p.T, p.max_parts, keys, parts);
+                               p.tpr, p.T, p.max_parts, keys, sums);
     if (e != cudaSuccess) return e;
     return launch_pdl(beam_merge_kernel, dim3((unsigned)n_groups), dim3(BEAM_THREADS), 0, st, (const uint64_t*)keys,
-                      (const BeamPart*)parts, p.tpr, p.T, p.G, p.max_parts, scores, finished, eos, n_beams, k, out_scores,
+                      (const float2*)sums, p.tpr, p.T, p.G, p.max_parts, scores, finished, eos, n_beams, k, out_scores,
                       out_rows, out_tokens);
 }
 
