@@ -147,6 +147,7 @@ __device__ int prune_keys(uint64_t* list, uint64_t* tmp, int n, int k, Select& S
         const uint64_t mine = threadIdx.x < m ? from[threadIdx.x] : 0;
         int rank = 0;
         if (threadIdx.x < m)
+#pragma unroll 4
             for (int i = 0; i < m; i++) rank += from[i] > mine;
         __syncthreads();
         if (threadIdx.x < m && rank < keep) list[rank] = mine;
@@ -330,11 +331,12 @@ constexpr int MERGE_TILE = BEAM_THREADS * MERGE_PER;
 
 // one CTA per group; candidate c = (rank c / lists in part-list c % lists): the heads come first
 __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
-    const uint64_t* __restrict__ keys, const float2* __restrict__ sums, int tpr, int64_t T, int64_t G, int max_parts,
+    const uint64_t* __restrict__ keys, const float2* __restrict__ sums, int tpr, int64_t T, int G, int max_parts,
     const float* __restrict__ scores, const uint8_t* __restrict__ finished, int eos, int n_beams, int k,
     float* __restrict__ out_scores, int* __restrict__ out_rows, int* __restrict__ out_tokens) {
     __shared__ Cand list[BEAM_RANK + MERGE_TILE];
-    __shared__ double lse[BEAM_MAX_BEAMS];
+    __shared__ double score_of[BEAM_MAX_BEAMS], lse_of[BEAM_MAX_BEAMS];   // not finite: no candidate
+    __shared__ int n_parts[BEAM_MAX_BEAMS];     // of each beam; 0: finished
     __shared__ Cand tmp[BEAM_RANK];
     __shared__ Select S;
     __shared__ Cand best_of[BEAM_WARPS];
@@ -342,52 +344,58 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
     pdl_trigger();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t row0 = (int64_t)blockIdx.x * n_beams;
-    // lse of each beam, not finite where the beam offers no candidate
+    const int lists = n_beams * max_parts, N = lists * k;   // max_parts <= G: below 2^31
+    for (int b = t; b < n_beams; b += BEAM_THREADS) {
+        const int64_t u = (row0 + b) * tpr;
+        n_parts[b] = finished && finished[row0 + b] ? 0 : (int)(beam_owner(u + tpr - 1, T, G) - beam_owner(u, T, G)) + 1;
+    }
     for (int b = warp; b < n_beams; b += BEAM_WARPS) {
-        const int64_t first = (row0 + b) * tpr * BEAM_WARPS;
+        const float2* p = sums + (row0 + b) * tpr * BEAM_WARPS;
         const int np = tpr * BEAM_WARPS;
         float M = -INFINITY;
-        for (int i = lane; i < np; i += 32) M = fmaxf(M, sums[first + i].x);
+#pragma unroll 4
+        for (int i = lane; i < np; i += 32) M = fmaxf(M, p[i].x);
         M = warp_max(M);
         double s = 0.0;
+#pragma unroll 4
         for (int i = lane; i < np; i += 32) {
-            const float2 p = sums[first + i];
-            if (p.x > -INFINITY || p.y != 0.0f) s += (1.0 + (double)p.y) * (double)ex2((p.x - M) * LOG2E);
+            const float2 q = p[i];
+            if (q.x > -INFINITY || q.y != 0.0f) s += (1.0 + (double)q.y) * (double)ex2((q.x - M) * LOG2E);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) lse[b] = (double)M + log(s);
+        if (lane == 0) {
+            score_of[b] = scores[row0 + b];
+            lse_of[b] = (double)M + log(s);
+        }
     }
     if (t == 0) S.count = 0;
     __syncthreads();
-    const int64_t lists = (int64_t)n_beams * max_parts, N = lists * k;
     int n = 0;
     bool full = false;                     // list[k - 1] bounds what may still enter
     Cand bound = {-INFINITY, 0, 0};
-    for (int64_t c0 = 0; c0 < N; c0 += MERGE_TILE) {
+    uint32_t th = 0;
+    for (int c0 = 0; c0 < N; c0 += MERGE_TILE) {
         Cand v[MERGE_PER];
         uint32_t best = 0;
 #pragma unroll
         for (int j = 0; j < MERGE_PER; j++) {
-            const int64_t c = c0 + j * BEAM_THREADS + t;
+            const int c = c0 + j * BEAM_THREADS + t;
             v[j] = {-INFINITY, 0, -1};
             if (c < N) {
-                const int l = (int)(c % lists), rank = (int)(c / lists), b = l / max_parts, part = l % max_parts;
-                const int64_t row = row0 + b;
-                const double sc = scores[row];
-                const bool done = finished && finished[row];
-                if (done && rank == 0 && part == 0) {
-                    v[j] = {sc, ~0ull, b};
-                } else if (!done && part <= beam_owner(row * tpr + tpr - 1, T, G) - beam_owner(row * tpr, T, G)) {
-                    const uint64_t key = keys[(row * max_parts + part) * k + rank];
-                    if (key) v[j] = {sc + ((double)key_logit(key) - lse[b]), key, b};
+                const int rank = c / lists, l = c - rank * lists, b = l / max_parts, part = l - b * max_parts;
+                if (n_parts[b] == 0 ? rank == 0 && part == 0 : part < n_parts[b]) {
+                    const uint64_t key = n_parts[b] == 0 ? ~0ull : keys[((row0 + b) * max_parts + part) * k + rank];
+                    const double score = n_parts[b] == 0 ? score_of[b] : score_of[b] + ((double)key_logit(key) - lse_of[b]);
+                    if (key && isfinite(score)) {
+                        v[j] = {score, key, b};
+                        best = max(best, float_key(__double2float_rd(score)));
+                    }
                 }
-                if (!isfinite(sc) || !isfinite(v[j].score)) v[j].row = -1;
-                if (v[j].row >= 0) best = max(best, float_key(__double2float_rd(v[j].score)));
             }
         }
         // scores rounded down keep their order
-        const uint32_t th = c0 == 0 ? block_threshold(best, k, S.sh) : 0;
+        if (c0 == 0) th = block_threshold(best, k, S.sh);
         bool over = false;
 #pragma unroll
         for (int j = 0; j < MERGE_PER; j++)
@@ -420,6 +428,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
                 int rank = 0;
                 if (t < m) {
                     mine = from[t];
+#pragma unroll 4
                     for (int i = 0; i < m; i++) rank += better(from[i], mine);
                 }
                 __syncthreads();
@@ -507,7 +516,7 @@ cudaError_t launch_beam_select(const float* logits, int64_t ld, int n_groups, in
                                p.tpr, p.T, p.max_parts, keys, sums);
     if (e != cudaSuccess) return e;
     return launch_pdl(beam_merge_kernel, dim3((unsigned)n_groups), dim3(BEAM_THREADS), 0, st, (const uint64_t*)keys,
-                      (const float2*)sums, p.tpr, p.T, p.G, p.max_parts, scores, finished, eos, n_beams, k, out_scores,
+                      (const float2*)sums, p.tpr, p.T, (int)p.G, p.max_parts, scores, finished, eos, n_beams, k, out_scores,
                       out_rows, out_tokens);
 }
 

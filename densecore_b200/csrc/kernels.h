@@ -98,7 +98,7 @@ cudaError_t launch_kv_compact(void* k, void* v, int64_t n_arena_blocks, int n_la
 
 // beam search's selection (beam.cu)
 constexpr int BEAM_MAX_K = 64;
-constexpr int BEAM_MAX_BEAMS = 1024;
+constexpr int BEAM_MAX_BEAMS = 512;
 size_t beam_scratch_bytes(int n_groups, int n_beams, int64_t vocab, int k);
 cudaError_t launch_beam_select(const float* logits, int64_t ld, int n_groups, int n_beams, int64_t vocab,
                                const float* scores, const uint8_t* finished, int eos, int k, float* out_scores,
