@@ -1,20 +1,28 @@
 // attn_tree.cu -- attention of a drafted token tree over DenseCore's paged fp16 KV cache.
 //
 // Beside the causal masks of the reference's attention selector (core/src/inference.cpp:1506-1573):
-// drafted token i sees the whole history and, of the draft, the tokens
-// whose bit is set in its mask row (its ancestors and itself).  Layout and checks as attn.cu.
+// drafted token i sees the whole history and, of the draft, the tokens whose bit is set in its mask
+// row (its ancestors and itself).  Layout and checks as attn.cu.
+//
+// The (token, query head) pairs that share a kv head are the rows of one matrix: every K/V byte is
+// read once for up to 128 of them.  An item is (sequence, kv head, tile of 128 rows), a unit one tile
+// of 128 keys of an item; the units of the whole batch, in order, are cut into one equal range per
+// CTA (one CTA per SM), so ragged contexts load every SM alike.  Items that a range cuts leave their
+// parts (unnormalised output, max, sum) in scratch; tree_combine_kernel joins them in CTA order.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "../../include/dcgpu.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace dcg {
 
 constexpr int HD = 128;
 constexpr int KVB = 16;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int TREE_WARPS = 8;
 
 __device__ int g_tree_error = 0;
 
@@ -27,82 +35,765 @@ cudaError_t tree_device_error(int* out, bool clear) {
     return e;
 }
 
-// one CTA per (drafted token, query head); warp w takes keys w, w + 8, ...; a lane holds 4 dims
-__global__ void __launch_bounds__(TREE_WARPS * 32) tree_simple_kernel(
-    const float* __restrict__ q, const __half* __restrict__ karena, const __half* __restrict__ varena,
-    int64_t n_arena_blocks, int n_layer, int layer, const int* __restrict__ bt, int mbs,
-    const int* __restrict__ seq_starts, const int* __restrict__ ctx, const int64_t* __restrict__ mask,
-    int words, int n_tok, int max_seq_tokens, int hq, int hkv, float scale_log2, float* __restrict__ out) {
-    __shared__ float wm[TREE_WARPS], wl[TREE_WARPS], wo[TREE_WARPS][HD];
-    pdl_wait();
-    pdl_trigger();
-    const int seq = blockIdx.y, i = blockIdx.x, h = blockIdx.z;
-    const int s0 = seq_starts[seq], s1 = seq_starts[seq + 1], ns = s1 - s0, L = ctx[seq];
-    if (s0 < 0 || s1 < s0 || s1 > n_tok || ns > max_seq_tokens || L < ns || L > mbs * KVB || ns > 64 * words) {
-        if (threadIdx.x == 0) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
-        return;
+struct TreeArgs {
+    const float* q;
+    int64_t n_arena_blocks;
+    int n_layer, layer;
+    const int* bt;
+    int mbs;
+    const int *starts, *ctx;
+    const int64_t* mask;
+    int words, n_tok, n_seqs, max_tok, hq, hkv, nrep;
+    float scale_log2;
+    float* out;
+    // scratch
+    float *part_o, *part_ml;     // [2 G][rows][128], [2 G][rows][2]
+    struct TreeCut* cuts;        // [G]
+    int part_rows;
+};
+
+// an item that CTA c begins and later CTAs go on with (rows = 0: none)
+struct TreeCut {
+    int64_t begin, end, T;       // units of the item; of the batch
+    int rows, s0, row0, kvh;
+};
+
+// ---- the batch's units ----
+struct TreeSeq {
+    int s0, ns, L, tiles, row_tiles;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int seq, bool report) {
+    TreeSeq s;
+    s.s0 = a.starts[seq];
+    s.ns = a.starts[seq + 1] - s.s0;
+    s.L = a.ctx[seq];
+    const bool bad = s.s0 < 0 || s.ns < 0 || s.s0 > a.n_tok - s.ns || s.ns > a.max_tok || s.L < s.ns || s.L > a.mbs * KVB;
+    if (bad) {
+        if (report) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
+        s.ns = s.L = 0;
     }
-    if (i >= ns) return;
-    const int hist = L - ns, kvh = h / (hq / hkv);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t at = ((int64_t)(s0 + i) * hq + h) * HD + 4 * lane;
-    const float4 qv = *(const float4*)(q + at);
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = warp; j < L; j += TREE_WARPS) {
-        const int t = j - hist;
-        if (t >= 0 && !((mask[(int64_t)(s0 + i) * words + t / 64] >> (t % 64)) & 1)) continue;
-        const int page = bt[(int64_t)seq * mbs + j / KVB];
-        const bool there = page >= 0 && page < n_arena_blocks;
-        if (!there) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
-        const int64_t slot = (((int64_t)page * n_layer + layer) * KVB + j % KVB) * hkv + kvh;
-        uint2 kw = make_uint2(0, 0), vw = kw;
-        if (there) {
-            kw = *(const uint2*)(karena + slot * HD + 4 * lane);
-            vw = *(const uint2*)(varena + slot * HD + 4 * lane);
-        }
-        const float2 k0 = __half22float2(*(const __half2*)&kw.x), k1 = __half22float2(*(const __half2*)&kw.y);
-        const float2 v0 = __half22float2(*(const __half2*)&vw.x), v1 = __half22float2(*(const __half2*)&vw.y);
-        float s = qv.x * k0.x + qv.y * k0.y + qv.z * k1.x + qv.w * k1.y;
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= scale_log2;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : exp2f(m - mn), p = exp2f(s - mn);
-        m = mn;
-        l = l * c + p;
-        o.x = o.x * c + p * v0.x;
-        o.y = o.y * c + p * v0.y;
-        o.z = o.z * c + p * v1.x;
-        o.w = o.w * c + p * v1.y;
-    }
-    if (lane == 0) { wm[warp] = m; wl[warp] = l; }
-    *(float4*)&wo[warp][4 * lane] = o;
-    __syncthreads();
-    if (threadIdx.x < HD) {
-        float M = -INFINITY, Ls = 0.0f, O = 0.0f;
-        for (int w = 0; w < TREE_WARPS; w++)
-            if (wl[w] != 0.0f) M = fmaxf(M, wm[w]);
-        for (int w = 0; w < TREE_WARPS; w++)
-            if (wl[w] != 0.0f) {
-                const float f = exp2f(wm[w] - M);
-                Ls += wl[w] * f;
-                O += wo[w][threadIdx.x] * f;
-            }
-        out[((int64_t)(s0 + i) * hq + h) * HD + threadIdx.x] = Ls != 0.0f ? O / Ls : 0.0f;
-    }
+    s.tiles = s.ns ? (s.L + KEYS - 1) / KEYS : 0;
+    s.row_tiles = (s.ns * a.nrep + ROWS - 1) / ROWS;
+    return s;
 }
 
-size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) { return 0; }
+// consecutive tiles of one item in a CTA's range
+struct TreeSeg {
+    int seq, kvh, rt, rows;      // rows of this row tile
+    int tile0, tiles;            // of the item's
+    TreeSeq s;
+    int64_t left;                // units of the range behind this segment
+};
+template <int ROWS>
+__device__ __forceinline__ void seg_shape(const TreeArgs& a, TreeSeg& g) {
+    g.rows = min(ROWS, g.s.ns * a.nrep - g.rt * ROWS);
+    g.tiles = (int)min((int64_t)(g.s.tiles - g.tile0), g.left);
+    g.left -= g.tiles;
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ TreeSeg seg_first(const TreeArgs& a, int seq, int64_t off, int64_t units) {
+    TreeSeg g;
+    g.seq = seq;
+    g.s = tree_seq<ROWS, KEYS>(a, seq, false);
+    const int item = (int)(off / g.s.tiles);
+    g.tile0 = (int)(off - (int64_t)item * g.s.tiles);
+    g.kvh = item / g.s.row_tiles;
+    g.rt = item - g.kvh * g.s.row_tiles;
+    g.left = units;
+    seg_shape<ROWS>(a, g);
+    return g;
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool seg_next(const TreeArgs& a, TreeSeg& g) {
+    if (g.left <= 0) return false;
+    g.tile0 = 0;
+    if (++g.rt == g.s.row_tiles) {
+        g.rt = 0;
+        if (++g.kvh == a.hkv) {
+            g.kvh = 0;
+            do g.s = tree_seq<ROWS, KEYS>(a, ++g.seq, false);
+            while (!g.s.tiles);
+        }
+    }
+    seg_shape<ROWS>(a, g);
+    return true;
+}
+
+// Sum of all units, and the sequence and offset in it of unit begin(c): every thread of the CTA calls
+// it; at[0] = sequence, at[1] = its first unit, at[2] = T (shared memory); sums: a slot per warp.
+template <int ROWS, int KEYS, int THREADS>
+__device__ void tree_locate(const TreeArgs& a, int64_t* at, int64_t* sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t T = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        int64_t run = 0;
+        const int64_t u0 = pass ? sk_begin(blockIdx.x, T, gridDim.x) : 0;
+        for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
+            const int i = i0 + threadIdx.x;
+            int64_t u = 0;
+            if (i < a.n_seqs) {
+                const TreeSeq s = tree_seq<ROWS, KEYS>(a, i, pass == 0 && blockIdx.x == 0);
+                u = (int64_t)s.tiles * s.row_tiles * a.hkv;
+            }
+            int64_t x = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) sums[warp] = x;
+            __syncthreads();
+            int64_t before = run;
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; w++) {
+                if (w < warp) before += sums[w];
+                run += sums[w];
+            }
+            if (pass && u && u0 >= before + x - u && u0 < before + x) {
+                at[0] = i;
+                at[1] = before + x - u;
+            }
+        }
+        T = run;
+    }
+    if (threadIdx.x == 0) at[2] = T;
+    __syncthreads();
+}
+
+// mask bits of keys g0 .. g0 + 31 (as positions) for drafted token `tok` (row of q): history, then draft
+__device__ __forceinline__ uint32_t tree_bits(const TreeArgs& a, const TreeSeq& s, int tok, int g0) {
+    const int hist = s.L - s.ns, t0 = g0 - hist;
+    if (t0 <= -32) return 0xFFFFFFFFu;
+    if (g0 >= s.L) return 0u;
+    const uint64_t* m = (const uint64_t*)a.mask + (int64_t)tok * a.words;
+    uint32_t v;
+    if (t0 < 0) {
+        v = (uint32_t)(m[0] << -t0) | ((1u << -t0) - 1);
+    } else {
+        const int w = t0 >> 6, b = t0 & 63;
+        v = (uint32_t)(m[w] >> b);
+        if (b > 32 && w + 1 < a.words) v |= (uint32_t)(m[w + 1] << (64 - b));
+    }
+    const int n = s.L - g0;
+    return n >= 32 ? v : v & ((1u << n) - 1);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float x0, float x1) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// x = hi + lo as fp16 halves (to 2^-21 of x): hi is x cut to 11 bits, so the rest is exact
+__device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const float h0 = __uint_as_float(__float_as_uint(x0) & 0xFFFFE000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xFFFFE000u);
+    hi = pack_h2(h0, h1);
+    lo = pack_h2(x0 - h0, x1 - h1);
+}
+
+// ------------------------------------------------------------------------------------------
+// tree_wide_kernel: tcgen05, 128 rows x 128 keys per unit.
+//   S = Q K^T: Q as two fp16 halves (hi + lo) in shared memory, each row scaled by a power of two so
+//     that its largest value lies in [1, 2); K as it is in the cache; 16 MMAs of M128 N128 K16.
+//   p = 2^(c s - m + 8), c = scale log2(e) / row scale; cut into halves that overwrite S in tensor
+//     memory: k-step j's 8 + 8 columns lie where its 16 scores were.
+//   O += P V: A from tensor memory, V as it is in the cache (MN-major), 16 MMAs.
+// Tiles alternate between two streams with an S / P buffer, an O accumulator, a running max and sum,
+// and a softmax warpgroup (thread = row) each: the tensor core works on one while the other's softmax
+// runs, and neither waits for the other's max.  m follows the true max lazily (by at most 2^4), so the
+// accumulator is rescaled a few times per item only.
+// Warps: 0 TMA producer (ring of 5 x 32 KB, K and V tiles in the order the MMAs take them; pages
+// beyond the sequence load as zeros), 1 MMA issue, 2-3 next segment's Q, 4-7 and 8-11 softmax.
+// What bounds it: HBM up to 128 rows per item (64 KB per unit: 2800 cycles of an SM's share, against
+// 32 MMAs of 64 cycles); beyond, the tensor core.
+// ------------------------------------------------------------------------------------------
+constexpr int TW_ROWS = 128;
+constexpr int TW_KEYS = 128;
+constexpr int TW_RING = 5;
+constexpr int TW_BUF = TW_KEYS * HD * 2;          // 32 KB: [half of 64 dims][128 keys][128 B]
+constexpr int TW_HALF = TW_BUF / 2;
+constexpr int TW_THREADS = 384;
+constexpr int TW_OFF_RING = 2 * TW_BUF;           // Q hi, Q lo first
+constexpr int TW_OFF_CTRL = TW_OFF_RING + TW_RING * TW_BUF;
+constexpr int TW_CTRL = 2048;
+constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL + 1024;
+constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^(8 + 4): far from fp16's ends
+constexpr float TW_LAG = 4.0f;
+
+struct TwCtrl {
+    uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_done[2], q_full, q_empty, o_free, mma_done;
+    uint64_t cleaned[2], joined[2];                // per stream: V of a tile looked over; m and l, factors ready
+    uint32_t tmem;
+    uint32_t bad[2][4];                           // per stream: keys of its tile whose V is not finite
+    int8_t qexp[4][TW_ROWS];                      // row scale exponents, by segment & 3
+    float2 xch[TW_ROWS];
+};
+static_assert(sizeof(TwCtrl) <= TW_CTRL, "control block");
+
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
+    // D f32 (bits 4-5 = 1), A and B f16 (0), B MN-major (bit 16), N >> 3 at 17-22, M >> 4 at 24-28
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        ::"r"(d), "r"(at), "l"(bd), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+}
+// MN-major operand, 128-byte swizzle: rows of 64 MN-elements, 8-row (K) atoms 1 KB apart, the next 64
+// MN-elements TW_HALF further
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(TW_HALF >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+          "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+          "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+
+// ring position of the K and V tile of the range's n-th unit of N: K0 K1 V0 K2 V1 ... K(N-1) V(N-2) V(N-1)
+__device__ __forceinline__ int64_t tw_k(int64_t n) { return n ? 2 * n - 1 : 0; }
+__device__ __forceinline__ int64_t tw_v(int64_t n, int64_t N) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; }
+
+__global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
+    const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TreeArgs a) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* ring = smem + TW_OFF_RING;
+    TwCtrl& C = *(TwCtrl*)(smem + TW_OFF_CTRL);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < TW_RING; s++) {
+            mbar_init(&C.full[s], 1);
+            mbar_init(&C.empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&C.s_full[b], 1);
+            mbar_init(&C.p_full[b], 4);
+            mbar_init(&C.o_done[b], 1);
+            mbar_init(&C.cleaned[b], 4);
+            mbar_init(&C.joined[b], 4);
+        }
+        mbar_init(&C.q_full, 2);
+        mbar_init(&C.q_empty, 1);
+        mbar_init(&C.o_free, 8);
+        mbar_init(&C.mma_done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&C.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    int64_t* at = (int64_t*)smem;                 // the Q space, before Q
+    tree_locate<TW_ROWS, TW_KEYS, TW_THREADS>(a, at, at + 4);
+    const int64_t T = at[2], u0 = sk_begin(blockIdx.x, T, gridDim.x), u1 = sk_begin(blockIdx.x + 1, T, gridDim.x);
+    const int64_t N = u1 - u0;
+    const int seq0 = N ? (int)at[0] : 0;
+    const int64_t off0 = u0 - at[1];
+    if (threadIdx.x == 0) a.cuts[blockIdx.x].rows = 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = C.tmem;
+    bool ok = true;
+
+    if (N == 0) {
+    } else if (warp == 0) {
+        // ---------------- K and V tiles ----------------
+        TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+        TreeSeg gv = g;                            // V runs one unit behind K
+        int kt = 0, vt = 0;
+        const int page = lane >> 1, half = lane & 1;   // lanes 0-15: one box each
+        const int beyond = (int)(a.n_arena_blocks * a.n_layer * KVB);
+        auto load = [&](const CUtensorMap* map, const TreeSeg& s, int tile, int64_t l) {
+            const int slot = (int)(l % TW_RING);
+            const int p = (s.tile0 + tile) * (TW_KEYS / KVB) + page;
+            int row = beyond;                      // out of the arena: zeros
+            if (lane < 16 && p * KVB < s.s.L) {
+                const int b = a.bt[(int64_t)s.seq * a.mbs + p];
+                if (b >= 0 && b < a.n_arena_blocks) row = (b * a.n_layer + a.layer) * KVB;
+                else atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
+            }
+            if (l >= TW_RING) ok = mbar_wait(&C.empty[slot], (uint32_t)((l / TW_RING - 1) & 1), &g_tree_error);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            if (lane == 0) mbar_arrive_expect_tx(&C.full[slot], TW_BUF);
+            __syncwarp();
+            if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, s.kvh, &C.full[slot]);
+        };
+        int64_t l = 0;
+        for (int64_t n = 0; n <= N && ok; n++) {
+            if (n < N) {
+                if (kt == g.tiles) {
+                    seg_next<TW_ROWS, TW_KEYS>(a, g);
+                    kt = 0;
+                }
+                load(&kmap, g, kt++, l++);
+            }
+            if (n > 0 && ok) {
+                if (vt == gv.tiles) {
+                    seg_next<TW_ROWS, TW_KEYS>(a, gv);
+                    vt = 0;
+                }
+                load(&vmap, gv, vt++, l++);
+            }
+        }
+        if (!ok)                                   // given up: the copies in flight land before the CTA ends
+            for (int64_t i = l > TW_RING ? l - TW_RING : 0; i < l; i++) mbar_wait(&C.full[i % TW_RING], (uint32_t)((i / TW_RING) & 1), &g_tree_error, 1u << 16);
+    } else if (warp == 1) {
+        // ---------------- MMA issue ----------------
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
+            const uint32_t qh = smem_u32(smem), ql = qh + TW_BUF;
+            const uint32_t rg = smem_u32(ring);
+            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            int kt = 0, seg = 0;
+            int64_t first = 0;                     // first unit of the segment
+            // O of unit n's stream (+)= P V
+            auto pv = [&](int64_t n, int64_t sfirst, int sseg) {
+                const int b = (int)(n & 1);
+                const int64_t l = tw_v(n, N);
+                const int slot = (int)(l % TW_RING);
+                ok = mbar_wait(&C.p_full[b], (uint32_t)((n >> 1) & 1), &g_tree_error) &&
+                     mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
+                const bool fresh = n - sfirst < 2;
+                if (ok && fresh && sseg) ok = mbar_wait(&C.o_free, (uint32_t)((sseg - 1) & 1), &g_tree_error);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t P = tmem + b * 128, O = tmem + 256 + b * 128, v = rg + slot * TW_BUF;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint64_t vd = umma_desc_mn128(v + j * 2048);
+                    mma_f16_ts(O, P + 16 * j, vd, id_o, fresh && j == 0 ? 0u : 1u);
+                    mma_f16_ts(O, P + 16 * j + 8, vd, id_o, 1u);
+                }
+                tc_commit(&C.empty[slot]);
+                tc_commit(&C.o_done[b]);
+            };
+            for (int64_t n = 0; n < N && ok; n++) {
+                bool begins = n == 0;
+                if (kt == g.tiles) {               // a new segment: the old one's last PV goes first
+                    pv(n - 1, first, seg);
+                    if (!ok) break;
+                    seg_next<TW_ROWS, TW_KEYS>(a, g);
+                    kt = 0;
+                    seg++;
+                    first = n;
+                    begins = true;
+                }
+                if (begins) ok = mbar_wait(&C.q_full, (uint32_t)(seg & 1), &g_tree_error);
+                const int64_t l = tw_k(n);
+                const int slot = (int)(l % TW_RING);
+                ok = ok && mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
+                if (!ok) break;
+                tc_fence_after();
+                const int b = (int)(n & 1);
+                const uint32_t S = tmem + b * 128, k = rg + slot * TW_BUF;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint32_t o = (j >> 2) * TW_HALF + (j & 3) * 32;
+                    const uint64_t kd = umma_desc_sw128(k + o);
+                    mma_f16_ss(S, umma_desc_sw128(qh + o), kd, id_s, j ? 1u : 0u);
+                    mma_f16_ss(S, umma_desc_sw128(ql + o), kd, id_s, 1u);
+                }
+                tc_commit(&C.empty[slot]);
+                tc_commit(&C.s_full[b]);
+                if (++kt == g.tiles) tc_commit(&C.q_empty);
+                if (!begins) pv(n - 1, first, seg);
+            }
+            if (ok) pv(N - 1, first, seg);
+            tc_commit(&C.mma_done);
+            mbar_wait(&C.mma_done, 0, &g_tree_error);
+        }
+    } else if (warp < 4) {
+        // ---------------- Q of each segment, as halves ----------------
+        TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+        int seg = 0;
+        do {
+            if (seg) ok = __all_sync(0xffffffffu, mbar_wait(&C.q_empty, (uint32_t)((seg - 1) & 1), &g_tree_error));
+            if (!ok) break;
+            const int r1 = min(g.rows, (warp - 1) * 64);
+            constexpr int B = 8;                   // rows in flight
+            for (int r0 = (warp - 2) * 64; r0 < r1; r0 += B) {
+                float4 x[B];
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    const int R = g.rt * TW_ROWS + min(r0 + i, r1 - 1);
+                    x[i] = *(const float4*)(a.q + ((int64_t)(g.s.s0 + R / a.nrep) * a.hq + g.kvh * a.nrep + R % a.nrep) * HD + 4 * lane);
+                }
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    if (r0 + i >= r1) break;
+                    const int r = r0 + i;
+                    float m = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    // exponent of the largest value (0 rows and subnormal ones: the least)
+                    int e = (int)(__float_as_uint(m) >> 23) - 127;
+                    e = e < -100 ? -100 : e > 120 ? 120 : e;
+                    const float f = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
+                    uint32_t h0, l0, h1, l1;
+                    cut_h2(x[i].x * f, x[i].y * f, h0, l0);
+                    cut_h2(x[i].z * f, x[i].w * f, h1, l1);
+                    // dims 4 lane .. +3: 8 bytes of 16-byte chunk (lane / 2) & 7 of its half
+                    const uint32_t o = (lane >> 4) * TW_HALF + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                    *(uint2*)(smem + o) = make_uint2(h0, h1);
+                    *(uint2*)(smem + TW_BUF + o) = make_uint2(l0, l1);
+                    if (lane == 0) C.qexp[seg & 3][r] = (int8_t)e;
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&C.q_full);
+            seg++;
+        } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
+    } else {
+        // ---------------- softmax (thread = row) and output ----------------
+        const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        const uint32_t S = lanes + wg * 128, O = lanes + 256 + wg * 128;
+        TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+        int seg = 0;
+        uint32_t cleans = 0;
+        int64_t n0 = 0;                            // the segment's first unit within the range
+        bool more;
+        do {
+            const int R = g.rt * TW_ROWS + r;
+            const bool valid = r < g.rows, live = quad * 32 < g.rows;
+            const int tok = g.s.s0 + (valid ? R / a.nrep : 0);
+            const int hist = g.s.L - g.s.ns;
+            float m = -INFINITY, l = 0.0f, c = 0.0f;
+            bool started = false, poison = false;
+            for (int t = 0; t < g.tiles && ok; t++) {
+                const int64_t n = n0 + t;
+                if ((int)(n & 1) != wg) continue;
+                const uint32_t k = (uint32_t)(n >> 1);
+                ok = __all_sync(0xffffffffu, mbar_wait(&C.s_full[wg], k & 1, &g_tree_error));
+                if (!ok) break;
+                tc_fence_after();
+                const int kb = (g.tile0 + t) * TW_KEYS;
+                uint32_t vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                const bool special = kb + TW_KEYS > hist;
+                if (special) {
+                    // V of slots past the context may be anything, and that of a drafted token that this
+                    // row does not see may be NaN: 0 x NaN is NaN, so such rows become zeros
+                    const int64_t lv = tw_v(n, N);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (uint32_t)((lv / TW_RING) & 1), &g_tree_error));
+                    if (!ok) break;
+                    uint8_t* v = ring + (lv % TW_RING) * TW_BUF + r * 128;
+                    const int key = kb + r;
+                    bool odd = false;
+                    if (key >= hist && key < g.s.L) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            const uint4 w = *(const uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16);
+                            const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                odd |= (y[i] & 0x7C00u) == 0x7C00u || (y[i] & 0x7C000000u) == 0x7C000000u;
+                        }
+                    }
+                    if (odd || key >= g.s.L) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++) *(uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+                    if (lane == 0) C.bad[wg][quad] = odds;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&C.cleaned[wg]);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
+                    if (!ok) break;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        vis[w] = valid ? tree_bits(a, g.s, tok, kb + 32 * w) : 0u;
+                        poison |= (vis[w] & C.bad[wg][w]) != 0;
+                    }
+                }
+                if (live) {
+                    if (!started) c = a.scale_log2 * __uint_as_float((uint32_t)(127 + C.qexp[seg & 3][r]) << 23);
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        uint32_t s[32];
+                        tmem_ld32(S + 32 * w, s);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const float x = c < 0.0f ? -__uint_as_float(s[i]) : __uint_as_float(s[i]);
+                            mx = fmaxf(mx, special && !((vis[w] >> i) & 1) ? -INFINITY : x);
+                        }
+                    }
+                    const float mt = mx == -INFINITY ? -INFINITY : mx * fabsf(c);
+                    if (!started) {
+                        m = mt;
+                    } else {
+                        const bool need = valid && mt > m + TW_LAG;
+                        if (__any_sync(0xffffffffu, need)) {
+                            ok = __all_sync(0xffffffffu, mbar_wait(&C.o_done[wg], (k - 1) & 1, &g_tree_error));
+                            if (!ok) break;
+                            tc_fence_after();
+                            const float f = need ? ex2(m - mt) : 1.0f;
+                            if (need) m = mt;
+                            l *= f;
+#pragma unroll
+                            for (int w = 0; w < 4; w++) {
+                                uint32_t o[32];
+                                tmem_ld32(O + 32 * w, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st32(O + 32 * w, o);
+                            }
+                        }
+                    }
+                    const float shift = TW_SHIFT - (m == -INFINITY ? 0.0f : m);
+                    float lt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        uint32_t s[32];
+                        tmem_ld32(S + 32 * w, s);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            uint32_t h[8], o[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const int e = 16 * j + 2 * i;
+                                float p0 = ex2(fmaf(__uint_as_float(s[e]), c, shift));
+                                float p1 = ex2(fmaf(__uint_as_float(s[e + 1]), c, shift));
+                                if (special) {
+                                    p0 = (vis[w] >> e) & 1 ? p0 : 0.0f;
+                                    p1 = (vis[w] >> (e + 1)) & 1 ? p1 : 0.0f;
+                                }
+                                lt[i & 3] += p0 + p1;
+                                cut_h2(p0, p1, h[i], o[i]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                s[16 * j + i] = h[i];
+                                s[16 * j + 8 + i] = o[i];
+                            }
+                        }
+                        tmem_st32(S + 32 * w, s);
+                    }
+                    l += (lt[0] + lt[1]) + (lt[2] + lt[3]);
+                    tmem_wait_st();
+                }
+                started = true;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&C.p_full[wg]);
+            }
+            if (!ok) break;
+            // ---- the segment's end: join the two streams ----
+            const int64_t n1 = n0 + g.tiles;       // last unit of each stream: n1 - 1 and n1 - 2
+            const int64_t mine = ((n1 - 1) & 1) == wg ? n1 - 1 : n1 - 2;
+            if (mine >= n0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&C.o_done[wg], (uint32_t)((mine >> 1) & 1), &g_tree_error));
+                if (!ok) break;
+            }
+            if (poison) l = NAN;
+            const bool whole = g.tile0 == 0 && g.tiles == g.s.tiles;
+            const int64_t begin = u0 + n0 - g.tile0;
+            const size_t part = (size_t)blockIdx.x * 2 + (u0 > begin ? 0 : 1);
+            tc_fence_before();
+            if (wg == 1) {
+                C.xch[r] = make_float2(m, l);
+            } else {
+                ok = __all_sync(0xffffffffu, mbar_wait(&C.joined[1], (uint32_t)(seg & 1), &g_tree_error));
+                if (!ok) break;
+                const float2 y = C.xch[r];
+                const float M = fmaxf(m, y.x);
+                float f0 = l != 0.0f ? ex2(m - M) : 0.0f, f1 = y.y != 0.0f ? ex2(y.x - M) : 0.0f;
+                const float L = l * f0 + y.y * f1;
+                if (whole) {
+                    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+                    f0 *= inv;
+                    f1 *= inv;
+                } else if (valid) {
+                    a.part_ml[(part * a.part_rows + r) * 2] = M;
+                    a.part_ml[(part * a.part_rows + r) * 2 + 1] = L;
+                }
+                C.xch[r] = make_float2(f0, f1);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&C.joined[wg]);
+            if (wg == 1) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&C.joined[0], (uint32_t)(seg & 1), &g_tree_error));
+                if (!ok) break;
+            }
+            tc_fence_after();
+            if (live) {
+                const float2 f = C.xch[r];
+                float* dst = whole ? a.out + ((int64_t)tok * a.hq + g.kvh * a.nrep + R % a.nrep) * HD
+                                   : a.part_o + (part * a.part_rows + r) * HD;
+                dst += wg * 64;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    uint32_t x[32], y[32];
+                    tmem_ld32(lanes + 256 + wg * 64 + 32 * w, x);
+                    tmem_ld32(lanes + 384 + wg * 64 + 32 * w, y);
+                    tmem_wait_ld();
+                    if (valid) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float z[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)   // a stream without a unit has left nothing to read
+                                z[e] = (f.x != 0.0f ? __uint_as_float(x[i + e]) * f.x : 0.0f) +
+                                       (f.y != 0.0f ? __uint_as_float(y[i + e]) * f.y : 0.0f);
+                            *(float4*)(dst + 32 * w + i) = make_float4(z[0], z[1], z[2], z[3]);
+                        }
+                    }
+                }
+            }
+            if (!whole && g.tile0 == 0 && threadIdx.x == 128)
+                a.cuts[blockIdx.x] = {begin, begin + g.s.tiles, T, g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh};
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&C.o_free);
+            n0 = n1;
+            seg++;
+            more = seg_next<TW_ROWS, TW_KEYS>(a, g);
+        } while (more);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    pdl_trigger();
+}
+
+// Parts of an item that several CTAs worked on: out = sum O_c 2^(m_c - M) / sum l_c 2^(m_c - M), in CTA
+// order.  One CTA per (CTA that began an item, 8 rows); a warp is a row, a lane 4 dims.
+constexpr int TC_ROWS = 8;
+__global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeArgs a, int G) {
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, r = blockIdx.y * TC_ROWS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const TreeCut cut = a.cuts[c];
+    if (r >= cut.rows) return;
+    const int last = (int)sk_owner(cut.end - 1, cut.T, G);
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int x = c; x <= last; x++) {
+        if (sk_begin(x, cut.T, G) == sk_begin(x + 1, cut.T, G)) continue;
+        const size_t part = ((size_t)x * 2 + (x == c ? 1 : 0)) * a.part_rows + r;
+        const float m = a.part_ml[part * 2], l = a.part_ml[part * 2 + 1];
+        const float4 y = *(const float4*)(a.part_o + part * HD + 4 * lane);
+        if (l == 0.0f) continue;
+        const float mn = fmaxf(M, m), f = M == -INFINITY ? 0.0f : ex2(M - mn), e = ex2(m - mn);
+        M = mn;
+        L = L * f + l * e;
+        o.x = o.x * f + y.x * e;
+        o.y = o.y * f + y.y * e;
+        o.z = o.z * f + y.z * e;
+        o.w = o.w * f + y.w * e;
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    const int R = cut.row0 + r;
+    float* dst = a.out + ((int64_t)(cut.s0 + R / a.nrep) * a.hq + cut.kvh * a.nrep + R % a.nrep) * HD + 4 * lane;
+    *(float4*)dst = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // qmm.cu
+
+// arena as (64 dims of a half, slot, half, kv head); one box: 16 slots of one half
+static cudaError_t tree_map(CUtensorMap* map, const void* arena, int hkv, int64_t n_slots) {
+    auto fn = encode_fn();
+    if (!fn) return cudaErrorNotSupported;
+    const cuuint64_t dims[4] = {64u, (cuuint64_t)n_slots, 2u, (cuuint64_t)hkv};
+    const cuuint64_t strides[3] = {(cuuint64_t)hkv * HD * 2, 128u, (cuuint64_t)HD * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)KVB, 1, 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(arena), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+struct TreePlan {
+    int G, rows;
+    size_t o_bytes, ml_bytes, bytes;
+};
+static TreePlan tree_plan(int hq, int hkv, int max_seq_tokens) {
+    TreePlan p;
+    p.G = num_sms();
+    const int64_t rows = (int64_t)max_seq_tokens * (hq / hkv);
+    p.rows = (int)(rows < TW_ROWS ? rows : TW_ROWS);
+    p.o_bytes = align256((size_t)2 * p.G * p.rows * HD * 4);
+    p.ml_bytes = align256((size_t)2 * p.G * p.rows * 2 * 4);
+    p.bytes = p.o_bytes + p.ml_bytes + align256((size_t)p.G * sizeof(TreeCut));
+    return p;
+}
+size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
+    return tree_plan(hq, hkv, max_seq_tokens).bytes;
+}
 
 cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const void* varena, int64_t n_arena_blocks,
                                    int n_layer, int layer, const int* bt, int mbs, const int* seq_starts,
                                    const int* ctx, const int64_t* mask, int words, int n_tok, int n_seqs,
                                    int max_seq_tokens, int hq, int hkv, int max_ctx, float scale, float* out,
                                    void* scratch, cudaStream_t st) {
-    return launch_pdl(tree_simple_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs, (unsigned)hq),
-                      dim3(TREE_WARPS * 32), 0, st, q, (const __half*)karena, (const __half*)varena, n_arena_blocks,
-                      n_layer, layer, bt, mbs, seq_starts, ctx, mask, words, n_tok, max_seq_tokens, hq, hkv,
-                      scale * LOG2E, out);
+    const TreePlan p = tree_plan(hq, hkv, max_seq_tokens);
+    TreeArgs a;
+    a.q = q;
+    a.n_arena_blocks = n_arena_blocks;
+    a.n_layer = n_layer; a.layer = layer; a.bt = bt; a.mbs = mbs; a.starts = seq_starts; a.ctx = ctx;
+    a.mask = mask; a.words = words; a.n_tok = n_tok; a.n_seqs = n_seqs; a.max_tok = max_seq_tokens;
+    a.hq = hq; a.hkv = hkv; a.nrep = hq / hkv;
+    a.scale_log2 = scale * LOG2E;
+    a.out = out;
+    a.part_o = (float*)scratch;
+    a.part_ml = (float*)((uint8_t*)scratch + p.o_bytes);
+    a.cuts = (TreeCut*)((uint8_t*)scratch + p.o_bytes + p.ml_bytes);
+    a.part_rows = p.rows;
+    CUtensorMap km, vm;
+    const int64_t n_slots = n_arena_blocks * n_layer * KVB;
+    cudaError_t e = tree_map(&km, karena, hkv, n_slots);
+    if (e == cudaSuccess) e = tree_map(&vm, varena, hkv, n_slots);
+    if (e == cudaSuccess) e = DCG_SMEM_ATTR(tree_wide_kernel, TW_SMEM);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(tree_wide_kernel, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(tree_combine_kernel, dim3((unsigned)p.G, (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
+                      dim3(TC_ROWS * 32), 0, st, a, p.G);
 }
 
 }  // namespace dcg
