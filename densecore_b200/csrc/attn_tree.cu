@@ -43,7 +43,7 @@ struct TreeArgs {
     int mbs;
     const int *starts, *ctx;
     const int64_t* mask;
-    int words, n_tok, n_seqs, max_tok, hq, hkv, nrep;
+    int words, n_tok, n_seqs, max_tok, max_ctx, hq, hkv, nrep;
     float scale_log2;
     float* out;
     // scratch
@@ -68,7 +68,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int seq, bool rep
     s.s0 = a.starts[seq];
     s.ns = a.starts[seq + 1] - s.s0;
     s.L = a.ctx[seq];
-    const bool bad = s.s0 < 0 || s.ns < 0 || s.s0 > a.n_tok - s.ns || s.ns > a.max_tok || s.L < s.ns || s.L > a.mbs * KVB;
+    const bool bad = s.s0 < 0 || s.ns < 0 || s.s0 > a.n_tok - s.ns || s.ns > a.max_tok || s.L < s.ns || s.L > a.max_ctx;
     if (bad) {
         if (report) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
         s.ns = s.L = 0;
@@ -82,9 +82,13 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int seq, bool rep
 struct TreeSeg {
     int seq, kvh, rt, rows;      // rows of this row tile
     int tile0, tiles;            // of the item's
-    TreeSeq s;
+    TreeSeq s, next;             // next: of sequence seq + 1, its loads on the way meanwhile
     int64_t left;                // units of the range behind this segment
 };
+template <int ROWS, int KEYS>
+__device__ __forceinline__ TreeSeq seq_or_none(const TreeArgs& a, int seq) {
+    return seq < a.n_seqs ? tree_seq<ROWS, KEYS>(a, seq, false) : TreeSeq{0, 0, 0, 0, 0};
+}
 template <int ROWS>
 __device__ __forceinline__ void seg_shape(const TreeArgs& a, TreeSeg& g) {
     g.rows = min(ROWS, g.s.ns * a.nrep - g.rt * ROWS);
@@ -92,12 +96,13 @@ __device__ __forceinline__ void seg_shape(const TreeArgs& a, TreeSeg& g) {
     g.left -= g.tiles;
 }
 template <int ROWS, int KEYS>
-__device__ __forceinline__ TreeSeg seg_first(const TreeArgs& a, int seq, int64_t off, int64_t units) {
+__device__ __forceinline__ TreeSeg seg_first(const TreeArgs& a, int seq, int off, int64_t units) {
     TreeSeg g;
     g.seq = seq;
     g.s = tree_seq<ROWS, KEYS>(a, seq, false);
-    const int item = (int)(off / g.s.tiles);
-    g.tile0 = (int)(off - (int64_t)item * g.s.tiles);
+    g.next = seq_or_none<ROWS, KEYS>(a, seq + 1);
+    const int item = off / g.s.tiles;
+    g.tile0 = off - item * g.s.tiles;
     g.kvh = item / g.s.row_tiles;
     g.rt = item - g.kvh * g.s.row_tiles;
     g.left = units;
@@ -112,8 +117,10 @@ __device__ __forceinline__ bool seg_next(const TreeArgs& a, TreeSeg& g) {
         g.rt = 0;
         if (++g.kvh == a.hkv) {
             g.kvh = 0;
-            do g.s = tree_seq<ROWS, KEYS>(a, ++g.seq, false);
-            while (!g.s.tiles);
+            do {
+                g.s = g.next;
+                g.next = seq_or_none<ROWS, KEYS>(a, ++g.seq + 1);
+            } while (!g.s.tiles);   // ends: units are left
         }
     }
     seg_shape<ROWS>(a, g);
@@ -128,7 +135,6 @@ __device__ void tree_locate(const TreeArgs& a, int64_t* at, int64_t* sums) {
     int64_t T = 0;
     for (int pass = 0; pass < 2; pass++) {
         int64_t run = 0;
-        const int64_t u0 = pass ? sk_begin(blockIdx.x, T, gridDim.x) : 0;
         for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
             const int i = i0 + threadIdx.x;
             int64_t u = 0;
@@ -151,12 +157,16 @@ __device__ void tree_locate(const TreeArgs& a, int64_t* at, int64_t* sums) {
                 if (w < warp) before += sums[w];
                 run += sums[w];
             }
-            if (pass && u && u0 >= before + x - u && u0 < before + x) {
-                at[0] = i;
-                at[1] = before + x - u;
+            if (pass || a.n_seqs <= THREADS) {     // a batch that fits one step needs no second pass
+                const int64_t u0 = sk_begin(blockIdx.x, pass ? T : run, gridDim.x);
+                if (u && u0 >= before + x - u && u0 < before + x) {
+                    at[0] = i;
+                    at[1] = before + x - u;
+                }
             }
         }
         T = run;
+        if (a.n_seqs <= THREADS) break;
     }
     if (threadIdx.x == 0) at[2] = T;
     __syncthreads();
@@ -200,15 +210,17 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // tree_wide_kernel: tcgen05, 128 rows x 128 keys per unit.
 //   S = Q K^T: Q as two fp16 halves (hi + lo) in shared memory, each row scaled by a power of two so
 //     that its largest value lies in [1, 2); K as it is in the cache; 16 MMAs of M128 N128 K16.
-//   p = 2^(c s - m + 8), c = scale log2(e) / row scale; cut into halves that overwrite S in tensor
-//     memory: k-step j's 8 + 8 columns lie where its 16 scores were.
-//   O += P V: A from tensor memory, V as it is in the cache (MN-major), 16 MMAs.
-// Tiles alternate between two streams with an S / P buffer, an O accumulator, a running max and sum,
-// and a softmax warpgroup (thread = row) each: the tensor core works on one while the other's softmax
-// runs, and neither waits for the other's max.  m follows the true max lazily (by at most 2^4), so the
-// accumulator is rescaled a few times per item only.
-// Warps: 0 TMA producer (ring of 5 x 32 KB, K and V tiles in the order the MMAs take them; pages
-// beyond the sequence load as zeros), 1 MMA issue, 2-3 next segment's Q, 4-7 and 8-11 softmax.
+//   p = 2^(c s - m + 8), c = scale log2(e) / row scale, m the tile's own row max; cut into halves that
+//     overwrite S in tensor memory: k-step j's 8 + 8 columns lie where its 16 scores were.
+//   O = P V of this tile alone: A from tensor memory, V as it is in the cache (MN-major), 16 MMAs.
+//   The tiles' O, m and sum of p are joined in registers, in fp32 rounded to nearest.
+// The tensor core cuts its sums off rather than rounding them, a bias of up to 2^-24 for each MMA that
+// adds to a large accumulator: hence the lo halves first, and no accumulator that lives for longer
+// than a tile (one that lived for a segment was 2-4 x 10^-6 off, this is 4-6 x 10^-7).
+// Two S / P and two O buffers, used in turn.  Warps: 0 TMA producer (ring of 5 x 32 KB, K and V tiles
+// in the order the MMAs take them; pages beyond the sequence load as zeros), 1 MMA issue, 2-3 the next
+// segment's Q, 4-7 and 8-11 softmax of every other tile, 12-15 the running output (128 registers of
+// it per thread, thread = row).
 // What bounds it: HBM up to 128 rows per item (64 KB per unit: 2800 cycles of an SM's share, against
 // 32 MMAs of 64 cycles); beyond, the tensor core.
 // ------------------------------------------------------------------------------------------
@@ -217,21 +229,23 @@ constexpr int TW_KEYS = 128;
 constexpr int TW_RING = 5;
 constexpr int TW_BUF = TW_KEYS * HD * 2;          // 32 KB: [half of 64 dims][128 keys][128 B]
 constexpr int TW_HALF = TW_BUF / 2;
-constexpr int TW_THREADS = 384;
+constexpr int TW_THREADS = 512;
 constexpr int TW_OFF_RING = 2 * TW_BUF;           // Q hi, Q lo first
 constexpr int TW_OFF_CTRL = TW_OFF_RING + TW_RING * TW_BUF;
-constexpr int TW_CTRL = 2048;
-constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL + 1024;
-constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^(8 + 4): far from fp16's ends
-constexpr float TW_LAG = 4.0f;
+constexpr int TW_CTRL = 3072;
+constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // all of it: 227 KB
+constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^8: the small ones stay above fp16's least
+// registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128
+constexpr int TW_REGS_CTRL = 104, TW_REGS_SOFT = 104, TW_REGS_OUT = 200;
+static_assert(TW_REGS_CTRL + 2 * TW_REGS_SOFT + TW_REGS_OUT <= 512, "register split");
 
 struct TwCtrl {
-    uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_done[2], q_full, q_empty, o_free, mma_done;
-    uint64_t cleaned[2], joined[2];                // per stream: V of a tile looked over; m and l, factors ready
+    uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_full[2], o_free[2], x_free[2], cleaned[2];
+    uint64_t q_full, q_empty, mma_done;
     uint32_t tmem;
-    uint32_t bad[2][4];                           // per stream: keys of its tile whose V is not finite
+    uint32_t bad[2][4];                           // per buffer: keys of its tile whose V is not finite
     int8_t qexp[4][TW_ROWS];                      // row scale exponents, by segment & 3
-    float2 xch[TW_ROWS];
+    float2 x[2][TW_ROWS];                         // a tile's row max and sum of p
 };
 static_assert(sizeof(TwCtrl) <= TW_CTRL, "control block");
 
@@ -283,13 +297,69 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 __device__ __forceinline__ int64_t tw_k(int64_t n) { return n ? 2 * n - 1 : 0; }
 __device__ __forceinline__ int64_t tw_v(int64_t n, int64_t N) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; }
 
+// two fp32 operations at a time
+__device__ __forceinline__ uint64_t pack2(float x0, float x1) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x0), "f"(x1));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& x0, float& x1) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// Q of a segment as halves: a warp takes every other group of B rows; o: swizzled K-major tiles
+template <int B>
+__device__ __forceinline__ void tw_load_q(const TreeArgs& a, const TreeSeg& g, int r0, float4 (&x)[B]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < B; i++) {
+        const int R = g.rt * TW_ROWS + min(r0 + i, g.rows - 1);
+        x[i] = *(const float4*)(a.q + ((int64_t)(g.s.s0 + R / a.nrep) * a.hq + g.kvh * a.nrep + R % a.nrep) * HD + 4 * lane);
+    }
+}
+template <int B>
+__device__ __forceinline__ void tw_store_q(uint8_t* smem, int8_t* qexp, int rows, int r0, const float4 (&x)[B]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < B; i++) {
+        if (r0 + i >= rows) break;
+        const int r = r0 + i;
+        float m = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // exponent of the largest value (0 rows and subnormal ones: the least)
+        int e = (int)(__float_as_uint(m) >> 23) - 127;
+        e = e < -100 ? -100 : e > 120 ? 120 : e;
+        const float f = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
+        uint32_t h0, l0, h1, l1;
+        cut_h2(x[i].x * f, x[i].y * f, h0, l0);
+        cut_h2(x[i].z * f, x[i].w * f, h1, l1);
+        // dims 4 lane .. +3: 8 bytes of 16-byte chunk (lane / 2) & 7 of its half
+        const uint32_t o = (lane >> 4) * TW_HALF + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
+        *(uint2*)(smem + o) = make_uint2(h0, h1);
+        *(uint2*)(smem + TW_BUF + o) = make_uint2(l0, l1);
+        if (lane == 0) qexp[r] = (int8_t)e;
+    }
+}
+
 __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TreeArgs a) {
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t smem[];   // no static shared memory: starts on a KB
     uint8_t* ring = smem + TW_OFF_RING;
     TwCtrl& C = *(TwCtrl*)(smem + TW_OFF_CTRL);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (smem_u32(smem) & 1023) {                  // the swizzled tiles would not match their descriptors
+        if (threadIdx.x == 0) atomicExch(&g_tree_error, DCG_DEVERR_TIMEOUT);
+        return;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < TW_RING; s++) {
@@ -299,13 +369,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         for (int b = 0; b < 2; b++) {
             mbar_init(&C.s_full[b], 1);
             mbar_init(&C.p_full[b], 4);
-            mbar_init(&C.o_done[b], 1);
+            mbar_init(&C.o_full[b], 1);
+            mbar_init(&C.o_free[b], 4);
+            mbar_init(&C.x_free[b], 4);
             mbar_init(&C.cleaned[b], 4);
-            mbar_init(&C.joined[b], 4);
         }
         mbar_init(&C.q_full, 2);
         mbar_init(&C.q_empty, 1);
-        mbar_init(&C.o_free, 8);
         mbar_init(&C.mma_done, 1);
         fence_mbar_init();
     }
@@ -318,8 +388,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     tree_locate<TW_ROWS, TW_KEYS, TW_THREADS>(a, at, at + 4);
     const int64_t T = at[2], u0 = sk_begin(blockIdx.x, T, gridDim.x), u1 = sk_begin(blockIdx.x + 1, T, gridDim.x);
     const int64_t N = u1 - u0;
-    const int seq0 = N ? (int)at[0] : 0;
-    const int64_t off0 = u0 - at[1];
+    const int seq0 = N ? (int)at[0] : 0, off0 = N ? (int)(u0 - at[1]) : 0;
     if (threadIdx.x == 0) a.cuts[blockIdx.x].rows = 0;
     tc_fence_before();
     __syncthreads();
@@ -327,366 +396,366 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     const uint32_t tmem = C.tmem;
     bool ok = true;
 
-    if (N == 0) {
-    } else if (warp == 0) {
-        // ---------------- K and V tiles ----------------
-        TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-        TreeSeg gv = g;                            // V runs one unit behind K
-        int kt = 0, vt = 0;
-        const int page = lane >> 1, half = lane & 1;   // lanes 0-15: one box each
-        const int beyond = (int)(a.n_arena_blocks * a.n_layer * KVB);
-        auto load = [&](const CUtensorMap* map, const TreeSeg& s, int tile, int64_t l) {
-            const int slot = (int)(l % TW_RING);
-            const int p = (s.tile0 + tile) * (TW_KEYS / KVB) + page;
-            int row = beyond;                      // out of the arena: zeros
-            if (lane < 16 && p * KVB < s.s.L) {
-                const int b = a.bt[(int64_t)s.seq * a.mbs + p];
-                if (b >= 0 && b < a.n_arena_blocks) row = (b * a.n_layer + a.layer) * KVB;
-                else atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
-            }
-            if (l >= TW_RING) ok = mbar_wait(&C.empty[slot], (uint32_t)((l / TW_RING - 1) & 1), &g_tree_error);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
-            if (lane == 0) mbar_arrive_expect_tx(&C.full[slot], TW_BUF);
-            __syncwarp();
-            if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, s.kvh, &C.full[slot]);
-        };
-        int64_t l = 0;
-        for (int64_t n = 0; n <= N && ok; n++) {
-            if (n < N) {
-                if (kt == g.tiles) {
-                    seg_next<TW_ROWS, TW_KEYS>(a, g);
-                    kt = 0;
-                }
-                load(&kmap, g, kt++, l++);
-            }
-            if (n > 0 && ok) {
-                if (vt == gv.tiles) {
-                    seg_next<TW_ROWS, TW_KEYS>(a, gv);
-                    vt = 0;
-                }
-                load(&vmap, gv, vt++, l++);
-            }
-        }
-        if (!ok)                                   // given up: the copies in flight land before the CTA ends
-            for (int64_t i = l > TW_RING ? l - TW_RING : 0; i < l; i++) mbar_wait(&C.full[i % TW_RING], (uint32_t)((i / TW_RING) & 1), &g_tree_error, 1u << 16);
-    } else if (warp == 1) {
-        // ---------------- MMA issue ----------------
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
-            const uint32_t qh = smem_u32(smem), ql = qh + TW_BUF;
-            const uint32_t rg = smem_u32(ring);
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_CTRL));
+        if (N == 0) {
+        } else if (warp == 0) {
+            // ---------------- K and V tiles ----------------
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-            int kt = 0, seg = 0;
-            int64_t first = 0;                     // first unit of the segment
-            // O of unit n's stream (+)= P V
-            auto pv = [&](int64_t n, int64_t sfirst, int sseg) {
-                const int b = (int)(n & 1);
-                const int64_t l = tw_v(n, N);
-                const int slot = (int)(l % TW_RING);
-                ok = mbar_wait(&C.p_full[b], (uint32_t)((n >> 1) & 1), &g_tree_error) &&
-                     mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
-                const bool fresh = n - sfirst < 2;
-                if (ok && fresh && sseg) ok = mbar_wait(&C.o_free, (uint32_t)((sseg - 1) & 1), &g_tree_error);
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t P = tmem + b * 128, O = tmem + 256 + b * 128, v = rg + slot * TW_BUF;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint64_t vd = umma_desc_mn128(v + j * 2048);
-                    mma_f16_ts(O, P + 16 * j, vd, id_o, fresh && j == 0 ? 0u : 1u);
-                    mma_f16_ts(O, P + 16 * j + 8, vd, id_o, 1u);
-                }
-                tc_commit(&C.empty[slot]);
-                tc_commit(&C.o_done[b]);
+            const int page = lane >> 1, half = lane & 1;   // lanes 0-15: one box each
+            const int beyond = (int)(a.n_arena_blocks * a.n_layer * KVB);   // out of the arena: zeros
+            int kt = 0;
+            // block id of this lane's page in a tile, -1 behind the sequence's end (no read)
+            auto block = [&](const TreeSeg& s, int tile) {
+                const int p = (s.tile0 + tile) * (TW_KEYS / KVB) + page;
+                return lane < 16 && p * KVB < s.s.L ? a.bt[(int64_t)s.seq * a.mbs + p] : INT32_MIN;
             };
-            for (int64_t n = 0; n < N && ok; n++) {
-                bool begins = n == 0;
-                if (kt == g.tiles) {               // a new segment: the old one's last PV goes first
-                    pv(n - 1, first, seg);
-                    if (!ok) break;
-                    seg_next<TW_ROWS, TW_KEYS>(a, g);
-                    kt = 0;
-                    seg++;
-                    first = n;
-                    begins = true;
-                }
-                if (begins) ok = mbar_wait(&C.q_full, (uint32_t)(seg & 1), &g_tree_error);
-                const int64_t l = tw_k(n);
+            auto load = [&](const CUtensorMap* map, int kvh, int b, int64_t l) {
                 const int slot = (int)(l % TW_RING);
-                ok = ok && mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
-                if (!ok) break;
-                tc_fence_after();
-                const int b = (int)(n & 1);
-                const uint32_t S = tmem + b * 128, k = rg + slot * TW_BUF;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint32_t o = (j >> 2) * TW_HALF + (j & 3) * 32;
-                    const uint64_t kd = umma_desc_sw128(k + o);
-                    mma_f16_ss(S, umma_desc_sw128(qh + o), kd, id_s, j ? 1u : 0u);
-                    mma_f16_ss(S, umma_desc_sw128(ql + o), kd, id_s, 1u);
-                }
-                tc_commit(&C.empty[slot]);
-                tc_commit(&C.s_full[b]);
-                if (++kt == g.tiles) tc_commit(&C.q_empty);
-                if (!begins) pv(n - 1, first, seg);
-            }
-            if (ok) pv(N - 1, first, seg);
-            tc_commit(&C.mma_done);
-            mbar_wait(&C.mma_done, 0, &g_tree_error);
-        }
-    } else if (warp < 4) {
-        // ---------------- Q of each segment, as halves ----------------
-        TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-        int seg = 0;
-        do {
-            if (seg) ok = __all_sync(0xffffffffu, mbar_wait(&C.q_empty, (uint32_t)((seg - 1) & 1), &g_tree_error));
-            if (!ok) break;
-            const int r1 = min(g.rows, (warp - 1) * 64);
-            constexpr int B = 8;                   // rows in flight
-            for (int r0 = (warp - 2) * 64; r0 < r1; r0 += B) {
-                float4 x[B];
-#pragma unroll
-                for (int i = 0; i < B; i++) {
-                    const int R = g.rt * TW_ROWS + min(r0 + i, r1 - 1);
-                    x[i] = *(const float4*)(a.q + ((int64_t)(g.s.s0 + R / a.nrep) * a.hq + g.kvh * a.nrep + R % a.nrep) * HD + 4 * lane);
-                }
-#pragma unroll
-                for (int i = 0; i < B; i++) {
-                    if (r0 + i >= r1) break;
-                    const int r = r0 + i;
-                    float m = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    // exponent of the largest value (0 rows and subnormal ones: the least)
-                    int e = (int)(__float_as_uint(m) >> 23) - 127;
-                    e = e < -100 ? -100 : e > 120 ? 120 : e;
-                    const float f = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
-                    uint32_t h0, l0, h1, l1;
-                    cut_h2(x[i].x * f, x[i].y * f, h0, l0);
-                    cut_h2(x[i].z * f, x[i].w * f, h1, l1);
-                    // dims 4 lane .. +3: 8 bytes of 16-byte chunk (lane / 2) & 7 of its half
-                    const uint32_t o = (lane >> 4) * TW_HALF + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
-                    *(uint2*)(smem + o) = make_uint2(h0, h1);
-                    *(uint2*)(smem + TW_BUF + o) = make_uint2(l0, l1);
-                    if (lane == 0) C.qexp[seg & 3][r] = (int8_t)e;
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&C.q_full);
-            seg++;
-        } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
-    } else {
-        // ---------------- softmax (thread = row) and output ----------------
-        const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
-        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-        const uint32_t S = lanes + wg * 128, O = lanes + 256 + wg * 128;
-        TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-        int seg = 0;
-        uint32_t cleans = 0;
-        int64_t n0 = 0;                            // the segment's first unit within the range
-        bool more;
-        do {
-            const int R = g.rt * TW_ROWS + r;
-            const bool valid = r < g.rows, live = quad * 32 < g.rows;
-            const int tok = g.s.s0 + (valid ? R / a.nrep : 0);
-            const int hist = g.s.L - g.s.ns;
-            float m = -INFINITY, l = 0.0f, c = 0.0f;
-            bool started = false, poison = false;
-            for (int t = 0; t < g.tiles && ok; t++) {
-                const int64_t n = n0 + t;
-                if ((int)(n & 1) != wg) continue;
-                const uint32_t k = (uint32_t)(n >> 1);
-                ok = __all_sync(0xffffffffu, mbar_wait(&C.s_full[wg], k & 1, &g_tree_error));
-                if (!ok) break;
-                tc_fence_after();
-                const int kb = (g.tile0 + t) * TW_KEYS;
-                uint32_t vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
-                const bool special = kb + TW_KEYS > hist;
-                if (special) {
-                    // V of slots past the context may be anything, and that of a drafted token that this
-                    // row does not see may be NaN: 0 x NaN is NaN, so such rows become zeros
-                    const int64_t lv = tw_v(n, N);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (uint32_t)((lv / TW_RING) & 1), &g_tree_error));
-                    if (!ok) break;
-                    uint8_t* v = ring + (lv % TW_RING) * TW_BUF + r * 128;
-                    const int key = kb + r;
-                    bool odd = false;
-                    if (key >= hist && key < g.s.L) {
-#pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            const uint4 w = *(const uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16);
-                            const uint32_t y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                odd |= (y[i] & 0x7C00u) == 0x7C00u || (y[i] & 0x7C000000u) == 0x7C000000u;
-                        }
-                    }
-                    if (odd || key >= g.s.L) {
-#pragma unroll
-                        for (int x = 0; x < 16; x++) *(uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-                    if (lane == 0) C.bad[wg][quad] = odds;
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&C.cleaned[wg]);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
-                    if (!ok) break;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        vis[w] = valid ? tree_bits(a, g.s, tok, kb + 32 * w) : 0u;
-                        poison |= (vis[w] & C.bad[wg][w]) != 0;
-                    }
-                }
-                if (live) {
-                    if (!started) c = a.scale_log2 * __uint_as_float((uint32_t)(127 + C.qexp[seg & 3][r]) << 23);
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t s[32];
-                        tmem_ld32(S + 32 * w, s);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const float x = c < 0.0f ? -__uint_as_float(s[i]) : __uint_as_float(s[i]);
-                            mx = fmaxf(mx, special && !((vis[w] >> i) & 1) ? -INFINITY : x);
-                        }
-                    }
-                    const float mt = mx == -INFINITY ? -INFINITY : mx * fabsf(c);
-                    if (!started) {
-                        m = mt;
-                    } else {
-                        const bool need = valid && mt > m + TW_LAG;
-                        if (__any_sync(0xffffffffu, need)) {
-                            ok = __all_sync(0xffffffffu, mbar_wait(&C.o_done[wg], (k - 1) & 1, &g_tree_error));
-                            if (!ok) break;
-                            tc_fence_after();
-                            const float f = need ? ex2(m - mt) : 1.0f;
-                            if (need) m = mt;
-                            l *= f;
-#pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                uint32_t o[32];
-                                tmem_ld32(O + 32 * w, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tmem_st32(O + 32 * w, o);
-                            }
-                        }
-                    }
-                    const float shift = TW_SHIFT - (m == -INFINITY ? 0.0f : m);
-                    float lt[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t s[32];
-                        tmem_ld32(S + 32 * w, s);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            uint32_t h[8], o[8];
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const int e = 16 * j + 2 * i;
-                                float p0 = ex2(fmaf(__uint_as_float(s[e]), c, shift));
-                                float p1 = ex2(fmaf(__uint_as_float(s[e + 1]), c, shift));
-                                if (special) {
-                                    p0 = (vis[w] >> e) & 1 ? p0 : 0.0f;
-                                    p1 = (vis[w] >> (e + 1)) & 1 ? p1 : 0.0f;
-                                }
-                                lt[i & 3] += p0 + p1;
-                                cut_h2(p0, p1, h[i], o[i]);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                s[16 * j + i] = h[i];
-                                s[16 * j + 8 + i] = o[i];
-                            }
-                        }
-                        tmem_st32(S + 32 * w, s);
-                    }
-                    l += (lt[0] + lt[1]) + (lt[2] + lt[3]);
-                    tmem_wait_st();
-                }
-                started = true;
-                tc_fence_before();
+                if (l >= TW_RING) ok = mbar_wait(&C.empty[slot], (uint32_t)((l / TW_RING - 1) & 1), &g_tree_error);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                const bool in = b >= 0 && b < a.n_arena_blocks;
+                if (!in && b != INT32_MIN) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
+                const int row = in ? (b * a.n_layer + a.layer) * KVB : beyond;
+                if (lane == 0) mbar_arrive_expect_tx(&C.full[slot], TW_BUF);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&C.p_full[wg]);
-            }
-            if (!ok) break;
-            // ---- the segment's end: join the two streams ----
-            const int64_t n1 = n0 + g.tiles;       // last unit of each stream: n1 - 1 and n1 - 2
-            const int64_t mine = ((n1 - 1) & 1) == wg ? n1 - 1 : n1 - 2;
-            if (mine >= n0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&C.o_done[wg], (uint32_t)((mine >> 1) & 1), &g_tree_error));
-                if (!ok) break;
-            }
-            if (poison) l = NAN;
-            const bool whole = g.tile0 == 0 && g.tiles == g.s.tiles;
-            const int64_t begin = u0 + n0 - g.tile0;
-            const size_t part = (size_t)blockIdx.x * 2 + (u0 > begin ? 0 : 1);
-            tc_fence_before();
-            if (wg == 1) {
-                C.xch[r] = make_float2(m, l);
-            } else {
-                ok = __all_sync(0xffffffffu, mbar_wait(&C.joined[1], (uint32_t)(seg & 1), &g_tree_error));
-                if (!ok) break;
-                const float2 y = C.xch[r];
-                const float M = fmaxf(m, y.x);
-                float f0 = l != 0.0f ? ex2(m - M) : 0.0f, f1 = y.y != 0.0f ? ex2(y.x - M) : 0.0f;
-                const float L = l * f0 + y.y * f1;
-                if (whole) {
-                    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-                    f0 *= inv;
-                    f1 *= inv;
-                } else if (valid) {
-                    a.part_ml[(part * a.part_rows + r) * 2] = M;
-                    a.part_ml[(part * a.part_rows + r) * 2 + 1] = L;
-                }
-                C.xch[r] = make_float2(f0, f1);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&C.joined[wg]);
-            if (wg == 1) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&C.joined[0], (uint32_t)(seg & 1), &g_tree_error));
-                if (!ok) break;
-            }
-            tc_fence_after();
-            if (live) {
-                const float2 f = C.xch[r];
-                float* dst = whole ? a.out + ((int64_t)tok * a.hq + g.kvh * a.nrep + R % a.nrep) * HD
-                                   : a.part_o + (part * a.part_rows + r) * HD;
-                dst += wg * 64;
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    uint32_t x[32], y[32];
-                    tmem_ld32(lanes + 256 + wg * 64 + 32 * w, x);
-                    tmem_ld32(lanes + 384 + wg * 64 + 32 * w, y);
-                    tmem_wait_ld();
-                    if (valid) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float z[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++)   // a stream without a unit has left nothing to read
-                                z[e] = (f.x != 0.0f ? __uint_as_float(x[i + e]) * f.x : 0.0f) +
-                                       (f.y != 0.0f ? __uint_as_float(y[i + e]) * f.y : 0.0f);
-                            *(float4*)(dst + 32 * w + i) = make_float4(z[0], z[1], z[2], z[3]);
-                        }
+                if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, kvh, &C.full[slot]);
+            };
+            int64_t l = 0;
+            int b_now = block(g, 0), h_now = g.kvh, b_last = 0, h_last = 0;
+            for (int64_t n = 0; n <= N && ok; n++) {       // V runs one unit behind K
+                int b_next = 0, h_next = 0;
+                if (n < N) {
+                    load(&kmap, h_now, b_now, l++);
+                    if (++kt == g.tiles) {
+                        kt = 0;
+                        if (n + 1 < N) seg_next<TW_ROWS, TW_KEYS>(a, g);
+                    }
+                    if (n + 1 < N) {                       // on its way while the ring is waited for
+                        b_next = block(g, kt);
+                        h_next = g.kvh;
                     }
                 }
+                if (n > 0 && ok) load(&vmap, h_last, b_last, l++);
+                b_last = b_now;
+                h_last = h_now;
+                b_now = b_next;
+                h_now = h_next;
             }
-            if (!whole && g.tile0 == 0 && threadIdx.x == 128)
-                a.cuts[blockIdx.x] = {begin, begin + g.s.tiles, T, g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh};
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&C.o_free);
-            n0 = n1;
-            seg++;
-            more = seg_next<TW_ROWS, TW_KEYS>(a, g);
-        } while (more);
+            if (!ok)                               // given up: the copies in flight land before the CTA ends
+                for (int64_t i = l > TW_RING ? l - TW_RING : 0; i < l; i++) mbar_wait(&C.full[i % TW_RING], (uint32_t)((i / TW_RING) & 1), &g_tree_error, 1u << 16);
+        } else if (warp == 1) {
+            // ---------------- MMA issue ----------------
+            if (lane == 0) {
+                constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
+                const uint32_t qh = smem_u32(smem), ql = qh + TW_BUF;
+                const uint32_t rg = smem_u32(ring);
+                TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+                int kt = 0, seg = 0;
+                auto pv = [&](int64_t n) {         // O of unit n = P V
+                    const int b = (int)(n & 1);
+                    const uint32_t k = (uint32_t)(n >> 1);
+                    const int64_t l = tw_v(n, N);
+                    const int slot = (int)(l % TW_RING);
+                    ok = mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
+                    if (ok && k) ok = mbar_wait(&C.o_free[b], (k - 1) & 1, &g_tree_error);
+                    if (ok) ok = mbar_wait(&C.p_full[b], k & 1, &g_tree_error);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t P = tmem + b * 128, O = tmem + 256 + b * 128;
+                    const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
+#pragma unroll
+                    for (int h = 1; h >= 0; h--)   // the lo halves first; 16 keys = 2048 bytes per k-step
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            mma_f16_ts(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o, h && j == 0 ? 0u : 1u);
+                    tc_commit(&C.empty[slot]);
+                    tc_commit(&C.o_full[b]);
+                };
+                for (int64_t n = 0; n < N && ok; n++) {
+                    bool begins = n == 0;
+                    if (kt == g.tiles) {           // a new segment: the old one's last PV goes first
+                        pv(n - 1);
+                        if (!ok) break;
+                        seg_next<TW_ROWS, TW_KEYS>(a, g);
+                        kt = 0;
+                        seg++;
+                        begins = true;
+                    }
+                    if (begins) ok = mbar_wait(&C.q_full, (uint32_t)(seg & 1), &g_tree_error);
+                    const int64_t l = tw_k(n);
+                    const int slot = (int)(l % TW_RING);
+                    ok = ok && mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int b = (int)(n & 1);
+                    const uint32_t S = tmem + b * 128;
+                    const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
+#pragma unroll
+                    for (int h = 1; h >= 0; h--) {
+                        const uint64_t qd = umma_desc_sw128(h ? ql : qh);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const uint64_t o = ((j >> 2) * TW_HALF + (j & 3) * 32) >> 4;
+                            mma_f16_ss(S, qd + o, kd + o, id_s, h && j == 0 ? 0u : 1u);
+                        }
+                    }
+                    tc_commit(&C.empty[slot]);
+                    tc_commit(&C.s_full[b]);
+                    if (++kt == g.tiles) tc_commit(&C.q_empty);
+                    if (!begins) pv(n - 1);
+                }
+                if (ok) pv(N - 1);
+                tc_commit(&C.mma_done);
+                mbar_wait(&C.mma_done, 0, &g_tree_error);
+            }
+        } else {
+            // ---------------- Q of each segment ----------------
+            constexpr int B = 8;
+            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            int seg = 0;
+            do {
+                int r0 = (warp - 2) * B;
+                float4 x[B], y[B];
+                tw_load_q<B>(a, g, r0, x);         // the first rows come while the tensor core still reads Q
+                tw_load_q<B>(a, g, r0 + 2 * B, y);
+                if (seg) ok = __all_sync(0xffffffffu, mbar_wait(&C.q_empty, (uint32_t)((seg - 1) & 1), &g_tree_error));
+                if (!ok) break;
+                for (; r0 < g.rows; r0 += 4 * B) {
+                    tw_store_q<B>(smem, C.qexp[seg & 3], g.rows, r0, x);
+                    if (r0 + 4 * B < g.rows) tw_load_q<B>(a, g, r0 + 4 * B, x);
+                    tw_store_q<B>(smem, C.qexp[seg & 3], g.rows, r0 + 2 * B, y);
+                    if (r0 + 6 * B < g.rows) tw_load_q<B>(a, g, r0 + 6 * B, y);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&C.q_full);
+                seg++;
+            } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
+        }
+    } else if (warp < 12) {
+        // ---------------- softmax of every other tile (thread = row) ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_SOFT));
+        const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t S = tmem + ((uint32_t)(quad * 32) << 16) + wg * 128;
+        uint32_t cleans = 0;
+        int seg = 0;
+        int64_t n = 0;
+        if (N) {
+            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            do {
+                const bool valid = r < g.rows, live = quad * 32 < g.rows;
+                const int hist = g.s.L - g.s.ns;
+                for (int t = 0; t < g.tiles && ok; t++, n++) {
+                    if ((int)(n & 1) != wg) continue;
+                    const uint32_t k = (uint32_t)(n >> 1);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&C.s_full[wg], k & 1, &g_tree_error));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int kb = (g.tile0 + t) * TW_KEYS;
+                    uint32_t vis0 = 0, vis1 = 0, vis2 = 0, vis3 = 0;   // bits of the keys this row sees
+                    bool poison = false;
+                    const bool special = kb + TW_KEYS > hist;
+                    if (special) {
+                        // V of slots past the context may be anything, and that of a drafted token that
+                        // this row does not see may be NaN: 0 x NaN is NaN, so such V become zeros
+                        const int64_t lv = tw_v(n, N);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (uint32_t)((lv / TW_RING) & 1), &g_tree_error));
+                        if (!ok) break;
+                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + r * 128;
+                        const int key = kb + r;
+                        bool odd = false;
+                        if (key >= hist && key < g.s.L) {
+#pragma unroll 4
+                            for (int x = 0; x < 16; x++) {
+                                const uint4 w = *(const uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16);
+                                const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    odd |= (y[i] & 0x7C00u) == 0x7C00u || (y[i] & 0x7C000000u) == 0x7C000000u;
+                            }
+                        }
+                        if (odd || key >= g.s.L) {
+#pragma unroll 4
+                            for (int x = 0; x < 16; x++) *(uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+                        if (lane == 0) C.bad[wg][quad] = odds;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&C.cleaned[wg]);
+                        if (valid) {
+                            const int tok = g.s.s0 + (g.rt * TW_ROWS + r) / a.nrep;
+                            vis0 = tree_bits(a, g.s, tok, kb);
+                            vis1 = tree_bits(a, g.s, tok, kb + 32);
+                            vis2 = tree_bits(a, g.s, tok, kb + 64);
+                            vis3 = tree_bits(a, g.s, tok, kb + 96);
+                        }
+                        ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
+                        if (!ok) break;
+                        poison = (vis0 & C.bad[wg][0]) | (vis1 & C.bad[wg][1]) | (vis2 & C.bad[wg][2]) | (vis3 & C.bad[wg][3]);
+                    }
+                    float m = -INFINITY, sum = 0.0f;
+                    if (live) {
+                        // rolled loops: the two warpgroups' code has to stay in the instruction cache
+                        const float c = a.scale_log2 * __uint_as_float((uint32_t)(127 + C.qexp[seg & 3][r]) << 23);
+                        float mx = -INFINITY, mn = INFINITY;
+#pragma unroll 1
+                        for (int w = 0; w < 4; w++) {
+                            uint32_t s[32];
+                            tmem_ld32(S + 32 * w, s);
+                            tmem_wait_ld();
+                            if (special) {
+                                const uint32_t vis = w == 0 ? vis0 : w == 1 ? vis1 : w == 2 ? vis2 : vis3;
+#pragma unroll
+                                for (int i = 0; i < 32; i++) {
+                                    if (!((vis >> i) & 1)) continue;
+                                    mx = fmaxf(mx, __uint_as_float(s[i]));
+                                    mn = fminf(mn, __uint_as_float(s[i]));
+                                }
+                            } else {
+                                float x[4] = {mx, mx, mx, mx};
+#pragma unroll
+                                for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                                    for (int e = 0; e < 4; e++)
+                                        x[e] = fmaxf(x[e], fmaxf(__uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4])));
+                                mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                                if (c < 0.0f)
+#pragma unroll
+                                    for (int i = 0; i < 32; i++) mn = fminf(mn, __uint_as_float(s[i]));
+                            }
+                        }
+                        if (c < 0.0f) mx = mn == INFINITY ? -INFINITY : mn;
+                        m = mx == -INFINITY ? -INFINITY : mx * c;
+                        const float shift = TW_SHIFT - (m == -INFINITY ? 0.0f : m);
+                        const uint64_t c2 = pack2(c, c), h2 = pack2(shift, shift);
+                        uint64_t sum2 = 0;
+#pragma unroll 1
+                        for (int w = 0; w < 4; w++) {
+                            uint32_t s[32];
+                            tmem_ld32(S + 32 * w, s);
+                            tmem_wait_ld();
+                            const uint32_t vis = w == 0 ? vis0 : w == 1 ? vis1 : w == 2 ? vis2 : vis3;
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                uint32_t hi[8], lo[8];
+#pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    const int e = 16 * j + 2 * i;
+                                    float p0, p1;
+                                    unpack2(fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, h2), p0, p1);
+                                    p0 = ex2(p0);
+                                    p1 = ex2(p1);
+                                    if (special) {
+                                        p0 = (vis >> e) & 1 ? p0 : 0.0f;
+                                        p1 = (vis >> (e + 1)) & 1 ? p1 : 0.0f;
+                                    }
+                                    sum2 = add2(sum2, pack2(p0, p1));
+                                    cut_h2(p0, p1, hi[i], lo[i]);
+                                }
+#pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    s[16 * j + i] = hi[i];
+                                    s[16 * j + 8 + i] = lo[i];
+                                }
+                            }
+                            tmem_st32(S + 32 * w, s);
+                        }
+                        float s1;
+                        unpack2(sum2, sum, s1);
+                        sum = poison ? NAN : sum + s1;
+                    }
+                    if (k) ok = __all_sync(0xffffffffu, mbar_wait(&C.x_free[wg], (k - 1) & 1, &g_tree_error));
+                    if (!ok) break;
+                    C.x[wg][r] = make_float2(m, sum);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&C.p_full[wg]);
+                }
+                seg++;
+            } while (ok && seg_next<TW_ROWS, TW_KEYS>(a, g));
+        }
+    } else {
+        // ---------------- the running output (thread = row) ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TW_REGS_OUT));
+        const int quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t O = tmem + ((uint32_t)(quad * 32) << 16) + 256;
+        int64_t n = 0;
+        if (N) {
+            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            do {
+                const bool valid = r < g.rows, live = quad * 32 < g.rows;
+                const int64_t begin = u0 + n - g.tile0;
+                uint64_t acc[64];
+#pragma unroll
+                for (int i = 0; i < 64; i++) acc[i] = 0;
+                float M = -INFINITY, L = 0.0f;
+                for (int t = 0; t < g.tiles && ok; t++, n++) {
+                    const int b = (int)(n & 1);
+                    const uint32_t k = (uint32_t)(n >> 1);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&C.o_full[b], k & 1, &g_tree_error));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float2 x = C.x[b][r];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&C.x_free[b]);
+                    if (live) {
+                        // a tile that the row sees nothing of (m = -inf, sum 0) has the weight 0
+                        const bool up = valid && x.x > M;
+                        if (__any_sync(0xffffffffu, up)) {
+                            const float f = up ? ex2(M - x.x) : 1.0f;   // M = -inf: 0, all it scales is 0
+                            const uint64_t f2 = pack2(f, f);
+                            if (up) M = x.x;
+                            L *= f;
+#pragma unroll
+                            for (int i = 0; i < 64; i++) acc[i] = fma2(acc[i], f2, 0ull);
+                        }
+                        const float w = x.x == -INFINITY ? 0.0f : ex2(x.x - M);
+                        const uint64_t w2 = pack2(w, w);
+                        L += x.y * w;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            uint32_t o[32];
+                            tmem_ld32(O + b * 128 + 32 * q, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                acc[16 * q + i] = fma2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), w2, acc[16 * q + i]);
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&C.o_free[b]);
+                }
+                if (!ok) break;
+                const bool whole = g.tile0 == 0 && g.tiles == g.s.tiles;
+                if (valid) {
+                    const int R = g.rt * TW_ROWS + r;
+                    const size_t part = ((size_t)blockIdx.x * 2 + (u0 > begin ? 0 : 1)) * a.part_rows + r;
+                    float* dst = a.part_o + part * HD;
+                    float f = 1.0f;
+                    if (whole) {
+                        dst = a.out + ((int64_t)(g.s.s0 + R / a.nrep) * a.hq + g.kvh * a.nrep + R % a.nrep) * HD;
+                        f = L != 0.0f ? 1.0f / L : 0.0f;
+                    } else {
+                        *(float2*)(a.part_ml + part * 2) = make_float2(M, L);
+                    }
+                    const uint64_t f2 = pack2(f, f);
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        float4 y;
+                        unpack2(fma2(acc[i], f2, 0ull), y.x, y.y);
+                        unpack2(fma2(acc[i + 1], f2, 0ull), y.z, y.w);
+                        *(float4*)(dst + 2 * i) = y;
+                    }
+                }
+                if (!whole && g.tile0 == 0 && threadIdx.x == 12 * 32)
+                    a.cuts[blockIdx.x] = {begin, begin + g.s.tiles, T, g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh};
+            } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
+        }
     }
 
     tc_fence_before();
@@ -776,7 +845,7 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     a.q = q;
     a.n_arena_blocks = n_arena_blocks;
     a.n_layer = n_layer; a.layer = layer; a.bt = bt; a.mbs = mbs; a.starts = seq_starts; a.ctx = ctx;
-    a.mask = mask; a.words = words; a.n_tok = n_tok; a.n_seqs = n_seqs; a.max_tok = max_seq_tokens;
+    a.mask = mask; a.words = words; a.n_tok = n_tok; a.n_seqs = n_seqs; a.max_tok = max_seq_tokens; a.max_ctx = max_ctx;
     a.hq = hq; a.hkv = hkv; a.nrep = hq / hkv;
     a.scale_log2 = scale * LOG2E;
     a.out = out;

@@ -351,7 +351,9 @@ int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena
     if (mask_words <= 0 || max_seq_tokens > (int64_t)64 * mask_words)
         return fail(DCG_EINVAL, "tree_mask has too few words for max_seq_tokens");
     if (n_seqs > 65535 || hq > 65535) return fail(DCG_EINVAL, "n_seqs and hq must be <= 65535");
-    if ((int64_t)max_seq_tokens * (hq / hkv) > INT32_MAX / 2) return fail(DCG_EINVAL, "max_seq_tokens too large");
+    // rows, and the key tiles of a sequence's items, are counted in 32 bits
+    if ((int64_t)max_seq_tokens * hq > INT32_MAX / 128 || ((int64_t)max_seq_tokens * hq / 16 + hkv) * (max_ctx / 16 + 1) > INT32_MAX)
+        return fail(DCG_EINVAL, "max_seq_tokens * hq * max_ctx too large");
     if (!aligned(k_arena, 16) || !aligned(v_arena, 16) || !aligned(q, 16) || !aligned(out, 16) || !aligned(tree_mask, 8))
         return fail(DCG_EINVAL, "q, out and the arenas must be 16-byte aligned, tree_mask 8-byte");
     const size_t need = dcg::tree_scratch_bytes(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
