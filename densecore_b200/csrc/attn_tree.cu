@@ -253,17 +253,25 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
     // D f32 (bits 4-5 = 1), A and B f16 (0), B MN-major (bit 16), N >> 3 at 17-22, M >> 4 at 24-28
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+// one thread of the warp, the same each time
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, uint32_t acc) {
+template <bool ACC>
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d), "r"(at), "l"(bd), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
+}
+template <bool ACC>
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(at), "l"(bd), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
 }
 // MN-major operand, 128-byte swizzle: rows of 64 MN-elements, 8-row (K) atoms 1 KB apart, the next 64
 // MN-elements TW_HALF further
@@ -294,8 +302,8 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 
 // ring position of the K and V tile of the range's n-th unit of N: K0 K1 V0 K2 V1 ... K(N-1) V(N-2) V(N-1)
-__device__ __forceinline__ int64_t tw_k(int64_t n) { return n ? 2 * n - 1 : 0; }
-__device__ __forceinline__ int64_t tw_v(int64_t n, int64_t N) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; }
+__device__ __forceinline__ uint32_t tw_k(int n) { return n ? 2 * n - 1 : 0; }
+__device__ __forceinline__ uint32_t tw_v(int n, int N) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; }
 
 // two fp32 operations at a time
 __device__ __forceinline__ uint64_t pack2(float x0, float x1) {
@@ -387,7 +395,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     int64_t* at = (int64_t*)smem;                 // the Q space, before Q
     tree_locate<TW_ROWS, TW_KEYS, TW_THREADS>(a, at, at + 4);
     const int64_t T = at[2], u0 = sk_begin(blockIdx.x, T, gridDim.x), u1 = sk_begin(blockIdx.x + 1, T, gridDim.x);
-    const int64_t N = u1 - u0;
+    const int N = (int)(u1 - u0);
     const int seq0 = N ? (int)at[0] : 0, off0 = N ? (int)(u0 - at[1]) : 0;
     if (threadIdx.x == 0) a.cuts[blockIdx.x].rows = 0;
     tc_fence_before();
@@ -410,9 +418,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 const int p = (s.tile0 + tile) * (TW_KEYS / KVB) + page;
                 return lane < 16 && p * KVB < s.s.L ? a.bt[(int64_t)s.seq * a.mbs + p] : INT32_MIN;
             };
-            auto load = [&](const CUtensorMap* map, int kvh, int b, int64_t l) {
-                const int slot = (int)(l % TW_RING);
-                if (l >= TW_RING) ok = mbar_wait(&C.empty[slot], (uint32_t)((l / TW_RING - 1) & 1), &g_tree_error);
+            auto load = [&](const CUtensorMap* map, int kvh, int b, uint32_t l) {
+                const uint32_t slot = l % TW_RING;
+                if (l >= TW_RING) ok = mbar_wait(&C.empty[slot], (l / TW_RING - 1) & 1, &g_tree_error);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return;
                 const bool in = b >= 0 && b < a.n_arena_blocks;
@@ -422,9 +430,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 __syncwarp();
                 if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, kvh, &C.full[slot]);
             };
-            int64_t l = 0;
+            uint32_t l = 0;
             int b_now = block(g, 0), h_now = g.kvh, b_last = 0, h_last = 0;
-            for (int64_t n = 0; n <= N && ok; n++) {       // V runs one unit behind K
+            for (int n = 0; n <= N && ok; n++) {           // V runs one unit behind K
                 int b_next = 0, h_next = 0;
                 if (n < N) {
                     load(&kmap, h_now, b_now, l++);
@@ -444,72 +452,76 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 h_now = h_next;
             }
             if (!ok)                               // given up: the copies in flight land before the CTA ends
-                for (int64_t i = l > TW_RING ? l - TW_RING : 0; i < l; i++) mbar_wait(&C.full[i % TW_RING], (uint32_t)((i / TW_RING) & 1), &g_tree_error, 1u << 16);
+                for (uint32_t i = l > TW_RING ? l - TW_RING : 0; i < l; i++) mbar_wait(&C.full[i % TW_RING], (i / TW_RING) & 1, &g_tree_error, 1u << 16);
         } else if (warp == 1) {
-            // ---------------- MMA issue ----------------
-            if (lane == 0) {
-                constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
-                const uint32_t qh = smem_u32(smem), ql = qh + TW_BUF;
-                const uint32_t rg = smem_u32(ring);
-                TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-                int kt = 0, seg = 0;
-                auto pv = [&](int64_t n) {         // O of unit n = P V
-                    const int b = (int)(n & 1);
-                    const uint32_t k = (uint32_t)(n >> 1);
-                    const int64_t l = tw_v(n, N);
-                    const int slot = (int)(l % TW_RING);
-                    ok = mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
-                    if (ok && k) ok = mbar_wait(&C.o_free[b], (k - 1) & 1, &g_tree_error);
-                    if (ok) ok = mbar_wait(&C.p_full[b], k & 1, &g_tree_error);
-                    if (!ok) return;
-                    tc_fence_after();
-                    const uint32_t P = tmem + b * 128, O = tmem + 256 + b * 128;
-                    const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
-#pragma unroll
-                    for (int h = 1; h >= 0; h--)   // the lo halves first; 16 keys = 2048 bytes per k-step
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            mma_f16_ts(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o, h && j == 0 ? 0u : 1u);
-                    tc_commit(&C.empty[slot]);
-                    tc_commit(&C.o_full[b]);
-                };
-                for (int64_t n = 0; n < N && ok; n++) {
-                    bool begins = n == 0;
-                    if (kt == g.tiles) {           // a new segment: the old one's last PV goes first
-                        pv(n - 1);
-                        if (!ok) break;
-                        seg_next<TW_ROWS, TW_KEYS>(a, g);
-                        kt = 0;
-                        seg++;
-                        begins = true;
+            // ---------------- MMA issue: the warp in step, one elected thread issues ----------------
+            constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
+            const uint32_t qh = smem_u32(smem), rg = qh + TW_OFF_RING;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const bool leader = elect_one();
+            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            int left = g.tiles, seg = 0;
+            for (int n = 0; n <= N && ok; n++) {   // S of unit n, then O of unit n - 1
+                if (n < N) {
+                    if (n == 0 || left == 0) {
+                        if (left == 0) {
+                            seg_next<TW_ROWS, TW_KEYS>(a, g);
+                            left = g.tiles;
+                            seg++;
+                        }
+                        ok = mbar_wait(&C.q_full, (uint32_t)(seg & 1), &g_tree_error);
                     }
-                    if (begins) ok = mbar_wait(&C.q_full, (uint32_t)(seg & 1), &g_tree_error);
-                    const int64_t l = tw_k(n);
-                    const int slot = (int)(l % TW_RING);
-                    ok = ok && mbar_wait(&C.full[slot], (uint32_t)((l / TW_RING) & 1), &g_tree_error);
+                    left--;
+                    const uint32_t l = tw_k(n), slot = l % TW_RING;
+                    ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error));
                     if (!ok) break;
                     tc_fence_after();
-                    const int b = (int)(n & 1);
-                    const uint32_t S = tmem + b * 128;
-                    const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
+                    if (leader) {
+                        const uint32_t S = tm + (n & 1) * 128;
+                        const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
 #pragma unroll
-                    for (int h = 1; h >= 0; h--) {
-                        const uint64_t qd = umma_desc_sw128(h ? ql : qh);
+                        for (int h = 1; h >= 0; h--) {   // the lo half first
+                            const uint64_t qd = umma_desc_sw128(qh + h * TW_BUF);
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const uint64_t o = ((j >> 2) * TW_HALF + (j & 3) * 32) >> 4;
-                            mma_f16_ss(S, qd + o, kd + o, id_s, h && j == 0 ? 0u : 1u);
+                            for (int j = 0; j < 8; j++) {
+                                const uint64_t o = ((j >> 2) * TW_HALF + (j & 3) * 32) >> 4;
+                                if (h && j == 0) mma_f16_ss<false>(S, qd + o, kd + o, id_s);
+                                else mma_f16_ss<true>(S, qd + o, kd + o, id_s);
+                            }
                         }
+                        tc_commit(&C.s_full[n & 1]);
+                        tc_commit(&C.empty[slot]);
+                        if (left == 0) tc_commit(&C.q_empty);
                     }
-                    tc_commit(&C.empty[slot]);
-                    tc_commit(&C.s_full[b]);
-                    if (++kt == g.tiles) tc_commit(&C.q_empty);
-                    if (!begins) pv(n - 1);
+                    __syncwarp();
                 }
-                if (ok) pv(N - 1);
-                tc_commit(&C.mma_done);
-                mbar_wait(&C.mma_done, 0, &g_tree_error);
+                if (n > 0) {
+                    const int u = n - 1, b = u & 1;
+                    const uint32_t k = (uint32_t)u >> 1, l = tw_v(u, N), slot = l % TW_RING;
+                    ok = mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error);
+                    if (ok && k) ok = mbar_wait(&C.o_free[b], (k - 1) & 1, &g_tree_error);
+                    ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.p_full[b], k & 1, &g_tree_error));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+                        const uint32_t P = tm + b * 128, O = tm + 256 + b * 128;
+                        const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
+#pragma unroll
+                        for (int h = 1; h >= 0; h--)   // 16 keys = 2048 bytes per k-step
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                if (h && j == 0) mma_f16_ts<false>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                                else mma_f16_ts<true>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                            }
+                        tc_commit(&C.o_full[b]);
+                        tc_commit(&C.empty[slot]);
+                    }
+                    __syncwarp();
+                }
             }
+            if (leader) tc_commit(&C.mma_done);
+            __syncwarp();
+            mbar_wait(&C.mma_done, 0, &g_tree_error);
         } else {
             // ---------------- Q of each segment ----------------
             constexpr int B = 8;
@@ -540,8 +552,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t S = tmem + ((uint32_t)(quad * 32) << 16) + wg * 128;
         uint32_t cleans = 0;
-        int seg = 0;
-        int64_t n = 0;
+        int seg = 0, n = 0;
         if (N) {
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
             do {
@@ -560,16 +571,16 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     if (special) {
                         // V of slots past the context may be anything, and that of a drafted token that
                         // this row does not see may be NaN: 0 x NaN is NaN, so such V become zeros
-                        const int64_t lv = tw_v(n, N);
-                        ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (uint32_t)((lv / TW_RING) & 1), &g_tree_error));
+                        const uint32_t lv = tw_v(n, N);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (lv / TW_RING) & 1, &g_tree_error));
                         if (!ok) break;
                         uint8_t* v = ring + (lv % TW_RING) * TW_BUF + r * 128;
                         const int key = kb + r;
                         bool odd = false;
                         if (key >= hist && key < g.s.L) {
 #pragma unroll 4
-                            for (int x = 0; x < 16; x++) {
-                                const uint4 w = *(const uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16);
+                            for (int x = 0; x < 16; x++) {   // chunks in an order that spreads the lanes over the banks
+                                const uint4 w = *(const uint4*)(v + (x >> 3) * TW_HALF + ((x + lane) & 7) * 16);
                                 const uint32_t y[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                                 for (int i = 0; i < 4; i++)
@@ -578,7 +589,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         }
                         if (odd || key >= g.s.L) {
 #pragma unroll 4
-                            for (int x = 0; x < 16; x++) *(uint4*)(v + (x >> 3) * TW_HALF + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            for (int x = 0; x < 16; x++) *(uint4*)(v + (x >> 3) * TW_HALF + ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
                         const uint32_t odds = __ballot_sync(0xffffffffu, odd);
                         if (lane == 0) C.bad[wg][quad] = odds;
@@ -683,7 +694,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TW_REGS_OUT));
         const int quad = warp & 3, r = quad * 32 + lane;
         const uint32_t O = tmem + ((uint32_t)(quad * 32) << 16) + 256;
-        int64_t n = 0;
+        int n = 0;
         if (N) {
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
             do {
