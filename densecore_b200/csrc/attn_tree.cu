@@ -49,7 +49,11 @@ struct TreeArgs {
     // scratch
     float *part_o, *part_ml;     // [2 G][rows][128], [2 G][rows][2]
     struct TreeCut* cuts;        // [G]
-    int part_rows;
+    int part_rows;               // rows of the largest row tile
+    int q_rows;                  // the same in eights: rows of a Q tile
+    int row_tiles;               // of the largest sequence
+    uint8_t* q_tiles;            // [n_seqs][row_tiles][hkv] x q_rows * 512 B: Q as halves, as shared memory wants it
+    int8_t* q_exps;              // the same x q_rows: exponents of the rows' scales
 };
 
 // an item that CTA c begins and later CTAs go on with (rows = 0: none)
@@ -83,7 +87,7 @@ struct TreeSeg {
     int seq, kvh, rt, rows;      // rows of this row tile
     int tile0, tiles;            // of the item's
     TreeSeq s, next;             // next: of sequence seq + 1, its loads on the way meanwhile
-    int64_t left;                // units of the range behind this segment
+    int left;                    // units of the range behind this segment
 };
 template <int ROWS, int KEYS>
 __device__ __forceinline__ TreeSeq seq_or_none(const TreeArgs& a, int seq) {
@@ -92,11 +96,11 @@ __device__ __forceinline__ TreeSeq seq_or_none(const TreeArgs& a, int seq) {
 template <int ROWS>
 __device__ __forceinline__ void seg_shape(const TreeArgs& a, TreeSeg& g) {
     g.rows = min(ROWS, g.s.ns * a.nrep - g.rt * ROWS);
-    g.tiles = (int)min((int64_t)(g.s.tiles - g.tile0), g.left);
+    g.tiles = min(g.s.tiles - g.tile0, g.left);
     g.left -= g.tiles;
 }
 template <int ROWS, int KEYS>
-__device__ __forceinline__ TreeSeg seg_first(const TreeArgs& a, int seq, int off, int64_t units) {
+__device__ __forceinline__ TreeSeg seg_first(const TreeArgs& a, int seq, int off, int units) {
     TreeSeg g;
     g.seq = seq;
     g.s = tree_seq<ROWS, KEYS>(a, seq, false);
@@ -218,9 +222,10 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // adds to a large accumulator: hence the lo halves first, and no accumulator that lives for longer
 // than a tile (one that lived for a segment was 2-4 x 10^-6 off, this is 4-6 x 10^-7).
 // Two S / P and two O buffers, used in turn.  Warps: 0 TMA producer (ring of 5 x 32 KB, K and V tiles
-// in the order the MMAs take them; pages beyond the sequence load as zeros), 1 MMA issue, 2-3 the next
-// segment's Q, 4-7 and 8-11 softmax of every other tile, 12-15 the running output (128 registers of
-// it per thread, thread = row).
+// in the order the MMAs take them; pages beyond the sequence load as zeros), 1 MMA issue, 2 the next
+// segment's Q (up to 64 rows into a second buffer), 4-7 and 8-11 softmax of every other tile, 12-15
+// the running output (128 registers of it per thread, thread = row).  tree_q_kernel has laid Q out
+// before: converting it here cost 20,000 cycles at every change of the item.
 // What bounds it: HBM up to 128 rows per item (64 KB per unit: 2800 cycles of an SM's share, against
 // 32 MMAs of 64 cycles); beyond, the tensor core.
 // ------------------------------------------------------------------------------------------
@@ -236,15 +241,14 @@ constexpr int TW_CTRL = 3072;
 constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // all of it: 227 KB
 constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^8: the small ones stay above fp16's least
 // registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128
-constexpr int TW_REGS_CTRL = 104, TW_REGS_SOFT = 104, TW_REGS_OUT = 200;
+constexpr int TW_REGS_CTRL = 56, TW_REGS_SOFT = 128, TW_REGS_OUT = 200;
 static_assert(TW_REGS_CTRL + 2 * TW_REGS_SOFT + TW_REGS_OUT <= 512, "register split");
 
 struct TwCtrl {
     uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_full[2], o_free[2], x_free[2], cleaned[2];
-    uint64_t q_full, q_empty, mma_done;
+    uint64_t q_full[2], q_empty[2], mma_done;
     uint32_t tmem;
     uint32_t bad[2][4];                           // per buffer: keys of its tile whose V is not finite
-    int8_t qexp[4][TW_ROWS];                      // row scale exponents, by segment & 3
     float2 x[2][TW_ROWS];                         // a tile's row max and sum of p
 };
 static_assert(sizeof(TwCtrl) <= TW_CTRL, "control block");
@@ -323,38 +327,36 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
-// Q of a segment as halves: a warp takes every other group of B rows; o: swizzled K-major tiles
-template <int B>
-__device__ __forceinline__ void tw_load_q(const TreeArgs& a, const TreeSeg& g, int r0, float4 (&x)[B]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < B; i++) {
-        const int R = g.rt * TW_ROWS + min(r0 + i, g.rows - 1);
-        x[i] = *(const float4*)(a.q + ((int64_t)(g.s.s0 + R / a.nrep) * a.hq + g.kvh * a.nrep + R % a.nrep) * HD + 4 * lane);
-    }
-}
-template <int B>
-__device__ __forceinline__ void tw_store_q(uint8_t* smem, int8_t* qexp, int rows, int r0, const float4 (&x)[B]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < B; i++) {
-        if (r0 + i >= rows) break;
-        const int r = r0 + i;
-        float m = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        // exponent of the largest value (0 rows and subnormal ones: the least)
-        int e = (int)(__float_as_uint(m) >> 23) - 127;
+// Q as fp16 halves in the tiles that tree_wide_kernel copies: [hi, lo][half of 64 dims][q_rows][128 B],
+// 128-byte swizzle, each row scaled by a power of two (its sign the scale's).  A warp is a row: CTA
+// (drafted token, sequence), heads in turn.
+constexpr int TQ_WARPS = 8;
+__global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, blockIdx.y, false);
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    if (t >= s.ns) return;
+    const float* q = a.q + (int64_t)(s.s0 + t) * a.hq * HD + 4 * lane;
+#pragma unroll 4
+    for (int h = threadIdx.x >> 5; h < a.hq; h += TQ_WARPS) {
+        const float4 x = *(const float4*)(q + h * HD);
+        const int kvh = h / a.nrep, R = t * a.nrep + h - kvh * a.nrep, rt = R / TW_ROWS, r = R - rt * TW_ROWS;
+        const int64_t tile = ((int64_t)blockIdx.y * a.row_tiles + rt) * a.hkv + kvh;
+        const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        // exponent of the row's largest value (0 rows and subnormal ones: the least)
+        int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(m)) >> 23) - 127;
         e = e < -100 ? -100 : e > 120 ? 120 : e;
-        const float f = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
+        const float f = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);   // 2^-e
         uint32_t h0, l0, h1, l1;
-        cut_h2(x[i].x * f, x[i].y * f, h0, l0);
-        cut_h2(x[i].z * f, x[i].w * f, h1, l1);
+        cut_h2(x.x * f, x.y * f, h0, l0);
+        cut_h2(x.z * f, x.w * f, h1, l1);
         // dims 4 lane .. +3: 8 bytes of 16-byte chunk (lane / 2) & 7 of its half
-        const uint32_t o = (lane >> 4) * TW_HALF + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
-        *(uint2*)(smem + o) = make_uint2(h0, h1);
-        *(uint2*)(smem + TW_BUF + o) = make_uint2(l0, l1);
-        if (lane == 0) qexp[r] = (int8_t)e;
+        uint8_t* to = a.q_tiles + tile * a.q_rows * 512 + (lane >> 4) * a.q_rows * 128 + r * 128 +
+                      ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
+        *(uint2*)to = make_uint2(h0, h1);
+        *(uint2*)(to + a.q_rows * 256) = make_uint2(l0, l1);
+        if (lane == 0) a.q_exps[tile * a.q_rows + r] = (int8_t)e;
     }
 }
 
@@ -381,9 +383,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             mbar_init(&C.o_free[b], 4);
             mbar_init(&C.x_free[b], 4);
             mbar_init(&C.cleaned[b], 4);
+            mbar_init(&C.q_full[b], 1);
+            mbar_init(&C.q_empty[b], 1);
         }
-        mbar_init(&C.q_full, 2);
-        mbar_init(&C.q_empty, 1);
         mbar_init(&C.mma_done, 1);
         fence_mbar_init();
     }
@@ -404,6 +406,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     const uint32_t tmem = C.tmem;
     bool ok = true;
 
+    // up to 64 rows there is room for two Q
+    const int q_bufs = a.q_rows <= 64 ? 2 : 1, q_bytes = a.q_rows * 512;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_CTRL));
         if (N == 0) {
@@ -461,103 +465,120 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             const bool leader = elect_one();
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
             int left = g.tiles, seg = 0;
-            for (int n = 0; n <= N && ok; n++) {   // S of unit n, then O of unit n - 1
-                if (n < N) {
-                    if (n == 0 || left == 0) {
-                        if (left == 0) {
-                            seg_next<TW_ROWS, TW_KEYS>(a, g);
-                            left = g.tiles;
-                            seg++;
-                        }
-                        ok = mbar_wait(&C.q_full, (uint32_t)(seg & 1), &g_tree_error);
-                    }
-                    left--;
-                    const uint32_t l = tw_k(n), slot = l % TW_RING;
-                    ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error));
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) {
-                        const uint32_t S = tm + (n & 1) * 128;
-                        const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
-#pragma unroll
-                        for (int h = 1; h >= 0; h--) {   // the lo half first
-                            const uint64_t qd = umma_desc_sw128(qh + h * TW_BUF);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                const uint64_t o = ((j >> 2) * TW_HALF + (j & 3) * 32) >> 4;
-                                if (h && j == 0) mma_f16_ss<false>(S, qd + o, kd + o, id_s);
-                                else mma_f16_ss<true>(S, qd + o, kd + o, id_s);
-                            }
-                        }
-                        tc_commit(&C.s_full[n & 1]);
-                        tc_commit(&C.empty[slot]);
-                        if (left == 0) tc_commit(&C.q_empty);
-                    }
-                    __syncwarp();
+            const uint32_t q_half = a.q_rows * 128;
+            // S of unit n: what it waits for, and the MMAs (issued by the leader)
+            auto wait_s = [&](int n) {
+                if (left == 0) {
+                    seg_next<TW_ROWS, TW_KEYS>(a, g);
+                    left = g.tiles;
+                    seg++;
                 }
-                if (n > 0) {
-                    const int u = n - 1, b = u & 1;
-                    const uint32_t k = (uint32_t)u >> 1, l = tw_v(u, N), slot = l % TW_RING;
-                    ok = mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error);
-                    if (ok && k) ok = mbar_wait(&C.o_free[b], (k - 1) & 1, &g_tree_error);
-                    ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.p_full[b], k & 1, &g_tree_error));
+                const int qb = seg % q_bufs;
+                if (left == g.tiles) ok = mbar_wait(&C.q_full[qb], (uint32_t)((seg / q_bufs) & 1), &g_tree_error);
+                const uint32_t l = tw_k(n), slot = l % TW_RING;
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error));
+            };
+            auto issue_s = [&](int n) {
+                left--;
+                if (leader) {
+                    const uint32_t slot = tw_k(n) % TW_RING, S = tm + (n & 1) * 128, q = qh + (seg % q_bufs) * q_bytes;
+                    const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
+#pragma unroll
+                    for (int h = 1; h >= 0; h--) {   // the lo half first
+#pragma unroll
+                        for (int d = 0; d < 2; d++) {
+                            const uint64_t qd = umma_desc_sw128(q + (2 * h + d) * q_half);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                if (h && !d && j == 0) mma_f16_ss<false>(S, qd + 2 * j, kd + d * (TW_HALF >> 4) + 2 * j, id_s);
+                                else mma_f16_ss<true>(S, qd + 2 * j, kd + d * (TW_HALF >> 4) + 2 * j, id_s);
+                            }
+                        }
+                    }
+                    tc_commit(&C.s_full[n & 1]);
+                    tc_commit(&C.empty[slot]);
+                    if (left == 0) tc_commit(&C.q_empty[seg % q_bufs]);
+                }
+                __syncwarp();
+            };
+            wait_s(0);
+            if (ok) {
+                tc_fence_after();
+                issue_s(0);
+                if (N > 1) wait_s(1);
+            }
+            if (ok && N > 1) {
+                tc_fence_after();
+                issue_s(1);
+            }
+            for (int n = 0; n < N && ok; n++) {    // O of unit n, then S of unit n + 2 into the same buffer
+                const int b = n & 1;
+                const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
+                const bool ahead = n + 2 < N && left > 0;   // of the same segment: its K was long asked for
+                ok = mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error);
+                if (ok && k) ok = mbar_wait(&C.o_free[b], (k - 1) & 1, &g_tree_error);
+                if (ok && ahead) wait_s(n + 2);
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.p_full[b], k & 1, &g_tree_error));
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
+                    const uint32_t P = tm + b * 128, O = tm + 256 + b * 128;
+                    const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
+#pragma unroll
+                    for (int h = 1; h >= 0; h--)   // 16 keys = 2048 bytes per k-step
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            if (h && j == 0) mma_f16_ts<false>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                            else mma_f16_ts<true>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                        }
+                    tc_commit(&C.o_full[b]);
+                    tc_commit(&C.empty[slot]);
+                }
+                __syncwarp();
+                if (n + 2 < N) {
+                    if (!ahead) wait_s(n + 2);
                     if (!ok) break;
                     tc_fence_after();
-                    if (leader) {
-                        const uint32_t P = tm + b * 128, O = tm + 256 + b * 128;
-                        const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
-#pragma unroll
-                        for (int h = 1; h >= 0; h--)   // 16 keys = 2048 bytes per k-step
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                if (h && j == 0) mma_f16_ts<false>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
-                                else mma_f16_ts<true>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
-                            }
-                        tc_commit(&C.o_full[b]);
-                        tc_commit(&C.empty[slot]);
-                    }
-                    __syncwarp();
+                    issue_s(n + 2);
                 }
             }
             if (leader) tc_commit(&C.mma_done);
             __syncwarp();
             mbar_wait(&C.mma_done, 0, &g_tree_error);
-        } else {
+        } else if (warp == 2) {
             // ---------------- Q of each segment ----------------
-            constexpr int B = 8;
-            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-            int seg = 0;
-            do {
-                int r0 = (warp - 2) * B;
-                float4 x[B], y[B];
-                tw_load_q<B>(a, g, r0, x);         // the first rows come while the tensor core still reads Q
-                tw_load_q<B>(a, g, r0 + 2 * B, y);
-                if (seg) ok = __all_sync(0xffffffffu, mbar_wait(&C.q_empty, (uint32_t)((seg - 1) & 1), &g_tree_error));
-                if (!ok) break;
-                for (; r0 < g.rows; r0 += 4 * B) {
-                    tw_store_q<B>(smem, C.qexp[seg & 3], g.rows, r0, x);
-                    if (r0 + 4 * B < g.rows) tw_load_q<B>(a, g, r0 + 4 * B, x);
-                    tw_store_q<B>(smem, C.qexp[seg & 3], g.rows, r0 + 2 * B, y);
-                    if (r0 + 6 * B < g.rows) tw_load_q<B>(a, g, r0 + 6 * B, y);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&C.q_full);
-                seg++;
-            } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
+            if (lane == 0) {
+                TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+                int seg = 0;
+                do {
+                    const int qb = seg % q_bufs;
+                    if (seg >= q_bufs) ok = mbar_wait(&C.q_empty[qb], (uint32_t)((seg / q_bufs - 1) & 1), &g_tree_error);
+                    if (!ok) break;
+                    const int64_t tile = ((int64_t)g.seq * a.row_tiles + g.rt) * a.hkv + g.kvh;
+                    mbar_arrive_expect_tx(&C.q_full[qb], (uint32_t)q_bytes);
+                    bulk_g2s(smem + qb * q_bytes, a.q_tiles + tile * q_bytes, (uint32_t)q_bytes, &C.q_full[qb]);
+                    seg++;
+                } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
+                if (!ok)
+                    for (int i = seg > q_bufs ? seg - q_bufs : 0; i < seg; i++) mbar_wait(&C.q_full[i % q_bufs], (uint32_t)((i / q_bufs) & 1), &g_tree_error, 1u << 16);
+            }
         }
     } else if (warp < 12) {
         // ---------------- softmax of every other tile (thread = row) ----------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_SOFT));
         const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t S = tmem + ((uint32_t)(quad * 32) << 16) + wg * 128;
         uint32_t cleans = 0;
-        int seg = 0, n = 0;
+        int n = 0;
         if (N) {
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
             do {
                 const bool valid = r < g.rows, live = quad * 32 < g.rows;
                 const int hist = g.s.L - g.s.ns;
+                const int tok = g.s.s0 + (valid ? (g.rt * TW_ROWS + r) / a.nrep : 0);
+                // c > 0 (the scale's sign is in Q), and not 0: c x -inf has to stay -inf
+                const int64_t tile = ((int64_t)g.seq * a.row_tiles + g.rt) * a.hkv + g.kvh;
+                const int qexp = valid ? a.q_exps[tile * a.q_rows + r] : 0;
+                const float c = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + qexp) << 23), 1e-37f);
                 for (int t = 0; t < g.tiles && ok; t++, n++) {
                     if ((int)(n & 1) != wg) continue;
                     const uint32_t k = (uint32_t)(n >> 1);
@@ -565,7 +586,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     if (!ok) break;
                     tc_fence_after();
                     const int kb = (g.tile0 + t) * TW_KEYS;
-                    uint32_t vis0 = 0, vis1 = 0, vis2 = 0, vis3 = 0;   // bits of the keys this row sees
                     bool poison = false;
                     const bool special = kb + TW_KEYS > hist;
                     if (special) {
@@ -596,59 +616,46 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&C.cleaned[wg]);
-                        if (valid) {
-                            const int tok = g.s.s0 + (g.rt * TW_ROWS + r) / a.nrep;
-                            vis0 = tree_bits(a, g.s, tok, kb);
-                            vis1 = tree_bits(a, g.s, tok, kb + 32);
-                            vis2 = tree_bits(a, g.s, tok, kb + 64);
-                            vis3 = tree_bits(a, g.s, tok, kb + 96);
-                        }
                         ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
                         if (!ok) break;
-                        poison = (vis0 & C.bad[wg][0]) | (vis1 & C.bad[wg][1]) | (vis2 & C.bad[wg][2]) | (vis3 & C.bad[wg][3]);
+                        if (live) {
+#pragma unroll 1
+                            for (int w = 0; w < 4; w++) {
+                                const uint32_t vis = valid ? tree_bits(a, g.s, tok, kb + 32 * w) : 0u;   // keys this row sees
+                                poison |= (vis & C.bad[wg][w]) != 0;
+                                uint32_t s[32];
+                                tmem_ld32(S + 32 * w, s);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; i++) s[i] = (vis >> i) & 1 ? s[i] : 0xFF800000u;
+                                tmem_st32(S + 32 * w, s);
+                            }
+                            tmem_wait_st();
+                        }
                     }
                     float m = -INFINITY, sum = 0.0f;
                     if (live) {
                         // rolled loops: the two warpgroups' code has to stay in the instruction cache
-                        const float c = a.scale_log2 * __uint_as_float((uint32_t)(127 + C.qexp[seg & 3][r]) << 23);
-                        float mx = -INFINITY, mn = INFINITY;
+                        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-                        for (int w = 0; w < 4; w++) {
-                            uint32_t s[32];
-                            tmem_ld32(S + 32 * w, s);
+                        for (int w = 0; w < 4; w += 2) {
+                            uint32_t s[2][32];
+                            tmem_ld32(S + 32 * w, s[0]);
+                            tmem_ld32(S + 32 * w + 32, s[1]);
                             tmem_wait_ld();
-                            if (special) {
-                                const uint32_t vis = w == 0 ? vis0 : w == 1 ? vis1 : w == 2 ? vis2 : vis3;
 #pragma unroll
-                                for (int i = 0; i < 32; i++) {
-                                    if (!((vis >> i) & 1)) continue;
-                                    mx = fmaxf(mx, __uint_as_float(s[i]));
-                                    mn = fminf(mn, __uint_as_float(s[i]));
-                                }
-                            } else {
-                                float x[4] = {mx, mx, mx, mx};
+                            for (int i = 0; i < 32; i += 4)
 #pragma unroll
-                                for (int i = 0; i < 32; i += 8)
-#pragma unroll
-                                    for (int e = 0; e < 4; e++)
-                                        x[e] = fmaxf(x[e], fmaxf(__uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4])));
-                                mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                                if (c < 0.0f)
-#pragma unroll
-                                    for (int i = 0; i < 32; i++) mn = fminf(mn, __uint_as_float(s[i]));
-                            }
+                                for (int e = 0; e < 4; e++)
+                                    x[e] = fmaxf(x[e], fmaxf(__uint_as_float(s[0][i + e]), __uint_as_float(s[1][i + e])));
                         }
-                        if (c < 0.0f) mx = mn == INFINITY ? -INFINITY : mn;
-                        m = mx == -INFINITY ? -INFINITY : mx * c;
+                        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        m = mx * c;
                         const float shift = TW_SHIFT - (m == -INFINITY ? 0.0f : m);
                         const uint64_t c2 = pack2(c, c), h2 = pack2(shift, shift);
                         uint64_t sum2 = 0;
-#pragma unroll 1
-                        for (int w = 0; w < 4; w++) {
-                            uint32_t s[32];
-                            tmem_ld32(S + 32 * w, s);
-                            tmem_wait_ld();
-                            const uint32_t vis = w == 0 ? vis0 : w == 1 ? vis1 : w == 2 ? vis2 : vis3;
+                        // 32 scores -> p as halves, in their place
+                        auto halves = [&](uint32_t (&s)[32]) {
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
                                 uint32_t hi[8], lo[8];
@@ -659,10 +666,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                                     unpack2(fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, h2), p0, p1);
                                     p0 = ex2(p0);
                                     p1 = ex2(p1);
-                                    if (special) {
-                                        p0 = (vis >> e) & 1 ? p0 : 0.0f;
-                                        p1 = (vis >> (e + 1)) & 1 ? p1 : 0.0f;
-                                    }
                                     sum2 = add2(sum2, pack2(p0, p1));
                                     cut_h2(p0, p1, hi[i], lo[i]);
                                 }
@@ -672,11 +675,23 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                                     s[16 * j + 8 + i] = lo[i];
                                 }
                             }
-                            tmem_st32(S + 32 * w, s);
+                        };
+                        uint32_t s0[32], s1[32];           // one is loaded while the other is worked on
+                        tmem_ld32(S, s0);
+#pragma unroll 1
+                        for (int w = 0; w < 4; w += 2) {
+                            tmem_wait_ld();
+                            tmem_ld32(S + 32 * w + 32, s1);
+                            halves(s0);
+                            tmem_st32(S + 32 * w, s0);
+                            tmem_wait_ld();
+                            if (w == 0) tmem_ld32(S + 64, s0);
+                            halves(s1);
+                            tmem_st32(S + 32 * w + 32, s1);
                         }
-                        float s1;
-                        unpack2(sum2, sum, s1);
-                        sum = poison ? NAN : sum + s1;
+                        float odd;
+                        unpack2(sum2, sum, odd);
+                        sum = poison ? NAN : sum + odd;
                     }
                     if (k) ok = __all_sync(0xffffffffu, mbar_wait(&C.x_free[wg], (k - 1) & 1, &g_tree_error));
                     if (!ok) break;
@@ -686,7 +701,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&C.p_full[wg]);
                 }
-                seg++;
             } while (ok && seg_next<TW_ROWS, TW_KEYS>(a, g));
         }
     } else {
@@ -728,13 +742,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         const uint64_t w2 = pack2(w, w);
                         L += x.y * w;
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            uint32_t o[32];
-                            tmem_ld32(O + b * 128 + 32 * q, o);
+                        for (int q = 0; q < 8; q++) {
+                            uint32_t o[16];
+                            tmem_ld16(O + b * 128 + 16 * q, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                acc[16 * q + i] = fma2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), w2, acc[16 * q + i]);
+                            for (int i = 0; i < 8; i++)
+                                acc[8 * q + i] = fma2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), w2, acc[8 * q + i]);
                         }
                     }
                     tc_fence_before();
@@ -829,21 +843,27 @@ static cudaError_t tree_map(CUtensorMap* map, const void* arena, int hkv, int64_
 }
 
 struct TreePlan {
-    int G, rows;
-    size_t o_bytes, ml_bytes, bytes;
+    int G, rows, q_rows, row_tiles;
+    size_t o_bytes, ml_bytes, cut_bytes, q_bytes, e_bytes;
 };
-static TreePlan tree_plan(int hq, int hkv, int max_seq_tokens) {
+static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens) {
     TreePlan p;
     p.G = num_sms();
     const int64_t rows = (int64_t)max_seq_tokens * (hq / hkv);
     p.rows = (int)(rows < TW_ROWS ? rows : TW_ROWS);
+    p.q_rows = (p.rows + 7) / 8 * 8;
+    p.row_tiles = (int)((rows + TW_ROWS - 1) / TW_ROWS);
     p.o_bytes = align256((size_t)2 * p.G * p.rows * HD * 4);
     p.ml_bytes = align256((size_t)2 * p.G * p.rows * 2 * 4);
-    p.bytes = p.o_bytes + p.ml_bytes + align256((size_t)p.G * sizeof(TreeCut));
+    p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
+    const size_t q = (size_t)n_seqs * p.row_tiles * hkv * p.q_rows;
+    p.q_bytes = align256(q * 512);
+    p.e_bytes = align256(q);
     return p;
 }
 size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
-    return tree_plan(hq, hkv, max_seq_tokens).bytes;
+    const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens);
+    return p.o_bytes + p.ml_bytes + p.cut_bytes + p.q_bytes + p.e_bytes;
 }
 
 cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const void* varena, int64_t n_arena_blocks,
@@ -851,7 +871,7 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
                                    const int* ctx, const int64_t* mask, int words, int n_tok, int n_seqs,
                                    int max_seq_tokens, int hq, int hkv, int max_ctx, float scale, float* out,
                                    void* scratch, cudaStream_t st) {
-    const TreePlan p = tree_plan(hq, hkv, max_seq_tokens);
+    const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens);
     TreeArgs a;
     a.q = q;
     a.n_arena_blocks = n_arena_blocks;
@@ -860,15 +880,22 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     a.hq = hq; a.hkv = hkv; a.nrep = hq / hkv;
     a.scale_log2 = scale * LOG2E;
     a.out = out;
-    a.part_o = (float*)scratch;
-    a.part_ml = (float*)((uint8_t*)scratch + p.o_bytes);
-    a.cuts = (TreeCut*)((uint8_t*)scratch + p.o_bytes + p.ml_bytes);
+    uint8_t* at = (uint8_t*)scratch;
+    a.part_o = (float*)at;
+    a.part_ml = (float*)(at += p.o_bytes);
+    a.cuts = (TreeCut*)(at += p.ml_bytes);
+    a.q_tiles = at += p.cut_bytes;
+    a.q_exps = (int8_t*)(at += p.q_bytes);
     a.part_rows = p.rows;
+    a.q_rows = p.q_rows;
+    a.row_tiles = p.row_tiles;
     CUtensorMap km, vm;
     const int64_t n_slots = n_arena_blocks * n_layer * KVB;
     cudaError_t e = tree_map(&km, karena, hkv, n_slots);
     if (e == cudaSuccess) e = tree_map(&vm, varena, hkv, n_slots);
     if (e == cudaSuccess) e = DCG_SMEM_ATTR(tree_wide_kernel, TW_SMEM);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(tree_wide_kernel, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
     if (e != cudaSuccess) return e;
