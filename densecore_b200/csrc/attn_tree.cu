@@ -257,6 +257,13 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
     // D f32 (bits 4-5 = 1), A and B f16 (0), B MN-major (bit 16), N >> 3 at 17-22, M >> 4 at 24-28
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
+// whether phase `parity` of `bar` is over, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, done != 0);
+}
 // one thread of the warp, the same each time
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -466,17 +473,18 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
             int left = g.tiles, seg = 0;
             const uint32_t q_half = a.q_rows * 128;
-            // S of unit n: what it waits for, and the MMAs (issued by the leader)
-            auto wait_s = [&](int n) {
+            // S of unit n begins a segment: its Q
+            auto wait_q = [&](int n) {
                 if (left == 0) {
                     seg_next<TW_ROWS, TW_KEYS>(a, g);
                     left = g.tiles;
                     seg++;
                 }
-                const int qb = seg % q_bufs;
-                if (left == g.tiles) ok = mbar_wait(&C.q_full[qb], (uint32_t)((seg / q_bufs) & 1), &g_tree_error);
-                const uint32_t l = tw_k(n), slot = l % TW_RING;
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error));
+                return mbar_wait(&C.q_full[seg % q_bufs], (uint32_t)((seg / q_bufs) & 1), &g_tree_error);
+            };
+            auto wait_k = [&](int n) {
+                const uint32_t l = tw_k(n);
+                return mbar_wait(&C.full[l % TW_RING], (l / TW_RING) & 1, &g_tree_error);
             };
             auto issue_s = [&](int n) {
                 left--;
@@ -501,24 +509,32 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 }
                 __syncwarp();
             };
-            wait_s(0);
-            if (ok) {
+            for (int n = 0; n < 2 && n < N && ok; n++) {
+                ok = __all_sync(0xffffffffu, (n && left ? true : wait_q(n)) && wait_k(n));
+                if (!ok) break;
                 tc_fence_after();
-                issue_s(0);
-                if (N > 1) wait_s(1);
-            }
-            if (ok && N > 1) {
-                tc_fence_after();
-                issue_s(1);
+                issue_s(n);
             }
             for (int n = 0; n < N && ok; n++) {    // O of unit n, then S of unit n + 2 into the same buffer
                 const int b = n & 1;
                 const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
-                const bool ahead = n + 2 < N && left > 0;   // of the same segment: its K was long asked for
-                ok = mbar_wait(&C.full[slot], (l / TW_RING) & 1, &g_tree_error);
-                if (ok && k) ok = mbar_wait(&C.o_free[b], (k - 1) & 1, &g_tree_error);
-                if (ok && ahead) wait_s(n + 2);
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(&C.p_full[b], k & 1, &g_tree_error));
+                // one poll for all: lane 0 V, 1 O's buffer, 2 the next K (if it is there already), others P
+                uint64_t* bar = &C.p_full[b];
+                uint32_t parity = k & 1;
+                bool wait = true;
+                if (lane == 0) {
+                    bar = &C.full[slot];
+                    parity = (l / TW_RING) & 1;
+                } else if (lane == 1) {
+                    bar = &C.o_free[b];
+                    parity = (k - 1) & 1;
+                    wait = k > 0;
+                } else if (lane == 2) {
+                    wait = false;
+                }
+                ok = __all_sync(0xffffffffu, !wait || mbar_wait(bar, parity, &g_tree_error));
+                const uint32_t lk = tw_k(n + 2);
+                const bool have_k = n + 2 < N && mbar_test(&C.full[lk % TW_RING], (lk / TW_RING) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
@@ -536,9 +552,11 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 }
                 __syncwarp();
                 if (n + 2 < N) {
-                    if (!ahead) wait_s(n + 2);
-                    if (!ok) break;
-                    tc_fence_after();
+                    if (left == 0 || !have_k) {
+                        ok = __all_sync(0xffffffffu, (left ? true : wait_q(n + 2)) && wait_k(n + 2));
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
                     issue_s(n + 2);
                 }
             }
