@@ -221,9 +221,9 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // The tensor core cuts its sums off rather than rounding them, a bias of up to 2^-24 for each MMA that
 // adds to a large accumulator: hence the lo halves first, and no accumulator that lives for longer
 // than a tile (one that lived for a segment was 2-4 x 10^-6 off, this is 4-6 x 10^-7).
-// Two S / P and two O buffers, used in turn.  Warps: 0 TMA producer (ring of 5 x 32 KB, K and V tiles
-// in the order the MMAs take them; pages beyond the sequence load as zeros), 1 MMA issue, 2 the next
-// segment's Q (up to 64 rows into a second buffer), 4-7 and 8-11 softmax of every other tile, 12-15
+// Two S / P and two O buffers, used in turn.  Warps: 0 and 3 TMA producers of K and V (one ring of
+// 5 x 32 KB, in the order the MMAs take them; pages beyond the sequence load as zeros), 1 MMA issue, 2
+// the next segment's Q (up to 64 rows into a second buffer), 4-7 and 8-11 softmax of every other tile, 12-15
 // the running output (128 registers of it per thread, thread = row).  tree_q_kernel has laid Q out
 // before: converting it here cost 20,000 cycles at every change of the item.
 // What bounds it: HBM up to 128 rows per item (64 KB per unit: 2800 cycles of an SM's share, against
@@ -418,52 +418,44 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_CTRL));
         if (N == 0) {
-        } else if (warp == 0) {
-            // ---------------- K and V tiles ----------------
+        } else if (warp == 0 || warp == 3) {
+            // ---------------- K tiles (warp 0), V tiles (warp 3) ----------------
+            // 16 boxes of 2 KB a tile, one for each of 16 lanes: a warp issues one in about 80 cycles
+            const bool is_v = warp == 3;
+            const CUtensorMap* map = is_v ? &vmap : &kmap;
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-            const int page = lane >> 1, half = lane & 1;   // lanes 0-15: one box each
+            const int page = lane >> 1, half = lane & 1;
             const int beyond = (int)(a.n_arena_blocks * a.n_layer * KVB);   // out of the arena: zeros
-            int kt = 0;
-            // block id of this lane's page in a tile, -1 behind the sequence's end (no read)
+            // block id of this lane's page in a tile, INT32_MIN behind the sequence's end (no read)
             auto block = [&](const TreeSeg& s, int tile) {
                 const int p = (s.tile0 + tile) * (TW_KEYS / KVB) + page;
                 return lane < 16 && p * KVB < s.s.L ? a.bt[(int64_t)s.seq * a.mbs + p] : INT32_MIN;
             };
-            auto load = [&](const CUtensorMap* map, int kvh, int b, uint32_t l) {
-                const uint32_t slot = l % TW_RING;
-                if (l >= TW_RING) ok = mbar_wait(&C.empty[slot], (l / TW_RING - 1) & 1, &g_tree_error);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
+            int t = 0, b = block(g, 0), kvh = g.kvh, n = 0;
+            for (; n < N; n++) {
+                const uint32_t l = is_v ? tw_v(n, N) : tw_k(n), slot = l % TW_RING;
                 const bool in = b >= 0 && b < a.n_arena_blocks;
                 if (!in && b != INT32_MIN) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
-                const int row = in ? (b * a.n_layer + a.layer) * KVB : beyond;
+                const int row = in ? (b * a.n_layer + a.layer) * KVB : beyond, head = kvh;
+                if (++t == g.tiles) {
+                    t = 0;
+                    if (n + 1 < N) seg_next<TW_ROWS, TW_KEYS>(a, g);
+                }
+                if (n + 1 < N) {                   // on its way while the ring is waited for
+                    b = block(g, t);
+                    kvh = g.kvh;
+                }
+                ok = __all_sync(0xffffffffu, l < TW_RING || mbar_wait(&C.empty[slot], (l / TW_RING - 1) & 1, &g_tree_error));
+                if (!ok) break;
                 if (lane == 0) mbar_arrive_expect_tx(&C.full[slot], TW_BUF);
                 __syncwarp();
-                if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, kvh, &C.full[slot]);
-            };
-            uint32_t l = 0;
-            int b_now = block(g, 0), h_now = g.kvh, b_last = 0, h_last = 0;
-            for (int n = 0; n <= N && ok; n++) {           // V runs one unit behind K
-                int b_next = 0, h_next = 0;
-                if (n < N) {
-                    load(&kmap, h_now, b_now, l++);
-                    if (++kt == g.tiles) {
-                        kt = 0;
-                        if (n + 1 < N) seg_next<TW_ROWS, TW_KEYS>(a, g);
-                    }
-                    if (n + 1 < N) {                       // on its way while the ring is waited for
-                        b_next = block(g, kt);
-                        h_next = g.kvh;
-                    }
-                }
-                if (n > 0 && ok) load(&vmap, h_last, b_last, l++);
-                b_last = b_now;
-                h_last = h_now;
-                b_now = b_next;
-                h_now = h_next;
+                if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, head, &C.full[slot]);
             }
             if (!ok)                               // given up: the copies in flight land before the CTA ends
-                for (uint32_t i = l > TW_RING ? l - TW_RING : 0; i < l; i++) mbar_wait(&C.full[i % TW_RING], (i / TW_RING) & 1, &g_tree_error, 1u << 16);
+                for (int i = max(0, n - TW_RING); i < n; i++) {
+                    const uint32_t l = is_v ? tw_v(i, N) : tw_k(i);
+                    mbar_wait(&C.full[l % TW_RING], (l / TW_RING) & 1, &g_tree_error, 1u << 16);
+                }
         } else if (warp == 1) {
             // ---------------- MMA issue: the warp in step, one elected thread issues ----------------
             constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
@@ -820,22 +812,40 @@ __global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeAr
     const TreeCut cut = a.cuts[c];
     if (r >= cut.rows) return;
     const int last = (int)sk_owner(cut.end - 1, cut.T, G);
+    // the parts' m and l 32 at a time (a lane each), then their outputs, all loads apart from the sums
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int x = c; x <= last; x++) {
-        if (sk_begin(x, cut.T, G) == sk_begin(x + 1, cut.T, G)) continue;
+    for (int x0 = c; x0 <= last; x0 += 32) {
+        const int x = x0 + lane;
         const size_t part = ((size_t)x * 2 + (x == c ? 1 : 0)) * a.part_rows + r;
-        const float m = a.part_ml[part * 2], l = a.part_ml[part * 2 + 1];
-        const float4 y = *(const float4*)(a.part_o + part * HD + 4 * lane);
-        if (l == 0.0f) continue;
-        const float mn = fmaxf(M, m), f = M == -INFINITY ? 0.0f : ex2(M - mn), e = ex2(m - mn);
-        M = mn;
-        L = L * f + l * e;
-        o.x = o.x * f + y.x * e;
-        o.y = o.y * f + y.y * e;
-        o.z = o.z * f + y.z * e;
-        o.w = o.w * f + y.w * e;
+        float2 y = make_float2(-INFINITY, 0.0f);
+        if (x <= last && sk_begin(x, cut.T, G) < sk_begin(x + 1, cut.T, G)) y = *(const float2*)(a.part_ml + part * 2);
+        float m = fmaxf(M, y.x);
+#pragma unroll
+        for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+        const float f = M == -INFINITY ? 0.0f : ex2(M - m), w = y.y == 0.0f ? 0.0f : ex2(y.x - m);
+        float l = y.y * w;
+#pragma unroll
+        for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+        M = m;
+        L = L * f + l;
+        o.x *= f;
+        o.y *= f;
+        o.z *= f;
+        o.w *= f;
+        const int n = min(32, last - x0 + 1);
+        const uint32_t used = __ballot_sync(0xffffffffu, y.y != 0.0f);   // others left nothing to read
+#pragma unroll 8
+        for (int i = 0; i < n; i++) {
+            if (!((used >> i) & 1)) continue;
+            const float v = __shfl_sync(0xffffffffu, w, i);
+            const size_t p = ((size_t)(x0 + i) * 2 + (x0 + i == c ? 1 : 0)) * a.part_rows + r;
+            const float4 z = *(const float4*)(a.part_o + p * HD + 4 * lane);
+            o.x += z.x * v;
+            o.y += z.y * v;
+            o.z += z.z * v;
+            o.w += z.w * v;
+        }
     }
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
     const int R = cut.row0 + r;
