@@ -221,10 +221,10 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // The tensor core cuts its sums off rather than rounding them, a bias of up to 2^-24 for each MMA that
 // adds to a large accumulator: hence the lo halves first, and no accumulator that lives for longer
 // than a tile (one that lived for a segment was 2-4 x 10^-6 off, this is 4-6 x 10^-7).
-// Two S / P and two O buffers, used in turn.  Warps: 0 and 3 TMA producers of K and V (one ring of
-// 5 x 32 KB, in the order the MMAs take them; pages beyond the sequence load as zeros), 1 MMA issue, 2
-// the next segment's Q (up to 64 rows into a second buffer), 4-7 and 8-11 softmax of every other tile, 12-15
-// the running output (128 registers of it per thread, thread = row).  tree_q_kernel has laid Q out
+// Two S / P and two O buffers, used in turn.  Warps: 0 and 3 TMA producers of K (and each segment's Q,
+// up to 64 rows into a second buffer) and V (one ring of 5 x 32 KB, in the order the MMAs take them;
+// pages beyond the sequence load as zeros), 1 and 2 MMA issue for every other tile, 4-7 and 8-11 its
+// softmax, 12-15 the running output (128 registers of it per thread, thread = row).  tree_q_kernel has laid Q out
 // before: converting it here cost 20,000 cycles at every change of the item.
 // What bounds it: HBM up to 128 rows per item (64 KB per unit: 2800 cycles of an SM's share, against
 // 32 MMAs of 64 cycles); beyond, the tensor core.
@@ -246,7 +246,7 @@ static_assert(TW_REGS_CTRL + 2 * TW_REGS_SOFT + TW_REGS_OUT <= 512, "register sp
 
 struct TwCtrl {
     uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_full[2], o_free[2], x_free[2], cleaned[2];
-    uint64_t q_full[2], q_empty[2], mma_done;
+    uint64_t q_full[2], q_empty[2][2], mma_end[2];   // q_empty: by MMA warp and buffer
     uint32_t tmem;
     uint32_t bad[2][4];                           // per buffer: keys of its tile whose V is not finite
     float2 x[2][TW_ROWS];                         // a tile's row max and sum of p
@@ -391,9 +391,10 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             mbar_init(&C.x_free[b], 4);
             mbar_init(&C.cleaned[b], 4);
             mbar_init(&C.q_full[b], 1);
-            mbar_init(&C.q_empty[b], 1);
+            mbar_init(&C.q_empty[0][b], 1);
+            mbar_init(&C.q_empty[1][b], 1);
+            mbar_init(&C.mma_end[b], 1);
         }
-        mbar_init(&C.mma_done, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_CTRL));
         if (N == 0) {
         } else if (warp == 0 || warp == 3) {
-            // ---------------- K tiles (warp 0), V tiles (warp 3) ----------------
+            // ---------------- Q and K tiles (warp 0), V tiles (warp 3) ----------------
             // 16 boxes of 2 KB a tile, one for each of 16 lanes: a warp issues one in about 80 cycles
             const bool is_v = warp == 3;
             const CUtensorMap* map = is_v ? &vmap : &kmap;
@@ -431,14 +432,28 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 const int p = (s.tile0 + tile) * (TW_KEYS / KVB) + page;
                 return lane < 16 && p * KVB < s.s.L ? a.bt[(int64_t)s.seq * a.mbs + p] : INT32_MIN;
             };
-            int t = 0, b = block(g, 0), kvh = g.kvh, n = 0;
+            int t = 0, b = block(g, 0), kvh = g.kvh, n = 0, seg = 0;
+            bool begins = true;
             for (; n < N; n++) {
                 const uint32_t l = is_v ? tw_v(n, N) : tw_k(n), slot = l % TW_RING;
                 const bool in = b >= 0 && b < a.n_arena_blocks;
                 if (!in && b != INT32_MIN) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
                 const int row = in ? (b * a.n_layer + a.layer) * KVB : beyond, head = kvh;
+                if (begins && !is_v) {             // the segment's Q, ahead of its first K
+                    const int qb = seg % q_bufs;
+                    const int64_t q_tile = ((int64_t)g.seq * a.row_tiles + g.rt) * a.hkv + g.kvh;
+                    ok = __all_sync(0xffffffffu, seg < q_bufs || mbar_wait(&C.q_empty[lane & 1][qb], (uint32_t)((seg / q_bufs - 1) & 1), &g_tree_error));
+                    if (!ok) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&C.q_full[qb], (uint32_t)q_bytes);
+                        bulk_g2s(smem + qb * q_bytes, a.q_tiles + q_tile * q_bytes, (uint32_t)q_bytes, &C.q_full[qb]);
+                    }
+                    seg++;
+                }
+                begins = false;
                 if (++t == g.tiles) {
                     t = 0;
+                    begins = true;
                     if (n + 1 < N) seg_next<TW_ROWS, TW_KEYS>(a, g);
                 }
                 if (n + 1 < N) {                   // on its way while the ring is waited for
@@ -451,37 +466,49 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 __syncwarp();
                 if (lane < 16) tma_load_4d(ring + (size_t)slot * TW_BUF + half * TW_HALF + page * 2048, map, 0, row, half, head, &C.full[slot]);
             }
-            if (!ok)                               // given up: the copies in flight land before the CTA ends
+            if (!ok) {                             // given up: the copies in flight land before the CTA ends
+                if (!is_v)
+                    for (int i = max(0, seg - q_bufs); i < seg; i++) mbar_wait(&C.q_full[i % q_bufs], (uint32_t)((i / q_bufs) & 1), &g_tree_error, 1u << 16);
                 for (int i = max(0, n - TW_RING); i < n; i++) {
                     const uint32_t l = is_v ? tw_v(i, N) : tw_k(i);
                     mbar_wait(&C.full[l % TW_RING], (l / TW_RING) & 1, &g_tree_error, 1u << 16);
                 }
-        } else if (warp == 1) {
-            // ---------------- MMA issue: the warp in step, one elected thread issues ----------------
+            }
+        } else {
+            // ---------------- MMA issue: warp 1 the even units, warp 2 the odd ones ----------------
+            // Each in step, one elected thread issuing.  A warp's polls, and its waits for the tensor core to
+            // take its last operands, leave the core with the other's work.
             constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
-            const uint32_t qh = smem_u32(smem), rg = qh + TW_OFF_RING;
+            const uint32_t qs = smem_u32(smem), rg = qs + TW_OFF_RING, q_half = a.q_rows * 128;
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const bool leader = elect_one();
+            const int b = warp - 1;
+            const uint32_t S = tm + b * 128, O = tm + 256 + b * 128;   // P takes S's place
             TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-            int left = g.tiles, seg = 0;
-            const uint32_t q_half = a.q_rows * 128;
-            // S of unit n begins a segment: its Q
-            auto wait_q = [&](int n) {
-                if (left == 0) {
+            int seg = 0, end = g.tiles;            // the segment's end among the range's units
+            bool begins = true;                    // its Q not waited for yet
+            uint64_t* q_empty = C.q_empty[b];
+            // S of unit n
+            auto issue_s = [&](int n, bool have_k) {
+                while (n >= end) {                 // (a segment that has no unit of this warp: given back at once)
+                    if (begins && leader) tc_commit(&q_empty[seg % q_bufs]);
                     seg_next<TW_ROWS, TW_KEYS>(a, g);
-                    left = g.tiles;
                     seg++;
+                    end += g.tiles;
+                    begins = true;
                 }
-                return mbar_wait(&C.q_full[seg % q_bufs], (uint32_t)((seg / q_bufs) & 1), &g_tree_error);
-            };
-            auto wait_k = [&](int n) {
-                const uint32_t l = tw_k(n);
-                return mbar_wait(&C.full[l % TW_RING], (l / TW_RING) & 1, &g_tree_error);
-            };
-            auto issue_s = [&](int n) {
-                left--;
+                const int qb = seg % q_bufs;
+                const uint32_t l = tw_k(n), slot = l % TW_RING;
+                uint64_t* bar = lane == 0 ? &C.q_full[qb] : &C.full[slot];
+                const uint32_t parity = lane == 0 ? (uint32_t)((seg / q_bufs) & 1) : (l / TW_RING) & 1;
+                if (begins || !have_k) {
+                    ok = __all_sync(0xffffffffu, (lane == 0 && !begins) || mbar_wait(bar, parity, &g_tree_error));
+                    if (!ok) return;
+                    begins = false;
+                    tc_fence_after();
+                }
                 if (leader) {
-                    const uint32_t slot = tw_k(n) % TW_RING, S = tm + (n & 1) * 128, q = qh + (seg % q_bufs) * q_bytes;
+                    const uint32_t q = qs + qb * q_bytes;
                     const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
 #pragma unroll
                     for (int h = 1; h >= 0; h--) {   // the lo half first
@@ -495,22 +522,17 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                             }
                         }
                     }
-                    tc_commit(&C.s_full[n & 1]);
+                    tc_commit(&C.s_full[b]);
                     tc_commit(&C.empty[slot]);
-                    if (left == 0) tc_commit(&C.q_empty[seg % q_bufs]);
+                    if (n + 2 >= end) tc_commit(&q_empty[qb]);
                 }
                 __syncwarp();
             };
-            for (int n = 0; n < 2 && n < N && ok; n++) {
-                ok = __all_sync(0xffffffffu, (n && left ? true : wait_q(n)) && wait_k(n));
-                if (!ok) break;
-                tc_fence_after();
-                issue_s(n);
-            }
-            for (int n = 0; n < N && ok; n++) {    // O of unit n, then S of unit n + 2 into the same buffer
-                const int b = n & 1;
+            if (b < N) issue_s(b, false);
+            for (int n = b; n < N && ok; n += 2) {  // O of unit n, then S of unit n + 2 into the same buffer
                 const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
-                // one poll for all: lane 0 V, 1 O's buffer, 2 the next K (if it is there already), others P
+                // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit, others P.  (The third keeps the
+                // two streams half a period apart: side by side, both softmaxes leave the tensor core idle.)
                 uint64_t* bar = &C.p_full[b];
                 uint32_t parity = k & 1;
                 bool wait = true;
@@ -522,56 +544,33 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     parity = (k - 1) & 1;
                     wait = k > 0;
                 } else if (lane == 2) {
-                    wait = false;
+                    bar = &C.s_full[b ^ 1];
+                    parity = ((uint32_t)(n + 1) >> 1) & 1;
+                    wait = n + 1 < N;
                 }
                 ok = __all_sync(0xffffffffu, !wait || mbar_wait(bar, parity, &g_tree_error));
-                const uint32_t lk = tw_k(n + 2);
-                const bool have_k = n + 2 < N && mbar_test(&C.full[lk % TW_RING], (lk / TW_RING) & 1);
                 if (!ok) break;
+                const uint32_t lk = tw_k(n + 2);   // S of unit n + 2 follows at once if its K is there
+                const bool have_k = n + 2 < N && mbar_test(&C.full[lk % TW_RING], (lk / TW_RING) & 1);
                 tc_fence_after();
                 if (leader) {
-                    const uint32_t P = tm + b * 128, O = tm + 256 + b * 128;
                     const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
 #pragma unroll
                     for (int h = 1; h >= 0; h--)   // 16 keys = 2048 bytes per k-step
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            if (h && j == 0) mma_f16_ts<false>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
-                            else mma_f16_ts<true>(O, P + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                            if (h && j == 0) mma_f16_ts<false>(O, S + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                            else mma_f16_ts<true>(O, S + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
                         }
                     tc_commit(&C.o_full[b]);
                     tc_commit(&C.empty[slot]);
                 }
                 __syncwarp();
-                if (n + 2 < N) {
-                    if (left == 0 || !have_k) {
-                        ok = __all_sync(0xffffffffu, (left ? true : wait_q(n + 2)) && wait_k(n + 2));
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    issue_s(n + 2);
-                }
+                if (n + 2 < N) issue_s(n + 2, have_k);
             }
-            if (leader) tc_commit(&C.mma_done);
+            if (leader) tc_commit(&C.mma_end[b]);
             __syncwarp();
-            mbar_wait(&C.mma_done, 0, &g_tree_error);
-        } else if (warp == 2) {
-            // ---------------- Q of each segment ----------------
-            if (lane == 0) {
-                TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
-                int seg = 0;
-                do {
-                    const int qb = seg % q_bufs;
-                    if (seg >= q_bufs) ok = mbar_wait(&C.q_empty[qb], (uint32_t)((seg / q_bufs - 1) & 1), &g_tree_error);
-                    if (!ok) break;
-                    const int64_t tile = ((int64_t)g.seq * a.row_tiles + g.rt) * a.hkv + g.kvh;
-                    mbar_arrive_expect_tx(&C.q_full[qb], (uint32_t)q_bytes);
-                    bulk_g2s(smem + qb * q_bytes, a.q_tiles + tile * q_bytes, (uint32_t)q_bytes, &C.q_full[qb]);
-                    seg++;
-                } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
-                if (!ok)
-                    for (int i = seg > q_bufs ? seg - q_bufs : 0; i < seg; i++) mbar_wait(&C.q_full[i % q_bufs], (uint32_t)((i / q_bufs) & 1), &g_tree_error, 1u << 16);
-            }
+            mbar_wait(&C.mma_end[b], 0, &g_tree_error);
         }
     } else if (warp < 12) {
         // ---------------- softmax of every other tile (thread = row) ----------------
