@@ -801,24 +801,350 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     pdl_trigger();
 }
 
-// Parts of an item that several CTAs worked on: out = sum O_c 2^(m_c - M) / sum l_c 2^(m_c - M), in CTA
-// order.  One CTA per (CTA that began an item, 8 rows); a warp is a row, a lane 4 dims.
-constexpr int TC_ROWS = 8;
-__global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeArgs a, int G) {
+// ------------------------------------------------------------------------------------------
+// tree_few_kernel<MT>: up to 16 MT rows per kv head (a chain of drafts, a small tree), mma.sync.
+// With so few rows the K/V bytes are all that counts, and a warp that owns whole blocks of 16 keys has
+// no hand-over to wait for: one CTA (3 consumer warps, 1 TMA producer warp, 2 CTAs per SM) per
+// (sequence, kv head, split of its blocks), consumer warp w takes blocks w, w + 3, ... from a ring of
+// whole blocks.  Per block: S = Q K^T and P V on m16n8k16, q and p as fp16 halves (hi + lo) as in the
+// wide kernel; a block's P V starts from zero and is added to the running output in fp32 rounded to
+// nearest, because the tensor core cuts its sums off.  The warps merge in shared memory; splits leave
+// their parts for tree_join_kernel.
+// ------------------------------------------------------------------------------------------
+constexpr int TF_CONS = 3;
+constexpr int TF_STAGES = 9;
+constexpr int TF_TILE = KVB * HD * 2;             // 4 KB: [half of 64 dims][16 keys][128 B]
+constexpr int TF_STAGE = 2 * TF_TILE;             // K, V
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+__device__ __forceinline__ void mma_h(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// byte address of 16-byte chunk c (of 16) of row r in a swizzled tile
+__device__ __forceinline__ uint32_t tf_at(uint32_t tile, int r, int c) {
+    return tile + (uint32_t)(c >> 3) * (TF_TILE / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+template <int MT>
+__global__ void __launch_bounds__((TF_CONS + 1) * 32, 2) tree_few_kernel(
+    const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TreeArgs a, int bps, int splits) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* ring = smem;
+    uint4* qf = (uint4*)(smem + TF_STAGES * TF_STAGE);            // [MT][k-step][hi, lo][lane]
+    uint64_t* full = (uint64_t*)(qf + MT * 8 * 2 * 32);
+    uint64_t* empty = full + TF_STAGES;
+    float* wm = (float*)(empty + TF_STAGES);                       // [warp][row]
+    float* wl = wm + TF_CONS * 16 * MT;
+    float* qc = wl + TF_CONS * 16 * MT;                            // [row] scale of the scores, in powers of 2
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int gid = lane >> 2, tig = lane & 3;
+    if (smem_u32(smem) & 1023) {                  // the swizzled tiles would not match their addresses
+        if (threadIdx.x == 0) atomicExch(&g_tree_error, DCG_DEVERR_TIMEOUT);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < TF_STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        fence_mbar_init();
+    }
     pdl_wait();
+    const int seq = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv;
+    const TreeSeq s = tree_seq<16 * MT, KVB>(a, seq, kvh == 0 && blockIdx.y == 0);
+    const int rows = s.ns * a.nrep, hist = s.L - s.ns;
+    const int b0 = blockIdx.y * bps, nb = max(0, min(s.tiles, b0 + bps) - b0);
+    if (rows == 0) return;                        // no drafted tokens, or a sequence that is out of range
+    // Q as A fragments: k-step j holds dims 16 j .. +15; rows gid (a0, a2) and gid + 8 (a1, a3).  Warp w
+    // makes row tile w.
+    if (warp < MT) {
+        const float* q[2];
+        float2 x[2][16];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = min(16 * warp + gid + 8 * h, rows - 1);
+            q[h] = a.q + ((int64_t)(s.s0 + r / a.nrep) * a.hq + kvh * a.nrep + r % a.nrep) * HD + 2 * tig;
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[h][j] = *(const float2*)(q[h] + 8 * j);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j++) m = fmaxf(m, fmaxf(fabsf(x[h][j].x), fabsf(x[h][j].y)));
+            uint32_t u = __float_as_uint(m);      // also of NaN and infinities, which make the row NaN
+            u = max(u, __shfl_xor_sync(0xffffffffu, u, 1));
+            u = max(u, __shfl_xor_sync(0xffffffffu, u, 2));
+            int e = (int)(u >> 23) - 127;
+            e = e < -100 ? -100 : e > 120 ? 120 : e;
+            const float f = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);
+            if (tig == 0) qc[16 * warp + gid + 8 * h] = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23), 1e-37f);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                x[h][j].x *= f;
+                x[h][j].y *= f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            uint4 hi, lo;
+            cut_h2(x[0][2 * j].x, x[0][2 * j].y, hi.x, lo.x);
+            cut_h2(x[1][2 * j].x, x[1][2 * j].y, hi.y, lo.y);
+            cut_h2(x[0][2 * j + 1].x, x[0][2 * j + 1].y, hi.z, lo.z);
+            cut_h2(x[1][2 * j + 1].x, x[1][2 * j + 1].y, hi.w, lo.w);
+            qf[((warp * 8 + j) * 2) * 32 + lane] = hi;
+            qf[((warp * 8 + j) * 2 + 1) * 32 + lane] = lo;
+        }
+    }
+    __syncthreads();
+
+    bool ok = true;
+    float o[MT][16][4];                           // [row tile][8 dims][rows gid (0, 1) and gid + 8 (2, 3)]
+    float m[MT][2], l[MT][2];
+    uint32_t poison = 0;
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+#pragma unroll
+        for (int n = 0; n < 16; n++) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.0f;
+        m[t][0] = m[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.0f;
+    }
+    if (warp == TF_CONS) {
+        if (lane == 0) {
+            const int beyond = (int)(a.n_arena_blocks * a.n_layer * KVB);   // out of the arena: zeros
+            const int* bt = a.bt + (int64_t)seq * a.mbs + b0;
+            int next = nb ? bt[0] : 0, i = 0;
+            for (; i < nb; i++) {
+                const int st = i % TF_STAGES, b = next;
+                if (i + 1 < nb) next = bt[i + 1];
+                const bool in = b >= 0 && b < a.n_arena_blocks;
+                if (!in) atomicExch(&g_tree_error, DCG_DEVERR_INDEX);
+                const int row = in ? (b * a.n_layer + a.layer) * KVB : beyond;
+                if (i >= TF_STAGES) ok = mbar_wait(&empty[st], (uint32_t)((i / TF_STAGES - 1) & 1), &g_tree_error);
+                if (!ok) break;
+                mbar_arrive_expect_tx(&full[st], TF_STAGE);
+                tma_load_4d(ring + (size_t)st * TF_STAGE, &kmap, 0, row, 0, kvh, &full[st]);
+                tma_load_4d(ring + (size_t)st * TF_STAGE + TF_TILE, &vmap, 0, row, 0, kvh, &full[st]);
+            }
+            if (!ok)                               // given up: the copies in flight land before the CTA ends
+                for (int x = max(0, i - TF_STAGES); x < i; x++) mbar_wait(&full[x % TF_STAGES], (uint32_t)((x / TF_STAGES) & 1), &g_tree_error, 1u << 16);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+    } else {
+        const uint32_t ring_s = smem_u32(ring);
+        const int mi = lane >> 3, mr = lane & 7;  // ldmatrix: matrix, row in it
+        float c[MT][2];
+        int tok[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                c[t][h] = qc[16 * t + gid + 8 * h];
+                tok[t][h] = s.s0 + min(16 * t + gid + 8 * h, rows - 1) / a.nrep;
+            }
+        for (int i = warp; i < nb; i += TF_CONS) {
+            const int st = i % TF_STAGES;
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)((i / TF_STAGES) & 1), &g_tree_error));
+            if (!ok) break;
+            const uint32_t kt = ring_s + (uint32_t)st * TF_STAGE, vt = kt + TF_TILE;
+            const int kb = (b0 + i) * KVB;
+            // ---- S: lane has rows gid, gid + 8 and keys 8 n + 2 tig, + 1 ----
+            float sh[MT][2][4], sl[MT][2][4];
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sh[t][n][e] = sl[t][n][e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                uint32_t k0, k1, k2, k3;
+                ldsm_x4(tf_at(kt, (mi >> 1) * 8 + mr, 2 * j + (mi & 1)), k0, k1, k2, k3);
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    const uint4 hi = qf[((t * 8 + j) * 2) * 32 + lane], lo = qf[((t * 8 + j) * 2 + 1) * 32 + lane];
+                    mma_h(sh[t][0], hi, k0, k1);
+                    mma_h(sl[t][0], lo, k0, k1);
+                    mma_h(sh[t][1], hi, k2, k3);
+                    mma_h(sl[t][1], lo, k2, k3);
+                }
+            }
+            // ---- masks, and V that must not reach the sums ----
+            uint32_t vm01 = 0xFFFFFFFFu, vm23 = 0xFFFFFFFFu;   // V of keys 2 tig, +1 and 8 + 2 tig, +1
+            uint32_t vis[MT][2];
+            const bool special = kb + KVB > hist;
+            if (special) {
+                // V of slots past the context may be anything, and that of a drafted token that a row does
+                // not see may be NaN: 0 x NaN is NaN, so such V count as zeros
+                bool odd = false;
+                const int key = kb + (lane >> 1);
+                if (key >= hist && key < s.L) {
+                    const uint32_t v = vt + (lane & 1) * (TF_TILE / 2) + (lane >> 1) * 128;
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        uint32_t y[4];
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]) : "r"(v + ((x + lane) & 7) * 16));
+#pragma unroll
+                        for (int e = 0; e < 4; e++) odd |= (y[e] & 0x7C00u) == 0x7C00u || (y[e] & 0x7C000000u) == 0x7C000000u;
+                    }
+                }
+                const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+                uint32_t bad = 0;                  // bit per key
+#pragma unroll
+                for (int x = 0; x < KVB; x++) bad |= ((odds >> (2 * x)) & 3u ? 1u : 0u) << x;
+                const int n = s.L - kb;
+                const uint32_t none = bad | (n >= KVB ? 0u : 0xFFFFu << n);
+                vm01 = ((none >> (2 * tig)) & 1 ? 0u : 0x0000FFFFu) | ((none >> (2 * tig + 1)) & 1 ? 0u : 0xFFFF0000u);
+                vm23 = ((none >> (8 + 2 * tig)) & 1 ? 0u : 0x0000FFFFu) | ((none >> (9 + 2 * tig)) & 1 ? 0u : 0xFFFF0000u);
+#pragma unroll
+                for (int t = 0; t < MT; t++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        vis[t][h] = tree_bits(a, s, tok[t][h], kb);
+                        if (vis[t][h] & bad) poison |= 1u << (2 * t + h);
+                    }
+            }
+            // ---- p, and its halves as A fragments ----
+            uint4 ph[MT], pl[MT];
+            float corr[MT][2];
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                float p[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float v = sh[t][n][2 * h + e] + sl[t][n][2 * h + e];
+                            if (special && !((vis[t][h] >> (8 * n + 2 * tig + e)) & 1)) v = -INFINITY;
+                            p[n][2 * h + e] = v;
+                            mx = fmaxf(mx, v);
+                        }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float mn = fmaxf(m[t][h], mx * c[t][h]);
+                    corr[t][h] = mn == -INFINITY ? 1.0f : ex2(m[t][h] - mn);
+                    m[t][h] = mn;
+                    const float shift = TW_SHIFT - (mn == -INFINITY ? 0.0f : mn);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            p[n][2 * h + e] = ex2(fmaf(p[n][2 * h + e], c[t][h], shift));
+                            sum += p[n][2 * h + e];
+                        }
+                    l[t][h] = l[t][h] * corr[t][h] + sum;   // this lane's four keys; the lanes are joined at the end
+                }
+                cut_h2(p[0][0], p[0][1], ph[t].x, pl[t].x);
+                cut_h2(p[0][2], p[0][3], ph[t].y, pl[t].y);
+                cut_h2(p[1][0], p[1][1], ph[t].z, pl[t].z);
+                cut_h2(p[1][2], p[1][3], ph[t].w, pl[t].w);
+            }
+            // ---- O = O corr + P V ----
+#pragma unroll
+            for (int n2 = 0; n2 < 8; n2++) {
+                uint32_t v0, v1, v2, v3;
+                ldsm_x4_t(tf_at(vt, (mi & 1) * 8 + mr, 2 * n2 + (mi >> 1)), v0, v1, v2, v3);
+                v0 &= vm01;
+                v2 &= vm01;
+                v1 &= vm23;
+                v3 &= vm23;
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    float y0[4] = {0.f, 0.f, 0.f, 0.f}, y1[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_h(y0, pl[t], v0, v1);
+                    mma_h(y1, pl[t], v2, v3);
+                    mma_h(y0, ph[t], v0, v1);
+                    mma_h(y1, ph[t], v2, v3);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        o[t][2 * n2][e] = fmaf(o[t][2 * n2][e], corr[t][e >> 1], y0[e]);
+                        o[t][2 * n2 + 1][e] = fmaf(o[t][2 * n2 + 1][e], corr[t][e >> 1], y1[e]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+    }
     pdl_trigger();
-    const int c = blockIdx.x, r = blockIdx.y * TC_ROWS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const TreeCut cut = a.cuts[c];
-    if (r >= cut.rows) return;
-    const int last = (int)sk_owner(cut.end - 1, cut.T, G);
-    // the parts' m and l 32 at a time (a lane each), then their outputs, all loads apart from the sums
+    ok = __syncthreads_and(ok);
+    if (!ok) return;
+    // ---- merge the consumer warps: the ring becomes [warp][row][dim] ----
+    float* acc = (float*)ring;
+    static_assert(TF_CONS * 16 * MT * HD * 4 <= TF_STAGES * TF_STAGE, "merge space");
+    if (warp < TF_CONS) {
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int r = 16 * t + gid + 8 * h;
+                float x = l[t][h];
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                if ((poison >> (2 * t + h)) & 1) x = NAN;
+                if (tig == 0) {
+                    wm[warp * 16 * MT + r] = m[t][h];
+                    wl[warp * 16 * MT + r] = x;
+                }
+#pragma unroll
+                for (int n = 0; n < 16; n++)
+                    *(float2*)&acc[(warp * 16 * MT + r) * HD + 8 * n + 2 * tig] = make_float2(o[t][n][2 * h], o[t][n][2 * h + 1]);
+            }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < rows * (HD / 4); x += (TF_CONS + 1) * 32) {
+        const int r = x / (HD / 4), d = x % (HD / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < TF_CONS; w++) M = fmaxf(M, wm[w * 16 * MT + r]);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < TF_CONS; w++) {
+            const float lw = wl[w * 16 * MT + r], f = lw != 0.0f ? ex2(wm[w * 16 * MT + r] - M) : 0.0f;
+            if (lw == 0.0f) continue;
+            const float4 z = *(const float4*)&acc[(w * 16 * MT + r) * HD + d];
+            L += lw * f;
+            y.x += z.x * f;
+            y.y += z.y * f;
+            y.z += z.z * f;
+            y.w += z.w * f;
+        }
+        if (splits == 1) {
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            *(float4*)(a.out + ((int64_t)(s.s0 + r / a.nrep) * a.hq + kvh * a.nrep + r % a.nrep) * HD + d) =
+                make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+        } else {
+            const size_t part = ((size_t)blockIdx.x * splits + blockIdx.y) * a.part_rows + r;
+            *(float4*)(a.part_o + part * HD + d) = y;
+            if (d == 0) *(float2*)(a.part_ml + part * 2) = make_float2(M, L);
+        }
+    }
+}
+
+// The parts of a row, 32 at a time: m and l a lane each, then the outputs with all loads apart from the
+// sums (a lane 4 dims).  part(x): index of the x-th part, or -1 if it left nothing.
+template <class F>
+__device__ __forceinline__ void tree_join(const TreeArgs& a, int parts, F part, float* dst) {
+    const int lane = threadIdx.x & 31;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int x0 = c; x0 <= last; x0 += 32) {
-        const int x = x0 + lane;
-        const size_t part = ((size_t)x * 2 + (x == c ? 1 : 0)) * a.part_rows + r;
+    for (int x0 = 0; x0 < parts; x0 += 32) {
+        const int64_t p = x0 + lane < parts ? part(x0 + lane) : -1;
         float2 y = make_float2(-INFINITY, 0.0f);
-        if (x <= last && sk_begin(x, cut.T, G) < sk_begin(x + 1, cut.T, G)) y = *(const float2*)(a.part_ml + part * 2);
+        if (p >= 0) y = *(const float2*)(a.part_ml + p * 2);
         float m = fmaxf(M, y.x);
 #pragma unroll
         for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
@@ -832,14 +1158,14 @@ __global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeAr
         o.y *= f;
         o.z *= f;
         o.w *= f;
-        const int n = min(32, last - x0 + 1);
+        const int n = min(32, parts - x0);
         const uint32_t used = __ballot_sync(0xffffffffu, y.y != 0.0f);   // others left nothing to read
 #pragma unroll 8
         for (int i = 0; i < n; i++) {
             if (!((used >> i) & 1)) continue;
             const float v = __shfl_sync(0xffffffffu, w, i);
-            const size_t p = ((size_t)(x0 + i) * 2 + (x0 + i == c ? 1 : 0)) * a.part_rows + r;
-            const float4 z = *(const float4*)(a.part_o + p * HD + 4 * lane);
+            const int64_t q = __shfl_sync(0xffffffffu, p, i);
+            const float4 z = *(const float4*)(a.part_o + q * HD + 4 * lane);
             o.x += z.x * v;
             o.y += z.y * v;
             o.z += z.z * v;
@@ -847,20 +1173,46 @@ __global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeAr
         }
     }
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    *(float4*)(dst + 4 * lane) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// tree_few_kernel's splits: a warp per row, CTA (sequence and kv head, 8 rows)
+constexpr int TC_ROWS = 8;
+__global__ void __launch_bounds__(TC_ROWS * 32) tree_join_kernel(const TreeArgs a, int splits) {
+    pdl_wait();
+    pdl_trigger();
+    const int seq = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, r = blockIdx.y * TC_ROWS + (threadIdx.x >> 5);
+    const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, seq, false);
+    if (r >= s.ns * a.nrep) return;
+    tree_join(a, splits, [&](int x) { return ((int64_t)blockIdx.x * splits + x) * a.part_rows + r; },
+              a.out + ((int64_t)(s.s0 + r / a.nrep) * a.hq + kvh * a.nrep + r % a.nrep) * HD);
+}
+
+// tree_wide_kernel's items that several CTAs worked on, in CTA order: CTA (CTA that began an item, 8 rows)
+__global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeArgs a, int G) {
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, r = blockIdx.y * TC_ROWS + (threadIdx.x >> 5);
+    const TreeCut cut = a.cuts[c];
+    if (r >= cut.rows) return;
     const int R = cut.row0 + r;
-    float* dst = a.out + ((int64_t)(cut.s0 + R / a.nrep) * a.hq + cut.kvh * a.nrep + R % a.nrep) * HD + 4 * lane;
-    *(float4*)dst = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    tree_join(a, (int)sk_owner(cut.end - 1, cut.T, G) - c + 1,
+              [&](int x) {
+                  if (sk_begin(c + x, cut.T, G) == sk_begin(c + x + 1, cut.T, G)) return (int64_t)-1;
+                  return ((int64_t)(c + x) * 2 + (x == 0 ? 1 : 0)) * a.part_rows + r;
+              },
+              a.out + ((int64_t)(cut.s0 + R / a.nrep) * a.hq + cut.kvh * a.nrep + R % a.nrep) * HD);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // qmm.cu
 
-// arena as (64 dims of a half, slot, half, kv head); one box: 16 slots of one half
-static cudaError_t tree_map(CUtensorMap* map, const void* arena, int hkv, int64_t n_slots) {
+// arena as (64 dims of a half, slot, half, kv head); one box: 16 slots of one half, or of both
+static cudaError_t tree_map(CUtensorMap* map, const void* arena, int hkv, int64_t n_slots, int halves) {
     auto fn = encode_fn();
     if (!fn) return cudaErrorNotSupported;
     const cuuint64_t dims[4] = {64u, (cuuint64_t)n_slots, 2u, (cuuint64_t)hkv};
     const cuuint64_t strides[3] = {(cuuint64_t)hkv * HD * 2, 128u, (cuuint64_t)HD * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)KVB, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)KVB, (cuuint32_t)halves, 1};
     const cuuint32_t es[4] = {1, 1, 1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(arena), dims, strides, box, es,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -870,27 +1222,56 @@ static cudaError_t tree_map(CUtensorMap* map, const void* arena, int hkv, int64_
 }
 
 struct TreePlan {
-    int G, rows, q_rows, row_tiles;
+    bool few;                   // up to TF_ROWS rows per kv head: tree_few_kernel
+    int rows;                   // of a part
+    int splits, bps;            // few: splits of a sequence's blocks, blocks of one
+    int G, q_rows, row_tiles;   // wide
     size_t o_bytes, ml_bytes, cut_bytes, q_bytes, e_bytes;
 };
-static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens) {
-    TreePlan p;
-    p.G = num_sms();
+constexpr int TF_ROWS = 32;
+static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
+    TreePlan p = {};
     const int64_t rows = (int64_t)max_seq_tokens * (hq / hkv);
-    p.rows = (int)(rows < TW_ROWS ? rows : TW_ROWS);
-    p.q_rows = (p.rows + 7) / 8 * 8;
-    p.row_tiles = (int)((rows + TW_ROWS - 1) / TW_ROWS);
-    p.o_bytes = align256((size_t)2 * p.G * p.rows * HD * 4);
-    p.ml_bytes = align256((size_t)2 * p.G * p.rows * 2 * 4);
-    p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
-    const size_t q = (size_t)n_seqs * p.row_tiles * hkv * p.q_rows;
-    p.q_bytes = align256(q * 512);
-    p.e_bytes = align256(q);
+    p.few = rows <= TF_ROWS;
+    size_t parts;
+    if (p.few) {
+        attn_plan(n_seqs, hkv, max_ctx, &p.splits, &p.bps);   // as many CTAs as decode attention
+        if (p.splits > 32768) {                               // a grid's second dimension
+            p.bps = (p.bps * p.splits + 32767) / 32768;
+            p.splits = 32768;
+        }
+        p.rows = (int)rows;
+        parts = p.splits > 1 ? (size_t)n_seqs * hkv * p.splits : 0;
+    } else {
+        p.G = num_sms();
+        p.rows = (int)(rows < TW_ROWS ? rows : TW_ROWS);
+        p.q_rows = (p.rows + 7) / 8 * 8;
+        p.row_tiles = (int)((rows + TW_ROWS - 1) / TW_ROWS);
+        parts = (size_t)2 * p.G;
+        p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
+        const size_t q = (size_t)n_seqs * p.row_tiles * hkv * p.q_rows;
+        p.q_bytes = align256(q * 512);
+        p.e_bytes = align256(q);
+    }
+    p.o_bytes = align256(parts * p.rows * HD * 4);
+    p.ml_bytes = align256(parts * p.rows * 2 * 4);
     return p;
 }
 size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
-    const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens);
+    const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
     return p.o_bytes + p.ml_bytes + p.cut_bytes + p.q_bytes + p.e_bytes;
+}
+
+template <int MT>
+static cudaError_t launch_few(const CUtensorMap& km, const CUtensorMap& vm, const TreeArgs& a, const TreePlan& p, cudaStream_t st) {
+    const size_t smem = (size_t)TF_STAGES * TF_STAGE + MT * 8 * 2 * 32 * 16 + 2 * TF_STAGES * 8 + (2 * TF_CONS + 1) * 16 * MT * 4;
+    cudaError_t e = DCG_SMEM_ATTR(tree_few_kernel<MT>, smem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(tree_few_kernel<MT>, dim3((unsigned)(a.n_seqs * a.hkv), (unsigned)p.splits), dim3((TF_CONS + 1) * 32), smem,
+                   st, km, vm, a, p.bps, p.splits);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    return launch_pdl(tree_join_kernel, dim3((unsigned)(a.n_seqs * a.hkv), (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
+                      dim3(TC_ROWS * 32), 0, st, a, p.splits);
 }
 
 cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const void* varena, int64_t n_arena_blocks,
@@ -898,7 +1279,7 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
                                    const int* ctx, const int64_t* mask, int words, int n_tok, int n_seqs,
                                    int max_seq_tokens, int hq, int hkv, int max_ctx, float scale, float* out,
                                    void* scratch, cudaStream_t st) {
-    const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens);
+    const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
     TreeArgs a;
     a.q = q;
     a.n_arena_blocks = n_arena_blocks;
@@ -918,9 +1299,11 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     a.row_tiles = p.row_tiles;
     CUtensorMap km, vm;
     const int64_t n_slots = n_arena_blocks * n_layer * KVB;
-    cudaError_t e = tree_map(&km, karena, hkv, n_slots);
-    if (e == cudaSuccess) e = tree_map(&vm, varena, hkv, n_slots);
-    if (e == cudaSuccess) e = DCG_SMEM_ATTR(tree_wide_kernel, TW_SMEM);
+    cudaError_t e = tree_map(&km, karena, hkv, n_slots, p.few ? 2 : 1);
+    if (e == cudaSuccess) e = tree_map(&vm, varena, hkv, n_slots, p.few ? 2 : 1);
+    if (e != cudaSuccess) return e;
+    if (p.few) return p.rows <= 16 ? launch_few<1>(km, vm, a, p, st) : launch_few<2>(km, vm, a, p, st);
+    e = DCG_SMEM_ATTR(tree_wide_kernel, TW_SMEM);
     if (e != cudaSuccess) return e;
     e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;

@@ -86,6 +86,14 @@ def test_tree_head_layouts(ops, hq, hkv):
     check_tree(ops, [1, 2, 5, 17, 33], [1, 9, 40, 100, 211], hq, hkv)
 
 
+@pytest.mark.parametrize("hq,hkv,n", [(8, 8, 16), (8, 8, 17), (8, 8, 32), (8, 8, 33), (16, 8, 8), (16, 8, 9), (16, 8, 16),
+                                      (32, 8, 4), (32, 8, 5), (32, 8, 8), (64, 8, 2), (64, 8, 3), (64, 8, 4), (64, 8, 5),
+                                      (12, 4, 5), (12, 4, 6), (12, 4, 10), (7, 1, 2), (7, 1, 4), (33, 1, 1), (32, 1, 1)])
+def test_tree_few_rows(ops, hq, hkv, n):
+    """Around 16 and 32 (token, head) rows per kv head, where the kernels change."""
+    check_tree(ops, [n, 1, n], [n, 70, 333], hq, hkv, seed=n)
+
+
 @pytest.mark.parametrize("n", [1, 2, 3, 7, 8, 9, 15, 16, 17, 31, 32, 33, 48, 63, 64])
 def test_tree_sizes(ops, n):
     check_tree(ops, [n, 1, n], [n, n + 130, 300], 16, 4, seed=n)
