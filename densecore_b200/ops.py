@@ -230,32 +230,35 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_arena: torch.Tensor, v_arena: 
         "dcg_kv_append")
 
 
-def _check_all(dev: torch.device, *named):
-    """(tensor, name, dtype) triples: contiguous CUDA tensors of that type on device `dev`."""
+def _check_all(dev: int, *named):
+    """(tensor, name, dtype) triples: contiguous tensors of that type on CUDA device `dev` (its index).
+    These checks are most of a small call's time: one pass, no tensor touched twice."""
     for t, name, dtype in named:
-        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.device != dev:
+        if t.dtype is not dtype or t.get_device() != dev or dev < 0 or not t.is_contiguous():
             _check_cuda(t, name, dtype)
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
 
 
-def _call(dev: torch.device, fn: str, *args):
+def _call(dev: int, fn: str, *args):
     """Call a device entry point on `dev` and its current stream (whatever device is current)."""
-    if dev.index == torch.cuda.current_device():
-        rc = getattr(_lib.load(), fn)(*args, torch.cuda.current_stream().cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(dev)   # a Stream object costs more than a launch
+    if dev == torch._C._cuda_getDevice():
+        rc = getattr(_lib.load(), fn)(*args, stream)
     else:
         with torch.cuda.device(dev):
-            rc = getattr(_lib.load(), fn)(*args, torch.cuda.current_stream().cuda_stream)
+            rc = getattr(_lib.load(), fn)(*args, stream)
     if rc:
         _lib.check(rc, fn)
 
 
 def _arena_shape(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int):
     """(blocks, hkv, head_dim) of a pair of arenas [blocks * n_layer, 16, hkv, head_dim]."""
-    if k_arena.dim() != 4 or k_arena.shape[1] != 16 or n_layer < 1 or k_arena.shape[0] % n_layer:
-        raise ValueError(f"arenas must be [blocks * n_layer, 16, hkv, head_dim], got {tuple(k_arena.shape)}")
-    if v_arena.shape != k_arena.shape:
+    shape = k_arena.shape
+    if len(shape) != 4 or shape[1] != 16 or n_layer < 1 or shape[0] % n_layer:
+        raise ValueError(f"arenas must be [blocks * n_layer, 16, hkv, head_dim], got {tuple(shape)}")
+    if v_arena.shape != shape:
         raise ValueError("k_arena and v_arena differ in shape")
-    return k_arena.shape[0] // n_layer, k_arena.shape[2], k_arena.shape[3]
+    return shape[0] // n_layer, shape[2], shape[3]
 
 
 def tree_masks(parents) -> torch.Tensor:
@@ -288,20 +291,22 @@ def paged_attn_tree(q: torch.Tensor, k_arena: torch.Tensor, v_arena: torch.Tenso
     token t's K/V sit in slot ctx_lens[s] - n_s + t (already appended).  Row i sees the history and
     drafted token t of its sequence where bit t % 64 of tree_mask[i, t // 64] (int64) is set; a row
     that sees nothing is zeros (see dcg_paged_attn_tree)."""
-    dev = q.device
+    dev = q.get_device()
     _check_all(dev, (q, "q", torch.float32), (k_arena, "k_arena", torch.float16), (v_arena, "v_arena", torch.float16),
                (block_tables, "block_tables", torch.int32), (seq_starts, "seq_starts", torch.int32),
                (ctx_lens, "ctx_lens", torch.int32), (tree_mask, "tree_mask", torch.int64))
-    if q.dim() != 3 or block_tables.dim() != 2 or tree_mask.dim() != 2:
+    shape, tables, words = q.shape, block_tables.shape, tree_mask.shape
+    if len(shape) != 3 or len(tables) != 2 or len(words) != 2:
         raise ValueError("q must be [n_tok, hq, head_dim], block_tables and tree_mask two-dimensional")
-    n_tok, hq, hd = q.shape
-    n_seqs = ctx_lens.numel()
-    if seq_starts.numel() != n_seqs + 1 or block_tables.shape[0] != n_seqs:
-        raise ValueError("seq_starts needs one entry more than ctx_lens, block_tables as many rows")
-    if tree_mask.shape[0] != n_tok:
+    n_tok, hq, hd = shape
+    n_seqs, mbs = tables
+    if seq_starts.numel() != n_seqs + 1 or ctx_lens.numel() != n_seqs:
+        raise ValueError("seq_starts needs one entry more than block_tables has rows, ctx_lens as many")
+    if words[0] != n_tok:
         raise ValueError("tree_mask needs a row for each row of q")
     per_block = 16 * hkv * hd * n_layer
-    if per_block <= 0 or k_arena.numel() % per_block or v_arena.numel() != k_arena.numel():
+    elements = k_arena.numel()
+    if per_block <= 0 or elements % per_block or v_arena.numel() != elements:
         raise ValueError("arenas are not whole blocks of n_layer x 16 x hkv x head_dim")
     if scale is None:
         scale = 1.0 / float(hd) ** 0.5
@@ -309,15 +314,15 @@ def paged_attn_tree(q: torch.Tensor, k_arena: torch.Tensor, v_arena: torch.Tenso
         out = torch.empty_like(q)
     else:
         _check_all(dev, (out, "out", torch.float32))
-        if out.shape != q.shape:
+        if out.shape != shape:
             raise ValueError("out must have q's shape")
     if scratch is None:
-        scratch = torch.empty(max(1, paged_attn_tree_scratch_size(n_seqs, hq, hkv, max_seq_tokens, max_ctx, hd)), dtype=torch.uint8, device=dev)
+        scratch = torch.empty(max(1, paged_attn_tree_scratch_size(n_seqs, hq, hkv, max_seq_tokens, max_ctx, hd)), dtype=torch.uint8, device=f"cuda:{dev}")
     else:
         _check_all(dev, (scratch, "scratch", torch.uint8))
     _call(dev, "dcg_paged_attn_tree", q.data_ptr(), k_arena.data_ptr(), v_arena.data_ptr(),
-          k_arena.numel() // per_block, n_layer, layer, block_tables.data_ptr(), block_tables.shape[1],
-          seq_starts.data_ptr(), ctx_lens.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], n_tok, n_seqs,
+          elements // per_block, n_layer, layer, block_tables.data_ptr(), mbs,
+          seq_starts.data_ptr(), ctx_lens.data_ptr(), tree_mask.data_ptr(), words[1], n_tok, n_seqs,
           max_seq_tokens, hq, hkv, hd, max_ctx, scale, out.data_ptr(), scratch.data_ptr(), scratch.numel())
     return out
 
@@ -336,15 +341,16 @@ def kv_fork(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int, block_ta
     block_tables, ctx_lens, n_pages, ref_counts are int32 and updated in place; the arenas are
     [blocks * n_layer, 16, hkv, head_dim] fp16.  Returns status (int32): 0, or the number of blocks
     that were missing, or -1 for bad input; unless 0 nothing was changed (see dcg_kv_fork)."""
-    dev = k_arena.device
+    dev = k_arena.get_device()
     i32 = torch.int32
     _check_all(dev, (k_arena, "k_arena", torch.float16), (v_arena, "v_arena", torch.float16),
                (block_tables, "block_tables", i32), (ctx_lens, "ctx_lens", i32), (n_pages, "n_pages", i32),
                (ref_counts, "ref_counts", i32), (parents, "parents", i32))
     blocks, hkv, hd = _arena_shape(k_arena, v_arena, n_layer)
-    if block_tables.dim() != 2:
+    tables = block_tables.shape
+    if len(tables) != 2:
         raise ValueError("block_tables must be two-dimensional")
-    n, mbs = block_tables.shape
+    n, mbs = tables
     if ctx_lens.numel() != n or n_pages.numel() != n or parents.numel() != n:
         raise ValueError("ctx_lens, n_pages and parents need an entry for each row of block_tables")
     if ref_counts.numel() != blocks:
@@ -354,13 +360,13 @@ def kv_fork(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int, block_ta
         if reserve.numel() != n:
             raise ValueError("reserve needs an entry for each row of block_tables")
     if status is None:
-        status = torch.empty((), dtype=i32, device=dev)
+        status = torch.empty((), dtype=i32, device=f"cuda:{dev}")
     else:
         _check_all(dev, (status, "status", i32))
         if status.numel() < 1:
             raise ValueError("status must hold one int32")
     if scratch is None:
-        scratch = torch.empty(max(1, kv_fork_scratch_size(n, mbs, blocks)), dtype=torch.uint8, device=dev)
+        scratch = torch.empty(max(1, kv_fork_scratch_size(n, mbs, blocks)), dtype=torch.uint8, device=f"cuda:{dev}")
     else:
         _check_all(dev, (scratch, "scratch", torch.uint8))
     _call(dev, "dcg_kv_fork", k_arena.data_ptr(), v_arena.data_ptr(), blocks, n_layer, hkv, hd,
@@ -375,19 +381,20 @@ def kv_compact(k_arena: torch.Tensor, v_arena: torch.Tensor, n_layer: int, block
     """Move accepted drafted tokens together: slot base_lens[s] + path[s, j] of sequence s goes to
     slot base_lens[s] + j for j < path_lens[s], in every layer, and ctx_lens[s] becomes
     base_lens[s] + path_lens[s] (in place; int32; see dcg_kv_compact)."""
-    dev = k_arena.device
+    dev = k_arena.get_device()
     i32 = torch.int32
     _check_all(dev, (k_arena, "k_arena", torch.float16), (v_arena, "v_arena", torch.float16),
                (block_tables, "block_tables", i32), (base_lens, "base_lens", i32), (path, "path", i32),
                (path_lens, "path_lens", i32), (ctx_lens, "ctx_lens", i32))
     blocks, hkv, hd = _arena_shape(k_arena, v_arena, n_layer)
-    if block_tables.dim() != 2 or path.dim() != 2:
+    tables, paths = block_tables.shape, path.shape
+    if len(tables) != 2 or len(paths) != 2:
         raise ValueError("block_tables and path must be two-dimensional")
-    n = block_tables.shape[0]
-    if base_lens.numel() != n or path.shape[0] != n or path_lens.numel() != n or ctx_lens.numel() != n:
+    n = tables[0]
+    if base_lens.numel() != n or paths[0] != n or path_lens.numel() != n or ctx_lens.numel() != n:
         raise ValueError("base_lens, path, path_lens and ctx_lens need an entry for each row of block_tables")
     _call(dev, "dcg_kv_compact", k_arena.data_ptr(), v_arena.data_ptr(), blocks, n_layer, hkv, hd,
-          block_tables.data_ptr(), block_tables.shape[1], base_lens.data_ptr(), path.data_ptr(), path.shape[1],
+          block_tables.data_ptr(), tables[1], base_lens.data_ptr(), path.data_ptr(), paths[1],
           path_lens.data_ptr(), n, ctx_lens.data_ptr())
 
 
@@ -404,8 +411,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, k: int
     candidates score scores[row] + log_softmax(logits[row])[token].  Returns (scores [n_groups, k]
     f32, rows int32, tokens int32), best first; rows index `logits` (the parents for kv_fork).
     finished (uint8): a finished row offers itself alone, as token eos (see dcg_beam_select)."""
-    dev = logits.device
-    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+    dev = logits.get_device()
+    if dev < 0 or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("logits must be a two-dimensional CUDA tensor of float32 with contiguous rows")
     rows, vocab = logits.shape
     if n_beams < 1 or rows % n_beams:
@@ -419,16 +426,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_beams: int, k: int
         if finished.numel() != rows:
             raise ValueError("finished needs an entry for each row of logits")
     if out is None:
-        out = (torch.empty((groups, k), dtype=torch.float32, device=dev),
-               torch.empty((groups, k), dtype=torch.int32, device=dev),
-               torch.empty((groups, k), dtype=torch.int32, device=dev))
+        out = (torch.empty((groups, k), dtype=torch.float32, device=f"cuda:{dev}"),
+               torch.empty((groups, k), dtype=torch.int32, device=f"cuda:{dev}"),
+               torch.empty((groups, k), dtype=torch.int32, device=f"cuda:{dev}"))
     else:
         _check_all(dev, (out[0], "out scores", torch.float32), (out[1], "out rows", torch.int32),
                    (out[2], "out tokens", torch.int32))
         if any(t.numel() != groups * k for t in out):
             raise ValueError("out tensors must hold n_groups * k values")
     if scratch is None:
-        scratch = torch.empty(max(1, beam_select_scratch_size(groups, n_beams, vocab, k)), dtype=torch.uint8, device=dev)
+        scratch = torch.empty(max(1, beam_select_scratch_size(groups, n_beams, vocab, k)), dtype=torch.uint8, device=f"cuda:{dev}")
     else:
         _check_all(dev, (scratch, "scratch", torch.uint8))
     _call(dev, "dcg_beam_select", logits.data_ptr(), logits.stride(0) if rows > 1 else max(vocab, logits.stride(0)),
