@@ -9,6 +9,10 @@ matmul at M = prompt tokens, multi-token causal attention), batched over the req
 the same step; its last token's logits give the first generated token.  With prefill=False prompts
 are instead fed one token per step through the decode graph.  Sampling is greedy.  Idle slots
 point at one reserved block and run a harmless one-token step.
+
+Sequences that branch: BeamSearcher (beam search over groups of decoder rows) and TreeSpeculator
+(greedy decoding that scores drafted token trees) keep the blocks on the device, shared between rows
+and counted (PagePool).  Each takes the whole decoder's cache while it runs.
 """
 from __future__ import annotations
 
@@ -17,6 +21,7 @@ import dataclasses
 
 import torch
 
+from . import ops
 from .decoder import KV_BLOCK, Decoder
 
 
@@ -154,3 +159,228 @@ class ContinuousBatcher:
         while n < max_steps and self.step():
             n += 1
         return self.finished
+
+
+class PagePool:
+    """The decoder's KV blocks as pages shared between rows, kept on the device: the block table, how
+    many tokens and blocks each row holds, and how often each block is held.  fork and compact are
+    kv_fork and kv_compact on all rows at once; block 0 is the idle block that unused entries point
+    at.  Nothing waits for the host except `check`."""
+
+    def __init__(self, dec: Decoder):
+        self.dec = dec
+        dev, i32 = dec.device, torch.int32
+        self.tables = dec.block_tables
+        self.lens = torch.zeros(dec.batch, dtype=i32, device=dev)       # tokens in the cache
+        self.pages = torch.zeros(dec.batch, dtype=i32, device=dev)
+        self.refs = torch.zeros(dec.n_blocks, dtype=i32, device=dev)
+        self.refs[0] = 1
+        self.tables.zero_()
+        self.identity = torch.arange(dec.batch, dtype=i32, device=dev)
+        self.short = torch.zeros((), dtype=i32, device=dev)             # worst status so far (0: all went well)
+        self._status = torch.zeros((), dtype=i32, device=dev)
+        self._scratch = torch.empty(ops.kv_fork_scratch_size(dec.batch, self.tables.shape[1], dec.n_blocks),
+                                    dtype=torch.uint8, device=dev)
+
+    def fork(self, parents: torch.Tensor | None = None, reserve: torch.Tensor | None = None):
+        """Rows become children of `parents` (default: themselves) with room for `reserve` more tokens."""
+        d = self.dec
+        ops.kv_fork(d.k_arena, d.v_arena, d.cfg.n_layer, self.tables, self.lens, self.pages, self.refs,
+                    self.identity if parents is None else parents, reserve=reserve, fill_page=0,
+                    status=self._status, scratch=self._scratch)
+        self.short = torch.maximum(self.short, self._status.abs())
+
+    def compact(self, base: torch.Tensor, path: torch.Tensor, path_lens: torch.Tensor):
+        """Keep the accepted branches: base tokens before the draft, path in drafted tokens."""
+        d = self.dec
+        ops.kv_compact(d.k_arena, d.v_arena, d.cfg.n_layer, self.tables, base, path, path_lens, self.lens)
+
+    def check(self):
+        """Raise if a fork so far found too few blocks (it then changed nothing)."""
+        n = int(self.short)
+        if n:
+            raise MemoryError(f"the KV arena is {n} blocks short")
+
+
+class BeamSearcher:
+    """Beam search over the captured decode step: the decoder's rows are groups of n_beams beams, and
+    every step selects on the device (beam_select) and forks the cache rows after the selected parents
+    (kv_fork: shared blocks, one partial block copied per extra child)."""
+
+    def __init__(self, dec: Decoder, n_beams: int, eos: int | None = None):
+        if n_beams < 1 or dec.batch % n_beams:
+            raise ValueError(f"{dec.batch} decoder rows are not whole groups of {n_beams} beams")
+        self.dec, self.n_beams, self.eos = dec, n_beams, eos
+
+    def search(self, prompts, max_new: int):
+        """The n_beams best continuations of each prompt, best first: lists of (score, tokens), score the
+        sum of the tokens' log-probabilities; a continuation ends at eos (included) or max_new tokens.
+        Fewer, if the logits allow fewer."""
+        dec, nb = self.dec, self.n_beams
+        G, B, dev, i32 = len(prompts), dec.batch, dec.device, torch.int32
+        if not 0 < G <= B // nb:
+            raise ValueError(f"1 to {B // nb} prompts fit")
+        if max_new < 1 or any(not p or len(p) + max_new > dec.max_ctx for p in prompts):
+            raise ValueError(f"need non-empty prompts, max_new >= 1 and at most {dec.max_ctx} positions")
+        pool = PagePool(dec)
+        first = torch.arange(G, dtype=i32, device=dev) * nb
+        room = torch.zeros(B, dtype=i32, device=dev)
+        room[first.long()] = torch.tensor([len(p) for p in prompts], dtype=i32, device=dev)
+        pool.fork(reserve=room)
+        pool.check()
+        _, logits = dec.prefill([g * nb for g in range(G)], prompts)
+        pool.lens.copy_(room)
+        one = torch.ones(B, dtype=i32, device=dev)
+        scores = torch.full((B,), -float("inf"), device=dev)
+        parents = torch.full((B,), -1, dtype=i32, device=dev)
+        tokens = torch.full((B,), -1, dtype=i32, device=dev)
+        s, r, t = ops.beam_select(logits, torch.zeros(G, device=dev), 1, nb)
+        scores[:G * nb], tokens[:G * nb] = s.flatten(), t.flatten()
+        parents[:G * nb] = torch.where(r >= 0, r * nb, r).flatten()
+        finished = torch.zeros(B, dtype=torch.uint8, device=dev)
+        eos = -1 if self.eos is None else self.eos
+        steps = [(parents.clone(), tokens.clone())]
+        out = tuple(torch.empty((B // nb, nb), dtype=d, device=dev) for d in (torch.float32, i32, i32))
+        ws = torch.empty(ops.beam_select_scratch_size(B // nb, nb, dec.cfg.vocab, nb), dtype=torch.uint8, device=dev)
+        for _ in range(max_new - 1):
+            finished.copy_((tokens == eos) & (parents >= 0) if self.eos is not None else finished)
+            if bool(((finished != 0) | (parents < 0)).all()):
+                break
+            pool.fork(parents, reserve=one)
+            dec.tokens.copy_(tokens.clamp(min=0))
+            dec.ctx_lens.copy_(pool.lens + 1)
+            dec.replay()
+            pool.lens.add_((parents >= 0).int())
+            ops.beam_select(dec.logits, scores, nb, nb, finished=finished, eos=eos, out=out, scratch=ws)
+            scores.copy_(out[0].flatten())
+            parents.copy_(out[1].flatten())
+            tokens.copy_(out[2].flatten())
+            steps.append((parents.clone(), tokens.clone()))
+        pool.check()
+        return beam_paths(scores.tolist(), [(p.tolist(), t.tolist()) for p, t in steps], nb, G, self.eos)
+
+
+def beam_paths(scores, steps, n_beams: int, groups: int, eos: int | None):
+    """(score, tokens) of every live beam, read back through the steps' (parents, tokens)."""
+    found = []
+    for g in range(groups):
+        mine = []
+        for row in range(g * n_beams, (g + 1) * n_beams):
+            if scores[row] == -float("inf"):
+                continue
+            out, at = [], row
+            for parents, tokens in reversed(steps):
+                out.append(tokens[at])
+                at = parents[at]
+            out.reverse()
+            if eos is not None and eos in out:
+                out = out[:out.index(eos) + 1]
+            mine.append((scores[row], out))
+        found.append(mine)
+    return found
+
+
+def ngram_draft(history, n: int = 2, depth: int = 4, width: int = 4):
+    """Guess what follows `history` from what followed its last n tokens before: a tree of up to `width`
+    different continuations of up to `depth` tokens, latest first.  (tokens, parents), parents as
+    Decoder.verify_tree's; -1 = after the last token of the history."""
+    tokens, parents, kids = [], [], {}
+    key = history[-n:]
+    found = 0
+    for at in range(len(history) - n - 1, -1, -1):
+        if found == width:
+            break
+        if history[at:at + n] != key:
+            continue
+        cur, grew = -1, False
+        for t in history[at + n:at + n + depth]:
+            nxt = kids.get((cur, t))
+            if nxt is None:
+                nxt = kids[(cur, t)] = len(tokens)
+                tokens.append(t)
+                parents.append(cur)
+                grew = True
+            cur = nxt
+        found += grew
+    return tokens, parents
+
+
+def accept_path(tokens, parents, greedy):
+    """The drafted tokens that greedy decoding would have chosen: token 0 is the last known one, then
+    from token to child while a child is what the model says.  Drafted indexes, ascending."""
+    path = [0]
+    while True:
+        nxt = [j for j in range(path[-1] + 1, len(tokens)) if parents[j] == path[-1] and tokens[j] == greedy[path[-1]]]
+        if not nxt:
+            return path
+        path.append(nxt[0])
+
+
+class TreeSpeculator:
+    """Greedy decoding with drafted token trees: `draft(history)` guesses continuations, one pass scores
+    the whole tree (Decoder.verify_tree), and the longest branch that greedy decoding would have taken
+    is kept (kv_compact).  The tokens are those of greedy decoding."""
+
+    def __init__(self, dec: Decoder, draft=ngram_draft, max_nodes: int = 64):
+        if not 1 <= max_nodes <= 1024:
+            raise ValueError("max_nodes must be in 1 .. 1024")
+        self.dec, self.draft, self.max_nodes = dec, draft, max_nodes
+        self.passes = self.accepted = 0
+
+    def generate(self, prompts, max_new: int, eos: int | None = None):
+        """The greedy continuation of each prompt (at most max_new tokens, up to eos included)."""
+        dec = self.dec
+        B, dev, i32 = dec.batch, dec.device, torch.int32
+        n = len(prompts)
+        if not 0 < n <= B:
+            raise ValueError(f"1 to {B} prompts fit")
+        if max_new < 1 or any(not p or len(p) + max_new > dec.max_ctx for p in prompts):
+            raise ValueError(f"need non-empty prompts, max_new >= 1 and at most {dec.max_ctx} positions")
+        pool = PagePool(dec)
+
+        def per_row(values):
+            return torch.tensor(list(values) + [0] * (B - n), dtype=i32).to(dev)
+
+        pool.fork(reserve=per_row(len(p) for p in prompts))
+        pool.check()
+        nxt, _ = dec.prefill(list(range(n)), prompts)
+        pool.lens.copy_(per_row(len(p) for p in prompts))
+        cached = [len(p) for p in prompts]
+        out = [[int(t)] for t in nxt.tolist()]
+
+        def done(i):
+            return len(out[i]) >= max_new or (eos is not None and out[i][-1] == eos)
+
+        while True:
+            live = [i for i in range(n) if not done(i)]
+            if not live:
+                return out
+            trees = {}
+            for i in live:
+                t, p = self.draft(list(prompts[i]) + out[i])
+                # token 0 is the one just chosen; every drafted token takes a slot of the cache
+                room = min(self.max_nodes, dec.max_ctx - cached[i]) - 1
+                trees[i] = ([out[i][-1]] + list(t)[:room], [-1] + [q + 1 for q in list(p)[:room]])
+            pool.fork(reserve=per_row(len(trees[i][0]) if i in trees else 0 for i in range(n)))
+            pool.check()
+            greedy, _ = dec.verify_tree(live, [trees[i] for i in live], [cached[i] for i in live])
+            greedy = greedy.tolist()
+            paths, at = [[] for _ in range(n)], 0
+            base = list(cached)
+            for i in live:
+                t, p = trees[i]
+                g = greedy[at:at + len(t)]
+                at += len(t)
+                path = accept_path(t, p, g)
+                new = [t[j] for j in path[1:]] + [g[path[-1]]]
+                if eos is not None and eos in new:
+                    new = new[:new.index(eos) + 1]
+                new = new[:max_new - len(out[i])]
+                paths[i] = path
+                out[i] += new
+                cached[i] += len(path)
+                self.accepted += len(new)
+            width = max(len(p) for p in paths)
+            table = torch.tensor([p + [0] * (width - len(p)) for p in paths] + [[0] * width] * (B - n), dtype=i32).to(dev)
+            pool.compact(per_row(base), table, per_row(len(p) for p in paths))
+            self.passes += 1

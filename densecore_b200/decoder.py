@@ -466,7 +466,30 @@ class Decoder:
         finally:
             lib.dcg_set_programmatic_launch(prev)
 
-    def _prefill(self, seqs, prompts, start):
+    def verify_tree(self, seqs, trees, start):
+        """Score a drafted token tree for each of the sequences `seqs` in one pass (speculative
+        decoding).  trees[i] = (tokens, parents): parents[j] < j is the token before token j in its
+        branch, -1 the last token in the cache; start[i] tokens of sequence seqs[i] are in the cache.
+        Token j's K/V go to slot start[i] + j (blocks up to there must be in the table) at the position
+        of its depth.  Returns (next_tokens, logits) for every drafted token, the sequences' tokens one
+        after the other.  kv_compact then keeps the accepted branch."""
+        tokens = [list(t) for t, _ in trees]
+        parents = [list(p) for _, p in trees]
+        if any(len(t) != len(p) for t, p in zip(tokens, parents)):
+            raise ValueError("every drafted token needs a parent")
+        if len(trees) != len(seqs) or len(start) != len(seqs):
+            raise ValueError("seqs, trees and start differ in length")
+        if self.tp_size == 1:
+            return self._prefill(seqs, tokens, start, parents)
+        lib = ops._lib.load()
+        prev = lib.dcg_set_programmatic_launch(0)
+        try:
+            return self._prefill(seqs, tokens, start, parents)
+        finally:
+            lib.dcg_set_programmatic_launch(prev)
+
+    def _prefill(self, seqs, prompts, start, parents=None):
+        """The pass of prefill, or with parents that of verify_tree (a tree for each sequence)."""
         cfg, dev = self.cfg, self.device
         D, hq, hkv, H, ffn = cfg.head_dim, self.hq, self.hkv, cfg.hidden, self.ffn
         qd, kvd = hq * D, hkv * D
@@ -479,8 +502,19 @@ class Decoder:
         i32 = torch.int32
         tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=dev)
         local_seq = torch.tensor([i for i, n in enumerate(n_s) for _ in range(n)], dtype=i32, device=dev)
-        positions = torch.tensor([start[i] + j for i, n in enumerate(n_s) for j in range(n)], dtype=i32,
-                                 device=dev)
+        slots = torch.tensor([start[i] + j for i, n in enumerate(n_s) for j in range(n)], dtype=i32, device=dev)
+        positions = slots
+        if parents is not None:
+            masks = [ops.tree_masks(p) for p in parents]
+            words = max(m.shape[1] for m in masks)
+            mask = torch.cat([torch.nn.functional.pad(m, (0, words - m.shape[1])) for m in masks]).to(dev)
+            depth = []
+            for i, p in enumerate(parents):
+                d = []
+                for q in p:
+                    d.append(d[q] + 1 if q >= 0 else 0)
+                depth += [start[i] + x for x in d]
+            positions = torch.tensor(depth, dtype=i32, device=dev)
         seq_starts = torch.tensor([0] + list(np.cumsum(n_s)), dtype=i32, device=dev)
         ctx = torch.tensor([start[i] + n_s[i] for i in range(S)], dtype=i32, device=dev)
         if int(ctx.max()) > self.max_ctx:
@@ -490,6 +524,9 @@ class Decoder:
         x = self.tok_embd[tokens].float()
         q_rot = torch.empty((T, hq, D), device=dev)
         attn_out = torch.empty((T, hq, D), device=dev)
+
+        attn_scr = None if parents is None else torch.empty(
+            max(1, ops.paged_attn_tree_scratch_size(S, hq, hkv, max(n_s), self.max_ctx)), dtype=torch.uint8, device=dev)
 
         def actbuf(k, wtype):
             at = VEC_DOT_TYPE[wtype]
@@ -515,12 +552,20 @@ class Decoder:
                 yv, ldv = mm(wv, act_v, T), kvd
             else:
                 yv, ldv = yqk[:, qd + kvd:], wqk.n
-            ops.qk_norm_rope_kv_append_tokens(yqk, wqk.n, yqk[:, qd:], wqk.n, yv, ldv, T, hq, hkv,
-                                              L["attn_q_norm"], L["attn_k_norm"], cfg.rms_eps, cfg.rope_theta,
-                                              local_seq, positions, q_rot, self.k_arena, self.v_arena,
-                                              cfg.n_layer, li, bt)
-            ops.paged_attn_prefill(q_rot, self.k_arena, self.v_arena, cfg.n_layer, li, bt, seq_starts, ctx, hkv,
-                                   max(n_s), self.max_ctx, scale, out=attn_out)
+            if parents is None:
+                ops.qk_norm_rope_kv_append_tokens(yqk, wqk.n, yqk[:, qd:], wqk.n, yv, ldv, T, hq, hkv,
+                                                  L["attn_q_norm"], L["attn_k_norm"], cfg.rms_eps, cfg.rope_theta,
+                                                  local_seq, positions, q_rot, self.k_arena, self.v_arena,
+                                                  cfg.n_layer, li, bt)
+                ops.paged_attn_prefill(q_rot, self.k_arena, self.v_arena, cfg.n_layer, li, bt, seq_starts, ctx, hkv,
+                                       max(n_s), self.max_ctx, scale, out=attn_out)
+            else:
+                ops.qk_norm_rope_kv_append_tree(yqk, wqk.n, yqk[:, qd:], wqk.n, yv, ldv, T, hq, hkv,
+                                                L["attn_q_norm"], L["attn_k_norm"], cfg.rms_eps, cfg.rope_theta,
+                                                local_seq, positions, slots, q_rot, self.k_arena, self.v_arena,
+                                                cfg.n_layer, li, bt)
+                ops.paged_attn_tree(q_rot, self.k_arena, self.v_arena, cfg.n_layer, li, bt, seq_starts, ctx, mask,
+                                    hkv, max(n_s), self.max_ctx, scale, out=attn_out, scratch=attn_scr)
             wo = L["attn_output"]
             act_o = actbuf(qd, wo.qtype)
             ops.quantize_act(attn_out.view(T, qd), VEC_DOT_TYPE[wo.qtype], out=act_o)
@@ -534,18 +579,19 @@ class Decoder:
             ops.swiglu_quantize(ygu, ygu[:, ffn:], 2 * ffn, T, ffn, VEC_DOT_TYPE[wd.qtype], act_d)
             delta = self._allreduce(mm(wd, act_d, T))
         x += delta
-        last = x[(seq_starts[1:] - 1).long()].contiguous()
+        last = x[(seq_starts[1:] - 1).long()].contiguous() if parents is None else x
+        R = last.shape[0]
         at = VEC_DOT_TYPE[self.output.qtype]
-        act_h = torch.empty(int(ops._lib.load().dcg_act_size(at, S, H)), dtype=torch.uint8, device=dev)
+        act_h = torch.empty(int(ops._lib.load().dcg_act_size(at, R, H)), dtype=torch.uint8, device=dev)
         ops.add_rmsnorm_quantize(last, self.output_norm, cfg.rms_eps, at, act_h)
-        logits_r = mm(self.output, act_h, S)
+        logits_r = mm(self.output, act_h, R)
         if self.tp_size == 1:
             logits = logits_r
         else:
             import torch.distributed as dist
-            gathered = torch.empty((self.tp_size, S, self.vocab_r), device=dev)
+            gathered = torch.empty((self.tp_size, R, self.vocab_r), device=dev)
             dist.all_gather_into_tensor(gathered, logits_r.contiguous(), group=self.tp_group)
-            logits = gathered.permute(1, 0, 2).reshape(S, -1)
+            logits = gathered.permute(1, 0, 2).reshape(R, -1)
         return torch.argmax(logits, dim=-1), logits
 
     def _allreduce(self, y):

@@ -118,3 +118,59 @@ def test_tree_masks():
     for bad in ([0], [-1, 1], [-2], [-1, 2, 0]):
         with pytest.raises(ValueError):
             ops.tree_masks(bad)
+
+
+# ------------------------------------------------------------------------- host logic of the loops
+def test_accept_path():
+    from densecore_b200.batching import accept_path
+    #        0   1   2   3   4   5
+    tok = [10, 11, 12, 13, 14, 13]
+    par = [-1, 0, 0, 2, 3, 1]
+    assert accept_path(tok, par, [12, 0, 13, 14, 9, 9]) == [0, 2, 3, 4]
+    assert accept_path(tok, par, [11, 13, 0, 0, 0, 0]) == [0, 1, 5]
+    assert accept_path(tok, par, [99, 0, 0, 0, 0, 0]) == [0]
+    assert accept_path([7], [-1], [3]) == [0]
+    # the same guess twice: the first one
+    assert accept_path([1, 2, 2], [-1, 0, 0], [2, 5, 5]) == [0, 1]
+
+
+def test_ngram_draft():
+    from densecore_b200.batching import ngram_draft
+    t, p = ngram_draft([1, 2, 3, 4, 1, 2, 3, 5, 1, 2], n=2, depth=3, width=4)
+    # after the latest "1 2": 3 5 1; before that 3 4 1 (the 3 is shared)
+    assert t == [3, 5, 1, 4, 1] and p == [-1, 0, 1, 0, 3]
+    assert ngram_draft([1, 2, 3], n=2) == ([], [])
+    assert ngram_draft([1], n=2) == ([], []) and ngram_draft([], n=2) == ([], [])
+    t, p = ngram_draft([5] * 10, n=2, depth=4, width=2)
+    assert all(q < i for i, q in enumerate(p)) and set(t) == {5}
+    assert ops.tree_masks(p).shape[0] == len(t)
+
+
+def test_beam_paths():
+    from densecore_b200.batching import beam_paths
+    inf = float("inf")
+    # one group of three beams, three steps; the last beam is dead
+    steps = [([0, 0, 0], [5, 6, 7]), ([1, 0, -1], [8, 9, -1]), ([0, 0, -1], [2, 3, -1])]
+    assert beam_paths([-1.0, -2.0, -inf], steps, 3, 1, None) == [[(-1.0, [6, 8, 2]), (-2.0, [6, 8, 3])]]
+    assert beam_paths([-1.0, -2.0, -inf], steps, 3, 1, 8) == [[(-1.0, [6, 8]), (-2.0, [6, 8])]]
+
+
+def test_loops_refuse():
+    from densecore_b200.batching import BeamSearcher, TreeSpeculator
+
+    class Dec:
+        batch, max_ctx, device = 6, 32, "cpu"
+    with pytest.raises(ValueError):
+        BeamSearcher(Dec(), 4)
+    with pytest.raises(ValueError):
+        BeamSearcher(Dec(), 0)
+    for prompts, new in (([], 3), ([[1]] * 3, 3), ([[]], 3), ([[1] * 30], 3), ([[1]], 0)):
+        with pytest.raises(ValueError):
+            BeamSearcher(Dec(), 3).search(prompts, new)
+    for prompts, new in (([], 3), ([[1]] * 7, 3), ([[]], 3), ([[1] * 30], 3), ([[1]], 0)):
+        with pytest.raises(ValueError):
+            TreeSpeculator(Dec()).generate(prompts, new)
+    with pytest.raises(ValueError):
+        TreeSpeculator(Dec(), max_nodes=0)
+    with pytest.raises(ValueError):
+        TreeSpeculator(Dec(), max_nodes=2000)
