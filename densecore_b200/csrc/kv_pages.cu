@@ -30,9 +30,10 @@ cudaError_t pages_device_error(int* out, bool clear) {
 //   copy it to, and every row asks for the pages that len_p + reserve tokens need; request r gets
 //   the r-th lowest page without a reference.
 // A page that is copied from keeps a reference and a page that is copied to had none, so no copy
-// reads what another writes.  Three launches, in stream order:
+// reads what another writes.  Three launches (two for small tables), in stream order:
 //   deltas  one CTA per old row p: ref[b] += kids(p) - 1 for its pages (0 for the usual single
-//           child: no traffic), kids counted from `parents`;
+//           child: no traffic), kids counted from `parents`; tables of up to FORK_SMALL entries leave
+//           this to the plan's CTA, a launch less;
 //   plan    one CTA: requests, their prefix sum, the scan for free pages, the rows' new lengths;
 //   apply   column strips of the table permuted through shared memory (every row's old entry is read
 //           before a new one is written), and the partial pages' slots copied.
@@ -41,7 +42,9 @@ cudaError_t pages_device_error(int* out, bool clear) {
 // ------------------------------------------------------------------------------------------
 constexpr int FORK_MAX_ROWS = 4096;
 constexpr int FORK_THREADS = 256;
+constexpr int FORK_BATCH = 8;            // 16-byte loads in flight per thread of a copy
 constexpr int PLAN_THREADS = 1024;
+constexpr int FORK_SMALL = 65536;       // table entries (64 x 1024: a few microseconds for one CTA)
 constexpr int PLAN_PER = 16;             // reference counts per thread and scan step
 constexpr int STRIP_INTS = 8192;         // 32 KB of table entries per strip
 
@@ -68,30 +71,31 @@ struct OldRow {
     bool bad;
 };
 
-// kids and sizes of old row p, the same in every thread of the CTA
+// sizes of an old row with `kids` children (par: its own parent); a row that is bad moves nothing
+__device__ __forceinline__ OldRow sized_row(const ForkArgs& a, int par, int64_t len, int held, int kids) {
+    const int64_t used = (len + KVB - 1) / KVB;
+    OldRow r;
+    r.kids = kids;
+    r.bad = held < 0 || held > a.mbs || par < -1 || par >= a.n || (kids && (len < 0 || used > held));
+    r.held = r.bad ? 0 : held;
+    r.used = r.bad ? 0 : (int)(used < 0 ? 0 : (used > held ? held : used));
+    return r;
+}
+// the same with the children counted, by a CTA of FORK_THREADS
 __device__ OldRow old_row(const ForkArgs& a, int p) {
     int kids = 0;
     for (int i0 = 0; i0 < a.n; i0 += FORK_THREADS) {
         const int i = i0 + threadIdx.x;
         kids += __syncthreads_count(i < a.n && a.parents[i] == p);
     }
-    OldRow r;
-    r.kids = kids;
-    r.held = a.held[p];
-    const int64_t len = a.lens[p];
-    const int64_t used = (len + KVB - 1) / KVB;
-    const int par = a.parents[p];
-    r.bad = r.held < 0 || r.held > a.mbs || par < -1 || par >= a.n || (kids && (len < 0 || used > r.held));
-    r.used = r.bad ? 0 : (int)(used < 0 ? 0 : (used > r.held ? r.held : used));
-    if (r.bad) r.held = 0;
-    return r;
+    return sized_row(a, a.parents[p], a.lens[p], a.held[p], kids);
 }
 
-// ref[b] += sign * (kids - 1) for the pages that go to the children, -sign for the others; returns
-// whether a page id was out of range
-__device__ bool add_deltas(const ForkArgs& a, int p, const OldRow& r, int sign) {
+// ref[b] += sign * (kids - 1) for the pages that go to the children, -sign for the others, by threads
+// first, first + step, ...; returns whether a page id was out of range
+__device__ __forceinline__ bool add_deltas(const ForkArgs& a, int p, const OldRow& r, int sign, int first, int step) {
     bool bad = false;
-    for (int j = threadIdx.x; j < r.held; j += FORK_THREADS) {
+    for (int j = first; j < r.held; j += step) {
         const int b = a.bt[(int64_t)p * a.mbs + j];
         const bool ok = b >= 0 && b < a.n_pages_arena;
         bad |= !ok;
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_deltas_kernel(const ForkArg
     pdl_trigger();
     const int p = blockIdx.x;
     const OldRow r = old_row(a, p);
-    const bool bad = add_deltas(a, p, r, 1);
+    const bool bad = add_deltas(a, p, r, 1, threadIdx.x, FORK_THREADS);
     const int any = __syncthreads_or(bad || r.bad);
     if (threadIdx.x == 0) a.bad[p] = any;
 }
@@ -137,22 +141,46 @@ __device__ int block_scan(int v, int* warp_sums, int* sum) {
     return x - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
+// SMALL: the deltas of all rows as well, a warp per row (n <= PLAN_THREADS: a thread per row elsewhere)
+template <bool SMALL>
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs a) {
     __shared__ int s_src[FORK_MAX_ROWS];     // partly filled last page of each new row, or -1
+    __shared__ int s_par[SMALL ? PLAN_THREADS : 1], s_len[SMALL ? PLAN_THREADS : 1], s_kids[SMALL ? PLAN_THREADS : 1];
     __shared__ int warp_sums[32];
+    __shared__ int s_copies;
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x;
+    if (t == 0) s_copies = 0;
     bool bad = false;
-    for (int i = t; i < a.n; i += PLAN_THREADS) bad |= a.bad[i] != 0;
+    if (SMALL) {
+        int p = -1;
+        s_kids[t] = 0;
+        if (t < a.n) {
+            s_par[t] = p = a.parents[t];
+            s_len[t] = a.lens[t];
+            bad = p < -1 || p >= a.n;
+        }
+        __syncthreads();
+        if (p >= 0 && !bad) atomicAdd(&s_kids[p], 1);
+        __syncthreads();
+        for (int r = t >> 5; r < a.n; r += PLAN_THREADS / 32) {
+            const OldRow row = sized_row(a, s_par[r], s_len[r], a.held[r], s_kids[r]);
+            bad |= row.bad;
+            bad |= add_deltas(a, r, row, 1, t & 31, 32);
+        }
+    } else {
+        for (int i = t; i < a.n; i += PLAN_THREADS) bad |= a.bad[i] != 0;
+    }
     bad = __syncthreads_or(bad);
     if (bad) {
         if (t == 0) { a.head[0] = -1; *a.status = -1; }
         return;
     }
+    // the new rows
     for (int i = t; i < a.n; i += PLAN_THREADS) {
-        const int p = a.parents[i];
-        const int len = p >= 0 ? a.lens[p] : 0;
+        const int p = SMALL ? s_par[i] : a.parents[i];
+        const int len = p < 0 ? 0 : SMALL ? s_len[p] : a.lens[p];
         const int64_t need = p >= 0 ? (int64_t)len + (a.reserve ? a.reserve[i] : 0) : 0;
         const int used = (len + KVB - 1) / KVB;
         const int64_t total = (need + KVB - 1) / KVB;
@@ -168,38 +196,47 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs 
         if (t == 0) { a.head[0] = -1; *a.status = -1; }
         return;
     }
-    // requests, in row order
-    int asked = 0, n_copies = 0, columns = 0;
+    // requests, in row order (the copies' list in any order)
+    int asked = 0, columns = 0;
     for (int i0 = 0; i0 < a.n; i0 += PLAN_THREADS) {
         const int i = i0 + t;
         int copy = 0, want = 0;
         if (i < a.n) {
             const int b = s_src[i];
             if (b >= 0) {
+                const int held = __ldcg(&a.refs[b]);   // counts changed by this CTA's atomics: from L2
                 int rank = 0;
                 for (int j = 0; j < i; j++) rank += s_src[j] == b;
-                copy = a.refs[b] - rank > 1;
+                copy = held - rank > 1;
             }
-            want = copy + a.new_held[i] - a.used[i];
+            const int now = a.new_held[i];
+            want = copy + now - a.used[i];
             a.src[i] = copy ? b : -1;
-            columns = max(columns, max(a.new_held[i], a.old_held[i]));
+            if (copy) a.copies[atomicAdd(&s_copies, 1)] = i;
+            columns = max(columns, max(now, a.old_held[i]));
         }
-        int sum, copies;
+        int sum;
         const int at = block_scan(want, warp_sums, &sum);
-        const int nth = block_scan(copy, warp_sums, &copies);
         if (i < a.n) a.first[i] = asked + at;
-        if (copy) a.copies[n_copies + nth] = i;
         asked += sum;
-        n_copies += copies;
     }
     // the lowest pages without a reference
+    const bool aligned = ((uintptr_t)a.refs & 15) == 0;
     int found = 0;
     for (int64_t b0 = 0; b0 < a.n_pages_arena && found < asked; b0 += PLAN_THREADS * PLAN_PER) {
         const int64_t b = b0 + (int64_t)t * PLAN_PER;
         uint32_t free_bits = 0;
+        if (b + PLAN_PER <= a.n_pages_arena && aligned) {
 #pragma unroll
-        for (int u = 0; u < PLAN_PER; u++)
-            if (b + u < a.n_pages_arena && a.refs[b + u] == 0) free_bits |= 1u << u;
+            for (int u = 0; u < PLAN_PER; u += 4) {
+                const int4 c = __ldcg((const int4*)(a.refs + b + u));
+                free_bits |= ((c.x == 0) | (c.y == 0) << 1 | (c.z == 0) << 2 | (c.w == 0) << 3) << u;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < PLAN_PER; u++)
+                if (b + u < a.n_pages_arena && __ldcg(&a.refs[b + u]) == 0) free_bits |= 1u << u;
+        }
         int sum;
         int at = found + block_scan(__popc(free_bits), warp_sums, &sum);
         for (; free_bits; free_bits &= free_bits - 1, at++)
@@ -220,7 +257,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs 
     if (t == 0) {
         for (int w = 1; w < 32; w++) columns = max(columns, warp_sums[w]);
         a.head[0] = 0;
-        a.head[1] = n_copies;
+        a.head[1] = s_copies;
         a.head[2] = columns;
         *a.status = 0;
     }
@@ -234,7 +271,7 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_apply_kernel(const ForkArgs
     if (a.head[0]) {   // nothing changes: the deltas are taken back
         for (int p = blockIdx.x; p < a.n; p += gridDim.x) {
             const OldRow r = old_row(a, p);
-            add_deltas(a, p, r, -1);
+            add_deltas(a, p, r, -1, threadIdx.x, FORK_THREADS);
         }
         return;
     }
@@ -278,7 +315,16 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_apply_kernel(const ForkArgs
         const uint4* from = (const uint4*)(arena + ((int64_t)a.src[i] * a.n_layer + layer) * page_bytes);
         uint4* to = (uint4*)(arena + ((int64_t)a.list[a.first[i]] * a.n_layer + layer) * page_bytes);
         const int n16 = (int)(a.new_len[i] % KVB * a.slot_bytes / 16);
-        for (int x = threadIdx.x; x < n16; x += FORK_THREADS) to[x] = from[x];
+        // all of a thread's loads before its stores: from and to are different pages
+        for (int x0 = threadIdx.x; x0 < n16; x0 += FORK_BATCH * FORK_THREADS) {
+            uint4 r[FORK_BATCH];
+#pragma unroll
+            for (int e = 0; e < FORK_BATCH; e++)
+                if (x0 + e * FORK_THREADS < n16) r[e] = __ldcs(from + x0 + e * FORK_THREADS);
+#pragma unroll
+            for (int e = 0; e < FORK_BATCH; e++)
+                if (x0 + e * FORK_THREADS < n16) to[x0 + e * FORK_THREADS] = r[e];
+        }
     }
 }
 
@@ -309,9 +355,14 @@ cudaError_t launch_kv_fork(void* k, void* v, int64_t n_arena_blocks, int n_layer
     a.first = s; s += n;
     a.copies = s; s += n;
     a.list = s;
-    cudaError_t e = launch_pdl(fork_deltas_kernel, dim3((unsigned)n), dim3(FORK_THREADS), 0, st, a);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, a);
+    cudaError_t e;
+    if (n <= PLAN_THREADS && (int64_t)n * mbs <= FORK_SMALL) {
+        e = launch_pdl(fork_plan_kernel<true>, dim3(1), dim3(PLAN_THREADS), 0, st, a);
+    } else {
+        e = launch_pdl(fork_deltas_kernel, dim3((unsigned)n), dim3(FORK_THREADS), 0, st, a);
+        if (e != cudaSuccess) return e;
+        e = launch_pdl(fork_plan_kernel<false>, dim3(1), dim3(PLAN_THREADS), 0, st, a);
+    }
     if (e != cudaSuccess) return e;
     int cols = STRIP_INTS / n;
     cols = cols > 32 ? 32 : cols;

@@ -419,6 +419,21 @@ def test_fork_many_rows_and_a_large_arena(ops):
     assert run_fork(ops, t, refs, lens, held, [int(x) for x in rng.integers(-1, n, n)], [1] * n, n_layer=1, hkv=1)[5] == 0
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_fork_wide_tables(ops, seed):
+    """Tables of more entries than one CTA counts by itself, with bad input and too few blocks among them."""
+    rng = np.random.default_rng(100 + seed)
+    n = [30, 300, 1100, 64][seed]
+    t, refs, lens, held = random_rows(rng, n, 9, 15000, 130)
+    t = [r + [int(x) for x in rng.integers(-5, 20000, 2200 - len(r))] for r in t]
+    parents = [int(x) for x in rng.integers(-1, n, n)]
+    want = run_fork(ops, t, refs, lens, held, parents, [1] * n, n_layer=1, hkv=1)
+    assert want[5] == 0
+    if seed < 2:
+        assert run_fork(ops, t, refs, lens, held, parents, [1] * (n - 1) + [40000], n_layer=1, hkv=1)[5] == -1
+        assert run_fork(ops, t, refs, lens, held, [0] * n, [9000] * n, n_layer=1, hkv=1)[5] > 0
+
+
 def test_fork_far_blocks_and_capture(ops):
     """Copies between blocks behind the 2^31st element of the arena, from a captured graph."""
     nb = 140000
