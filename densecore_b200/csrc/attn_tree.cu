@@ -49,6 +49,9 @@ struct TreeArgs {
     // scratch
     float *part_o, *part_ml;     // [2 G][rows][128], [2 G][rows][2]
     struct TreeCut* cuts;        // [G]
+    struct TreeStart* begins;    // [G]
+    int64_t* prefix;             // [n_seqs + 1]: units before each sequence
+    int G;
     int part_rows;               // rows of the largest row tile
     int q_rows;                  // the same in eights: rows of a Q tile
     int row_tiles;               // of the largest sequence
@@ -58,8 +61,10 @@ struct TreeArgs {
 
 // an item that CTA c begins and later CTAs go on with (rows = 0: none)
 struct TreeCut {
-    int64_t begin, end, T;       // units of the item; of the batch
     int rows, s0, row0, kvh;
+    int parts;                   // CTAs that worked on it
+    int first;                   // sparse: its first unit
+    int T;                       // sparse: units of the batch, fewer than CTAs (0: no CTA is without one)
 };
 
 // ---- the batch's units ----
@@ -131,49 +136,65 @@ __device__ __forceinline__ bool seg_next(const TreeArgs& a, TreeSeg& g) {
     return true;
 }
 
-// Sum of all units, and the sequence and offset in it of unit begin(c): every thread of the CTA calls
-// it; at[0] = sequence, at[1] = its first unit, at[2] = T (shared memory); sums: a slot per warp.
+// where a CTA's range begins
+struct TreeStart {
+    int N;                       // its units
+    int sparse;                  // units of the batch if they are fewer than CTAs, else 0
+    int64_t u0;                  // its first unit
+    TreeSeg g;
+};
+
+// Every CTA's range, by one CTA of THREADS: the sequences' units summed up, then a thread per range.
 template <int ROWS, int KEYS, int THREADS>
-__device__ void tree_locate(const TreeArgs& a, int64_t* at, int64_t* sums) {
+__device__ void tree_plan_ranges(const TreeArgs& a) {
+    __shared__ int64_t sums[THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t T = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        int64_t run = 0;
-        for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
-            const int i = i0 + threadIdx.x;
-            int64_t u = 0;
-            if (i < a.n_seqs) {
-                const TreeSeq s = tree_seq<ROWS, KEYS>(a, i, pass == 0 && blockIdx.x == 0);
-                u = (int64_t)s.tiles * s.row_tiles * a.hkv;
-            }
-            int64_t x = u;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 31) sums[warp] = x;
-            __syncthreads();
-            int64_t before = run;
-#pragma unroll
-            for (int w = 0; w < THREADS / 32; w++) {
-                if (w < warp) before += sums[w];
-                run += sums[w];
-            }
-            if (pass || a.n_seqs <= THREADS) {     // a batch that fits one step needs no second pass
-                const int64_t u0 = sk_begin(blockIdx.x, pass ? T : run, gridDim.x);
-                if (u && u0 >= before + x - u && u0 < before + x) {
-                    at[0] = i;
-                    at[1] = before + x - u;
-                }
-            }
+    int64_t run = 0;
+    for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
+        const int i = i0 + threadIdx.x;
+        int64_t u = 0;
+        if (i < a.n_seqs) {
+            const TreeSeq s = tree_seq<ROWS, KEYS>(a, i, true);
+            u = (int64_t)s.tiles * s.row_tiles * a.hkv;
         }
-        T = run;
-        if (a.n_seqs <= THREADS) break;
+        int64_t x = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        int64_t before = run;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; w++) {
+            if (w < warp) before += sums[w];
+            run += sums[w];
+        }
+        if (i < a.n_seqs) a.prefix[i] = before + x - u;
     }
-    if (threadIdx.x == 0) at[2] = T;
+    const int64_t T = run;
+    if (threadIdx.x == 0) a.prefix[a.n_seqs] = T;
     __syncthreads();
+    for (int c = threadIdx.x; c < a.G; c += THREADS) {
+        const int64_t u0 = sk_begin(c, T, a.G), u1 = sk_begin(c + 1, T, a.G);
+        TreeStart b = {};
+        b.N = (int)(u1 - u0);
+        b.sparse = T < a.G ? (int)T : 0;
+        b.u0 = u0;
+        if (b.N) {
+            int lo = 0, hi = a.n_seqs;             // the last sequence that begins at or before u0
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (a.prefix[mid] <= u0) lo = mid;
+                else hi = mid;
+            }
+            b.g = seg_first<ROWS, KEYS>(a, lo, (int)(u0 - a.prefix[lo]), b.N);
+        }
+        a.begins[c] = b;
+        a.cuts[c].rows = 0;
+    }
 }
 
 // mask bits of keys g0 .. g0 + 31 (as positions) for drafted token `tok` (row of q): history, then draft
@@ -336,12 +357,17 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
 
 // Q as fp16 halves in the tiles that tree_wide_kernel copies: [hi, lo][half of 64 dims][q_rows][128 B],
 // 128-byte swizzle, each row scaled by a power of two (its sign the scale's).  A warp is a row: CTA
-// (drafted token, sequence), heads in turn.
+// (drafted token, sequence), heads in turn.  One CTA more plans the ranges.
 constexpr int TQ_WARPS = 8;
 __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a) {
     pdl_wait();
     pdl_trigger();
-    const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, blockIdx.y, false);
+    if (blockIdx.y == 0) {                        // first in the launch order
+        if (blockIdx.x == 0) tree_plan_ranges<TW_ROWS, TW_KEYS, TQ_WARPS * 32>(a);
+        return;
+    }
+    const int seq = blockIdx.y - 1;
+    const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, seq, false);
     const int t = blockIdx.x, lane = threadIdx.x & 31;
     if (t >= s.ns) return;
     const float* q = a.q + (int64_t)(s.s0 + t) * a.hq * HD + 4 * lane;
@@ -349,7 +375,7 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
     for (int h = threadIdx.x >> 5; h < a.hq; h += TQ_WARPS) {
         const float4 x = *(const float4*)(q + h * HD);
         const int kvh = h / a.nrep, R = t * a.nrep + h - kvh * a.nrep, rt = R / TW_ROWS, r = R - rt * TW_ROWS;
-        const int64_t tile = ((int64_t)blockIdx.y * a.row_tiles + rt) * a.hkv + kvh;
+        const int64_t tile = ((int64_t)seq * a.row_tiles + rt) * a.hkv + kvh;
         const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
         // exponent of the row's largest value (0 rows and subnormal ones: the least)
         int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(m)) >> 23) - 127;
@@ -402,12 +428,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();
-    int64_t* at = (int64_t*)smem;                 // the Q space, before Q
-    tree_locate<TW_ROWS, TW_KEYS, TW_THREADS>(a, at, at + 4);
-    const int64_t T = at[2], u0 = sk_begin(blockIdx.x, T, gridDim.x), u1 = sk_begin(blockIdx.x + 1, T, gridDim.x);
-    const int N = (int)(u1 - u0);
-    const int seq0 = N ? (int)at[0] : 0, off0 = N ? (int)(u0 - at[1]) : 0;
-    if (threadIdx.x == 0) a.cuts[blockIdx.x].rows = 0;
+    const TreeStart& start = a.begins[blockIdx.x];
+    const int N = start.N;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -424,7 +446,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             // 16 boxes of 2 KB a tile, one for each of 16 lanes: a warp issues one in about 80 cycles
             const bool is_v = warp == 3;
             const CUtensorMap* map = is_v ? &vmap : &kmap;
-            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            TreeSeg g = start.g;
             const int page = lane >> 1, half = lane & 1;
             const int beyond = (int)(a.n_arena_blocks * a.n_layer * KVB);   // out of the arena: zeros
             // block id of this lane's page in a tile, INT32_MIN behind the sequence's end (no read)
@@ -484,7 +506,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             const bool leader = elect_one();
             const int b = warp - 1;
             const uint32_t S = tm + b * 128, O = tm + 256 + b * 128;   // P takes S's place
-            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            TreeSeg g = start.g;
             int seg = 0, end = g.tiles;            // the segment's end among the range's units
             bool begins = true;                    // its Q not waited for yet
             uint64_t* q_empty = C.q_empty[b];
@@ -579,7 +601,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         uint32_t cleans = 0;
         int n = 0;
         if (N) {
-            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            TreeSeg g = start.g;
             do {
                 const bool valid = r < g.rows, live = quad * 32 < g.rows;
                 const int hist = g.s.L - g.s.ns;
@@ -719,10 +741,10 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         const uint32_t O = tmem + ((uint32_t)(quad * 32) << 16) + 256;
         int n = 0;
         if (N) {
-            TreeSeg g = seg_first<TW_ROWS, TW_KEYS>(a, seq0, off0, N);
+            TreeSeg g = start.g;
             do {
                 const bool valid = r < g.rows, live = quad * 32 < g.rows;
-                const int64_t begin = u0 + n - g.tile0;
+                const bool first = g.tile0 == 0;
                 uint64_t acc[64];
 #pragma unroll
                 for (int i = 0; i < 64; i++) acc[i] = 0;
@@ -768,7 +790,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 const bool whole = g.tile0 == 0 && g.tiles == g.s.tiles;
                 if (valid) {
                     const int R = g.rt * TW_ROWS + r;
-                    const size_t part = ((size_t)blockIdx.x * 2 + (u0 > begin ? 0 : 1)) * a.part_rows + r;
+                    const size_t part = ((size_t)blockIdx.x * 2 + (first ? 1 : 0)) * a.part_rows + r;
                     float* dst = a.part_o + part * HD;
                     float f = 1.0f;
                     if (whole) {
@@ -786,8 +808,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         *(float4*)(dst + 2 * i) = y;
                     }
                 }
-                if (!whole && g.tile0 == 0 && threadIdx.x == 12 * 32)
-                    a.cuts[blockIdx.x] = {begin, begin + g.s.tiles, T, g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh};
+                if (!whole && first && threadIdx.x == 12 * 32) {
+                    // the item ends in the CTA that has its last unit; with fewer units than CTAs, each of its
+                    // units is a CTA's only one
+                    const int64_t begin = start.u0 + n - g.tiles, T = a.prefix[a.n_seqs];
+                    const int parts = start.sparse ? g.s.tiles : (int)sk_owner(begin + g.s.tiles - 1, T, a.G) - (int)blockIdx.x + 1;
+                    a.cuts[blockIdx.x] = {g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh, parts, (int)begin, start.sparse};
+                }
             } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
         }
     }
@@ -1135,7 +1162,7 @@ __global__ void __launch_bounds__((TF_CONS + 1) * 32, 2) tree_few_kernel(
 }
 
 // The parts of a row, 32 at a time: m and l a lane each, then the outputs with all loads apart from the
-// sums (a lane 4 dims).  part(x): index of the x-th part, or -1 if it left nothing.
+// sums (a lane 4 dims).  part(x): index of the x-th part.
 template <class F>
 __device__ __forceinline__ void tree_join(const TreeArgs& a, int parts, F part, float* dst) {
     const int lane = threadIdx.x & 31;
@@ -1189,17 +1216,17 @@ __global__ void __launch_bounds__(TC_ROWS * 32) tree_join_kernel(const TreeArgs 
 }
 
 // tree_wide_kernel's items that several CTAs worked on, in CTA order: CTA (CTA that began an item, 8 rows)
-__global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeArgs a, int G) {
+__global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeArgs a) {
     pdl_wait();
     pdl_trigger();
     const int c = blockIdx.x, r = blockIdx.y * TC_ROWS + (threadIdx.x >> 5);
     const TreeCut cut = a.cuts[c];
     if (r >= cut.rows) return;
     const int R = cut.row0 + r;
-    tree_join(a, (int)sk_owner(cut.end - 1, cut.T, G) - c + 1,
+    tree_join(a, cut.parts,
               [&](int x) {
-                  if (sk_begin(c + x, cut.T, G) == sk_begin(c + x + 1, cut.T, G)) return (int64_t)-1;
-                  return ((int64_t)(c + x) * 2 + (x == 0 ? 1 : 0)) * a.part_rows + r;
+                  const int64_t cta = cut.T ? ((int64_t)(cut.first + x + 1) * a.G - 1) / cut.T : c + x;
+                  return (cta * 2 + (x == 0 ? 1 : 0)) * a.part_rows + r;
               },
               a.out + ((int64_t)(cut.s0 + R / a.nrep) * a.hq + cut.kvh * a.nrep + R % a.nrep) * HD);
 }
@@ -1226,7 +1253,7 @@ struct TreePlan {
     int rows;                   // of a part
     int splits, bps;            // few: splits of a sequence's blocks, blocks of one
     int G, q_rows, row_tiles;   // wide
-    size_t o_bytes, ml_bytes, cut_bytes, q_bytes, e_bytes;
+    size_t o_bytes, ml_bytes, cut_bytes, start_bytes, prefix_bytes, q_bytes, e_bytes;
 };
 constexpr int TF_ROWS = 32;
 static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
@@ -1249,6 +1276,8 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
         p.row_tiles = (int)((rows + TW_ROWS - 1) / TW_ROWS);
         parts = (size_t)2 * p.G;
         p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
+        p.start_bytes = align256((size_t)p.G * sizeof(TreeStart));
+        p.prefix_bytes = align256((size_t)(n_seqs + 1) * 8);
         const size_t q = (size_t)n_seqs * p.row_tiles * hkv * p.q_rows;
         p.q_bytes = align256(q * 512);
         p.e_bytes = align256(q);
@@ -1259,7 +1288,7 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
 }
 size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
     const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
-    return p.o_bytes + p.ml_bytes + p.cut_bytes + p.q_bytes + p.e_bytes;
+    return p.o_bytes + p.ml_bytes + p.cut_bytes + p.start_bytes + p.prefix_bytes + p.q_bytes + p.e_bytes;
 }
 
 template <int MT>
@@ -1292,7 +1321,10 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     a.part_o = (float*)at;
     a.part_ml = (float*)(at += p.o_bytes);
     a.cuts = (TreeCut*)(at += p.ml_bytes);
-    a.q_tiles = at += p.cut_bytes;
+    a.begins = (TreeStart*)(at += p.cut_bytes);
+    a.prefix = (int64_t*)(at += p.start_bytes);
+    a.G = p.G;
+    a.q_tiles = at += p.prefix_bytes;
     a.q_exps = (int8_t*)(at += p.q_bytes);
     a.part_rows = p.rows;
     a.q_rows = p.q_rows;
@@ -1305,12 +1337,12 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     if (p.few) return p.rows <= 16 ? launch_few<1>(km, vm, a, p, st) : launch_few<2>(km, vm, a, p, st);
     e = DCG_SMEM_ATTR(tree_wide_kernel, TW_SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs), dim3(TQ_WARPS * 32), 0, st, a);
+    e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(tree_wide_kernel, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
     if (e != cudaSuccess) return e;
     return launch_pdl(tree_combine_kernel, dim3((unsigned)p.G, (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
-                      dim3(TC_ROWS * 32), 0, st, a, p.G);
+                      dim3(TC_ROWS * 32), 0, st, a);
 }
 
 }  // namespace dcg
