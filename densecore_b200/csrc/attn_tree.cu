@@ -6,9 +6,9 @@
 //
 // The (token, query head) pairs that share a kv head are the rows of one matrix: every K/V byte is
 // read once for up to 128 of them.  An item is (sequence, kv head, tile of 128 rows), a unit one tile
-// of 128 keys of an item; the units of the whole batch, in order, are cut into one equal range per
-// CTA (one CTA per SM), so ragged contexts load every SM alike.  Items that a range cuts leave their
-// parts (unnormalised output, max, sum) in scratch; tree_combine_kernel joins them in CTA order.
+// of 128 keys of an item; the units of the whole batch, in order, are cut into one range of equal cost
+// per CTA (one CTA per SM), so ragged contexts load every SM alike.  Items that a range cuts leave
+// their parts (unnormalised output, max, sum) in scratch; tree_combine_kernel joins them in CTA order.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
@@ -50,7 +50,8 @@ struct TreeArgs {
     float *part_o, *part_ml;     // [2 G][rows][128], [2 G][rows][2]
     struct TreeCut* cuts;        // [G]
     struct TreeStart* begins;    // [G]
-    int64_t* prefix;             // [n_seqs + 1]: units before each sequence
+    int64_t* prefix;             // [2][n_seqs + 1]: costs and units before each sequence
+    int64_t* bounds;             // [G + 1]: first unit of each CTA
     int G;
     int part_rows;               // rows of the largest row tile
     int q_rows;                  // the same in eights: rows of a Q tile
@@ -62,9 +63,7 @@ struct TreeArgs {
 // an item that CTA c begins and later CTAs go on with (rows = 0: none)
 struct TreeCut {
     int rows, s0, row0, kvh;
-    int parts;                   // CTAs that worked on it
-    int first;                   // sparse: its first unit
-    int T;                       // sparse: units of the batch, fewer than CTAs (0: no CTA is without one)
+    int parts;                   // CTAs that worked on it: c, c + 1, ...
 };
 
 // ---- the batch's units ----
@@ -105,20 +104,6 @@ __device__ __forceinline__ void seg_shape(const TreeArgs& a, TreeSeg& g) {
     g.left -= g.tiles;
 }
 template <int ROWS, int KEYS>
-__device__ __forceinline__ TreeSeg seg_first(const TreeArgs& a, int seq, int off, int units) {
-    TreeSeg g;
-    g.seq = seq;
-    g.s = tree_seq<ROWS, KEYS>(a, seq, false);
-    g.next = seq_or_none<ROWS, KEYS>(a, seq + 1);
-    const int item = off / g.s.tiles;
-    g.tile0 = off - item * g.s.tiles;
-    g.kvh = item / g.s.row_tiles;
-    g.rt = item - g.kvh * g.s.row_tiles;
-    g.left = units;
-    seg_shape<ROWS>(a, g);
-    return g;
-}
-template <int ROWS, int KEYS>
 __device__ __forceinline__ bool seg_next(const TreeArgs& a, TreeSeg& g) {
     if (g.left <= 0) return false;
     g.tile0 = 0;
@@ -139,61 +124,94 @@ __device__ __forceinline__ bool seg_next(const TreeArgs& a, TreeSeg& g) {
 // where a CTA's range begins
 struct TreeStart {
     int N;                       // its units
-    int sparse;                  // units of the batch if they are fewer than CTAs, else 0
     int64_t u0;                  // its first unit
     TreeSeg g;
 };
 
-// Every CTA's range, by one CTA of THREADS: the sequences' units summed up, then a thread per range.
-template <int ROWS, int KEYS, int THREADS>
+// Every CTA's range, by one CTA of THREADS.  An item costs its units and EXTRA for its beginning, its
+// masked last units and its output; the ranges cut the summed costs into equal parts, and a cut that
+// falls into an item's extra cost goes to its first unit.  (A CTA inside an item has a unit at least, so
+// an item's CTAs are consecutive.)
+template <int ROWS, int KEYS, int EXTRA, int THREADS>
 __device__ void tree_plan_ranges(const TreeArgs& a) {
-    __shared__ int64_t sums[THREADS / 32];
+    __shared__ int64_t sums[2][THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t run = 0;
+    int64_t *cost = a.prefix, *units = a.prefix + a.n_seqs + 1;
+    int64_t run = 0, run_u = 0;
     for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
         const int i = i0 + threadIdx.x;
-        int64_t u = 0;
+        int64_t items = 0, u = 0;
         if (i < a.n_seqs) {
             const TreeSeq s = tree_seq<ROWS, KEYS>(a, i, true);
-            u = (int64_t)s.tiles * s.row_tiles * a.hkv;
+            items = s.tiles ? (int64_t)s.row_tiles * a.hkv : 0;
+            u = s.tiles * items;
         }
-        int64_t x = u;
+        const int64_t c = u + EXTRA * items;
+        int64_t x = c, y = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            const int64_t p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) {
+                x += p;
+                y += q;
+            }
         }
         __syncthreads();
-        if (lane == 31) sums[warp] = x;
+        if (lane == 31) {
+            sums[0][warp] = x;
+            sums[1][warp] = y;
+        }
         __syncthreads();
-        int64_t before = run;
+        int64_t before = run, before_u = run_u;
 #pragma unroll
         for (int w = 0; w < THREADS / 32; w++) {
-            if (w < warp) before += sums[w];
-            run += sums[w];
+            if (w < warp) {
+                before += sums[0][w];
+                before_u += sums[1][w];
+            }
+            run += sums[0][w];
+            run_u += sums[1][w];
         }
-        if (i < a.n_seqs) a.prefix[i] = before + x - u;
+        if (i < a.n_seqs) {
+            cost[i] = before + x - c;
+            units[i] = before_u + y - u;
+        }
     }
-    const int64_t T = run;
-    if (threadIdx.x == 0) a.prefix[a.n_seqs] = T;
+    const int64_t V = run;
+    const int G = (int)min((int64_t)a.G, V);      // no more ranges than cost: none is empty inside an item
     __syncthreads();
-    for (int c = threadIdx.x; c < a.G; c += THREADS) {
-        const int64_t u0 = sk_begin(c, T, a.G), u1 = sk_begin(c + 1, T, a.G);
+    for (int c = threadIdx.x; c <= a.G; c += THREADS) {
+        int64_t u0 = run_u;
         TreeStart b = {};
-        b.N = (int)(u1 - u0);
-        b.sparse = T < a.G ? (int)T : 0;
-        b.u0 = u0;
-        if (b.N) {
-            int lo = 0, hi = a.n_seqs;             // the last sequence that begins at or before u0
+        if (c < G) {
+            const int64_t v = sk_begin(c, V, G);
+            int lo = 0, hi = a.n_seqs;             // the last sequence that begins at or before v
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (a.prefix[mid] <= u0) lo = mid;
+                if (cost[mid] <= v) lo = mid;
                 else hi = mid;
             }
-            b.g = seg_first<ROWS, KEYS>(a, lo, (int)(u0 - a.prefix[lo]), b.N);
+            b.g.seq = lo;
+            b.g.s = tree_seq<ROWS, KEYS>(a, lo, false);
+            b.g.next = seq_or_none<ROWS, KEYS>(a, lo + 1);
+            const int off = (int)(v - cost[lo]), each = b.g.s.tiles + EXTRA, item = off / each;
+            b.g.tile0 = max(0, off - item * each - EXTRA);
+            b.g.kvh = item / b.g.s.row_tiles;
+            b.g.rt = item - b.g.kvh * b.g.s.row_tiles;
+            u0 = units[lo] + (int64_t)item * b.g.s.tiles + b.g.tile0;
         }
-        a.begins[c] = b;
-        a.cuts[c].rows = 0;
+        a.bounds[c] = b.u0 = u0;
+        if (c < a.G) {
+            a.begins[c] = b;
+            a.cuts[c].rows = 0;
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.G; c += THREADS) {
+        TreeStart& b = a.begins[c];
+        b.N = (int)(a.bounds[c + 1] - a.bounds[c]);
+        b.g.left = b.N;
+        if (b.N) seg_shape<ROWS>(a, b.g);
     }
 }
 
@@ -260,6 +278,7 @@ constexpr int TW_OFF_RING = 2 * TW_BUF;           // Q hi, Q lo first
 constexpr int TW_OFF_CTRL = TW_OFF_RING + TW_RING * TW_BUF;
 constexpr int TW_CTRL = 3072;
 constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // all of it: 227 KB
+constexpr int TW_EXTRA = 2;                       // an item's fixed cost in units (7,000 cycles against 3,300 a unit)
 constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^8: the small ones stay above fp16's least
 // registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128
 constexpr int TW_REGS_CTRL = 56, TW_REGS_SOFT = 128, TW_REGS_OUT = 200;
@@ -363,7 +382,7 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
     pdl_wait();
     pdl_trigger();
     if (blockIdx.y == 0) {                        // first in the launch order
-        if (blockIdx.x == 0) tree_plan_ranges<TW_ROWS, TW_KEYS, TQ_WARPS * 32>(a);
+        if (blockIdx.x == 0) tree_plan_ranges<TW_ROWS, TW_KEYS, TW_EXTRA, TQ_WARPS * 32>(a);
         return;
     }
     const int seq = blockIdx.y - 1;
@@ -809,11 +828,14 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     }
                 }
                 if (!whole && first && threadIdx.x == 12 * 32) {
-                    // the item ends in the CTA that has its last unit; with fewer units than CTAs, each of its
-                    // units is a CTA's only one
-                    const int64_t begin = start.u0 + n - g.tiles, T = a.prefix[a.n_seqs];
-                    const int parts = start.sparse ? g.s.tiles : (int)sk_owner(begin + g.s.tiles - 1, T, a.G) - (int)blockIdx.x + 1;
-                    a.cuts[blockIdx.x] = {g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh, parts, (int)begin, start.sparse};
+                    const int64_t end = start.u0 + n - g.tiles + g.s.tiles;
+                    int lo = blockIdx.x, hi = a.G;   // the CTA that has the item's last unit
+                    while (hi - lo > 1) {
+                        const int mid = (lo + hi) / 2;
+                        if (a.bounds[mid] < end) lo = mid;
+                        else hi = mid;
+                    }
+                    a.cuts[blockIdx.x] = {g.rows, g.s.s0, g.rt * TW_ROWS, g.kvh, lo - (int)blockIdx.x + 1};
                 }
             } while (seg_next<TW_ROWS, TW_KEYS>(a, g));
         }
@@ -1224,10 +1246,7 @@ __global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeAr
     if (r >= cut.rows) return;
     const int R = cut.row0 + r;
     tree_join(a, cut.parts,
-              [&](int x) {
-                  const int64_t cta = cut.T ? ((int64_t)(cut.first + x + 1) * a.G - 1) / cut.T : c + x;
-                  return (cta * 2 + (x == 0 ? 1 : 0)) * a.part_rows + r;
-              },
+              [&](int x) { return ((int64_t)(c + x) * 2 + (x == 0 ? 1 : 0)) * a.part_rows + r; },
               a.out + ((int64_t)(cut.s0 + R / a.nrep) * a.hq + cut.kvh * a.nrep + R % a.nrep) * HD);
 }
 
@@ -1253,7 +1272,7 @@ struct TreePlan {
     int rows;                   // of a part
     int splits, bps;            // few: splits of a sequence's blocks, blocks of one
     int G, q_rows, row_tiles;   // wide
-    size_t o_bytes, ml_bytes, cut_bytes, start_bytes, prefix_bytes, q_bytes, e_bytes;
+    size_t o_bytes, ml_bytes, cut_bytes, start_bytes, prefix_bytes, bound_bytes, q_bytes, e_bytes;
 };
 constexpr int TF_ROWS = 32;
 static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
@@ -1277,7 +1296,8 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
         parts = (size_t)2 * p.G;
         p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
         p.start_bytes = align256((size_t)p.G * sizeof(TreeStart));
-        p.prefix_bytes = align256((size_t)(n_seqs + 1) * 8);
+        p.prefix_bytes = align256((size_t)(n_seqs + 1) * 2 * 8);
+        p.bound_bytes = align256((size_t)(p.G + 1) * 8);
         const size_t q = (size_t)n_seqs * p.row_tiles * hkv * p.q_rows;
         p.q_bytes = align256(q * 512);
         p.e_bytes = align256(q);
@@ -1288,7 +1308,7 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
 }
 size_t tree_scratch_bytes(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
     const TreePlan p = tree_plan(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
-    return p.o_bytes + p.ml_bytes + p.cut_bytes + p.start_bytes + p.prefix_bytes + p.q_bytes + p.e_bytes;
+    return p.o_bytes + p.ml_bytes + p.cut_bytes + p.start_bytes + p.prefix_bytes + p.bound_bytes + p.q_bytes + p.e_bytes;
 }
 
 template <int MT>
@@ -1324,7 +1344,8 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     a.begins = (TreeStart*)(at += p.cut_bytes);
     a.prefix = (int64_t*)(at += p.start_bytes);
     a.G = p.G;
-    a.q_tiles = at += p.prefix_bytes;
+    a.bounds = (int64_t*)(at += p.prefix_bytes);
+    a.q_tiles = at += p.bound_bytes;
     a.q_exps = (int8_t*)(at += p.q_bytes);
     a.part_rows = p.rows;
     a.q_rows = p.q_rows;
