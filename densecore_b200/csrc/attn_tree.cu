@@ -412,6 +412,9 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
     }
 }
 
+// TM = 64 where every item has at most 64 rows: rows 16 q .. 16 q + 15 of a 64-row accumulator lie in lanes
+// 32 q .. 32 q + 15 of tensor memory.
+template <int TM>
 __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TreeArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];   // no static shared memory: starts on a KB
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             // ---------------- MMA issue: warp 1 the even units, warp 2 the odd ones ----------------
             // Each in step, one elected thread issuing.  A warp's polls, and its waits for the tensor core to
             // take its last operands, leave the core with the other's work.
-            constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
+            constexpr uint32_t id_s = idesc_f16(TM, TW_KEYS, false), id_o = idesc_f16(TM, HD, true);
             const uint32_t qs = smem_u32(smem), rg = qs + TW_OFF_RING, q_half = a.q_rows * 128;
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const bool leader = elect_one();
@@ -615,14 +618,15 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         }
     } else if (warp < 12) {
         // ---------------- softmax of every other tile (thread = row) ----------------
-        const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+        const int wg = (warp - 4) >> 2, quad = warp & 3, tid = quad * 32 + lane;
+        const int r = quad * (TM / 4) + lane;      // of lanes below TM / 4
         const uint32_t S = tmem + ((uint32_t)(quad * 32) << 16) + wg * 128;
         uint32_t cleans = 0;
         int n = 0;
         if (N) {
             TreeSeg g = start.g;
             do {
-                const bool valid = r < g.rows, live = quad * 32 < g.rows;
+                const bool valid = lane < TM / 4 && r < g.rows, live = quad * (TM / 4) < g.rows;
                 const int hist = g.s.L - g.s.ns;
                 const int tok = g.s.s0 + (valid ? (g.rt * TW_ROWS + r) / a.nrep : 0);
                 // c > 0 (the scale's sign is in Q), and not 0: c x -inf has to stay -inf
@@ -644,8 +648,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         const uint32_t lv = tw_v(n, N);
                         ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (lv / TW_RING) & 1, &g_tree_error));
                         if (!ok) break;
-                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + r * 128;
-                        const int key = kb + r;
+                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + tid * 128;   // a key per thread
+                        const int key = kb + tid;
                         bool odd = false;
                         if (key >= hist && key < g.s.L) {
 #pragma unroll 4
@@ -745,7 +749,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     }
                     if (k) ok = __all_sync(0xffffffffu, mbar_wait(&C.x_free[wg], (k - 1) & 1, &g_tree_error));
                     if (!ok) break;
-                    C.x[wg][r] = make_float2(m, sum);
+                    C.x[wg][tid] = make_float2(m, sum);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -756,13 +760,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     } else {
         // ---------------- the running output (thread = row) ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TW_REGS_OUT));
-        const int quad = warp & 3, r = quad * 32 + lane;
+        const int quad = warp & 3, r = quad * (TM / 4) + lane;
         const uint32_t O = tmem + ((uint32_t)(quad * 32) << 16) + 256;
         int n = 0;
         if (N) {
             TreeSeg g = start.g;
             do {
-                const bool valid = r < g.rows, live = quad * 32 < g.rows;
+                const bool valid = lane < TM / 4 && r < g.rows, live = quad * (TM / 4) < g.rows;
                 const bool first = g.tile0 == 0;
                 uint64_t acc[64];
 #pragma unroll
@@ -774,7 +778,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     ok = __all_sync(0xffffffffu, mbar_wait(&C.o_full[b], k & 1, &g_tree_error));
                     if (!ok) break;
                     tc_fence_after();
-                    const float2 x = C.x[b][r];
+                    const float2 x = C.x[b][quad * 32 + lane];
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&C.x_free[b]);
                     if (live) {
@@ -1356,11 +1360,11 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     if (e == cudaSuccess) e = tree_map(&vm, varena, hkv, n_slots, p.few ? 2 : 1);
     if (e != cudaSuccess) return e;
     if (p.few) return p.rows <= 16 ? launch_few<1>(km, vm, a, p, st) : launch_few<2>(km, vm, a, p, st);
-    e = DCG_SMEM_ATTR(tree_wide_kernel, TW_SMEM);
+    e = p.rows <= 64 ? DCG_SMEM_ATTR(tree_wide_kernel<64>, TW_SMEM) : DCG_SMEM_ATTR(tree_wide_kernel<128>, TW_SMEM);
     if (e != cudaSuccess) return e;
     e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(tree_wide_kernel, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
+    e = launch_pdl(p.rows <= 64 ? tree_wide_kernel<64> : tree_wide_kernel<128>, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
     if (e != cudaSuccess) return e;
     return launch_pdl(tree_combine_kernel, dim3((unsigned)p.G, (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
                       dim3(TC_ROWS * 32), 0, st, a);
