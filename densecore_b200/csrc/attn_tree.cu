@@ -286,7 +286,7 @@ static_assert(TW_REGS_CTRL + 2 * TW_REGS_SOFT + TW_REGS_OUT <= 512, "register sp
 
 struct TwCtrl {
     uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_full[2], o_free[2], x_free[2], cleaned[2];
-    uint64_t q_full[2], q_empty[2][2], mma_end[2];   // q_empty: by MMA warp and buffer
+    uint64_t q_full[2], q_empty[2][2], mma_end[2], s_sent[2];   // q_empty: by MMA warp and buffer
     uint32_t tmem;
     uint32_t bad[2][4];                           // per buffer: keys of its tile whose V is not finite
     float2 x[2][TW_ROWS];                         // a tile's row max and sum of p
@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             mbar_init(&C.q_empty[0][b], 1);
             mbar_init(&C.q_empty[1][b], 1);
             mbar_init(&C.mma_end[b], 1);
+            mbar_init(&C.s_sent[b], 1);
         }
         fence_mbar_init();
     }
@@ -566,6 +567,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                             }
                         }
                     }
+                    mbar_arrive(&C.s_sent[b]);
                     tc_commit(&C.s_full[b]);
                     tc_commit(&C.empty[slot]);
                     if (n + 2 >= end) tc_commit(&q_empty[qb]);
@@ -575,8 +577,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             if (b < N) issue_s(b, false);
             for (int n = b; n < N && ok; n += 2) {  // O of unit n, then S of unit n + 2 into the same buffer
                 const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
-                // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit, others P.  (The third keeps the
-                // two streams half a period apart: side by side, both softmaxes leave the tensor core idle.)
+                // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit issued, others P.  (The third keeps
+                // the two streams apart: side by side, both softmaxes leave the tensor core idle.)
                 uint64_t* bar = &C.p_full[b];
                 uint32_t parity = k & 1;
                 bool wait = true;
@@ -588,7 +590,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     parity = (k - 1) & 1;
                     wait = k > 0;
                 } else if (lane == 2) {
-                    bar = &C.s_full[b ^ 1];
+                    bar = &C.s_sent[b ^ 1];
                     parity = ((uint32_t)(n + 1) >> 1) & 1;
                     wait = n + 1 < N;
                 }
