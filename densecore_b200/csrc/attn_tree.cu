@@ -54,7 +54,7 @@ struct TreeArgs {
     int64_t* bounds;             // [G + 1]: first unit of each CTA
     int G;
     int part_rows;               // rows of the largest row tile
-    int q_rows;                  // the same in eights: rows of a Q tile
+    int q_rows;                  // the same in eights (up to TW_STACK of them: sixteens): rows of a Q tile
     int row_tiles;               // of the largest sequence
     uint8_t* q_tiles;            // [n_seqs][row_tiles][hkv] x q_rows * 512 B: Q as halves, as shared memory wants it
     int8_t* q_exps;              // the same x q_rows: exponents of the rows' scales
@@ -270,6 +270,7 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // ------------------------------------------------------------------------------------------
 constexpr int TW_ROWS = 128;
 constexpr int TW_KEYS = 128;
+constexpr int TW_STACK = 64;                      // up to so many rows an item: both halves in one accumulator
 constexpr int TW_RING = 5;
 constexpr int TW_BUF = TW_KEYS * HD * 2;          // 32 KB: [half of 64 dims][128 keys][128 B]
 constexpr int TW_HALF = TW_BUF / 2;
@@ -352,6 +353,23 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         : "memory");
 }
 
+// 16 lanes (16 into `taddr`'s 32, or from them on) x 32 columns as fragments: thread t has of each 8 columns b
+// row t / 4, columns 2 (t % 4) + {0, 1} in v[4 b], v[4 b + 1] and row t / 4 + 8 in the next two
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// and 16 lanes x 16 columns: of each 4 columns b row t / 4, column t % 4 in v[2 b] and row t / 4 + 8 in v[2 b + 1]
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 // ring position of the K and V tile of the range's n-th unit of N: K0 K1 V0 K2 V1 ... K(N-1) V(N-2) V(N-1)
 __device__ __forceinline__ uint32_t tw_k(int n) { return n ? 2 * n - 1 : 0; }
 __device__ __forceinline__ uint32_t tw_v(int n, int N) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; }
@@ -374,7 +392,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
-// Q as fp16 halves in the tiles that tree_wide_kernel copies: [hi, lo][half of 64 dims][q_rows][128 B],
+// Q as fp16 halves in the tiles that tree_wide_kernel copies: [hi, lo][half of 64 dims][q_rows][128 B], or
+// stacked [half of 64 dims][16 rows hi, the same lo, the next 16 hi, ...][128 B];
 // 128-byte swizzle, each row scaled by a power of two (its sign the scale's).  A warp is a row: CTA
 // (drafted token, sequence), heads in turn.  One CTA more plans the ranges.
 constexpr int TQ_WARPS = 8;
@@ -389,6 +408,8 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
     const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, seq, false);
     const int t = blockIdx.x, lane = threadIdx.x & 31;
     if (t >= s.ns) return;
+    const bool stacked = a.q_rows <= TW_STACK;
+    const int dims_half = a.q_rows * (stacked ? 256 : 128), to_lo = stacked ? 16 * 128 : a.q_rows * 256;
     const float* q = a.q + (int64_t)(s.s0 + t) * a.hq * HD + 4 * lane;
 #pragma unroll 4
     for (int h = threadIdx.x >> 5; h < a.hq; h += TQ_WARPS) {
@@ -404,17 +425,18 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
         cut_h2(x.x * f, x.y * f, h0, l0);
         cut_h2(x.z * f, x.w * f, h1, l1);
         // dims 4 lane .. +3: 8 bytes of 16-byte chunk (lane / 2) & 7 of its half
-        uint8_t* to = a.q_tiles + tile * a.q_rows * 512 + (lane >> 4) * a.q_rows * 128 + r * 128 +
+        const int at = stacked ? 2 * r - (r & 15) : r;
+        uint8_t* to = a.q_tiles + tile * a.q_rows * 512 + (lane >> 4) * dims_half + at * 128 +
                       ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
         *(uint2*)to = make_uint2(h0, h1);
-        *(uint2*)(to + a.q_rows * 256) = make_uint2(l0, l1);
+        *(uint2*)(to + to_lo) = make_uint2(l0, l1);
         if (lane == 0) a.q_exps[tile * a.q_rows + r] = (int8_t)e;
     }
 }
 
-// TM = 64 where every item has at most 64 rows: rows 16 q .. 16 q + 15 of a 64-row accumulator lie in lanes
-// 32 q .. 32 q + 15 of tensor memory.
-template <int TM>
+// STACKED: every item has at most 64 rows.  Row r = 16 q + i has its hi half in lane 32 q + i of the MMAs'
+// 128 and its lo half in lane 32 q + 16 + i, so 8 + 8 MMAs make a unit; S is the two lanes' sum, and so is O.
+template <bool STACKED>
 __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TreeArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];   // no static shared memory: starts on a KB
@@ -459,8 +481,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     const uint32_t tmem = C.tmem;
     bool ok = true;
 
-    // up to 64 rows there is room for two Q
-    const int q_bufs = a.q_rows <= 64 ? 2 : 1, q_bytes = a.q_rows * 512;
+    constexpr int q_bufs = STACKED ? 2 : 1;       // as many as there is room for
+    const int q_bytes = a.q_rows * 512;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_CTRL));
         if (N == 0) {
@@ -523,8 +545,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             // ---------------- MMA issue: warp 1 the even units, warp 2 the odd ones ----------------
             // Each in step, one elected thread issuing.  A warp's polls, and its waits for the tensor core to
             // take its last operands, leave the core with the other's work.
-            constexpr uint32_t id_s = idesc_f16(TM, TW_KEYS, false), id_o = idesc_f16(TM, HD, true);
-            const uint32_t qs = smem_u32(smem), rg = qs + TW_OFF_RING, q_half = a.q_rows * 128;
+            constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
+            const uint32_t qs = smem_u32(smem), rg = qs + TW_OFF_RING, q_half = a.q_rows * (STACKED ? 256 : 128);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const bool leader = elect_one();
             const int b = warp - 1;
@@ -556,13 +578,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     const uint32_t q = qs + qb * q_bytes;
                     const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
 #pragma unroll
-                    for (int h = 1; h >= 0; h--) {   // the lo half first
+                    for (int h = STACKED ? 0 : 1; h >= 0; h--) {   // the lo half first
 #pragma unroll
                         for (int d = 0; d < 2; d++) {
                             const uint64_t qd = umma_desc_sw128(q + (2 * h + d) * q_half);
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                if (h && !d && j == 0) mma_f16_ss<false>(S, qd + 2 * j, kd + d * (TW_HALF >> 4) + 2 * j, id_s);
+                                if (h == !STACKED && !d && j == 0) mma_f16_ss<false>(S, qd + 2 * j, kd + d * (TW_HALF >> 4) + 2 * j, id_s);
                                 else mma_f16_ss<true>(S, qd + 2 * j, kd + d * (TW_HALF >> 4) + 2 * j, id_s);
                             }
                         }
@@ -602,11 +624,12 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 if (leader) {
                     const uint64_t vd = umma_desc_mn128(rg + slot * TW_BUF);
 #pragma unroll
-                    for (int h = 1; h >= 0; h--)   // 16 keys = 2048 bytes per k-step
+                    for (int h = STACKED ? 0 : 1; h >= 0; h--)   // 16 keys = 2048 bytes per k-step
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            if (h && j == 0) mma_f16_ts<false>(O, S + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
-                            else mma_f16_ts<true>(O, S + 16 * j + 8 * h, vd + j * (2048 >> 4), id_o);
+                            const uint32_t P = S + (STACKED ? 8 : 16) * j + 8 * h;
+                            if (h == !STACKED && j == 0) mma_f16_ts<false>(O, P, vd + j * (2048 >> 4), id_o);
+                            else mma_f16_ts<true>(O, P, vd + j * (2048 >> 4), id_o);
                         }
                     tc_commit(&C.o_full[b]);
                     tc_commit(&C.empty[slot]);
@@ -619,22 +642,26 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             mbar_wait(&C.mma_end[b], 0, &g_tree_error);
         }
     } else if (warp < 12) {
-        // ---------------- softmax of every other tile (thread = row) ----------------
+        // ---------------- softmax of every other tile (thread = row; stacked: 4 threads for 2 rows) ----------------
         const int wg = (warp - 4) >> 2, quad = warp & 3, tid = quad * 32 + lane;
-        const int r = quad * (TM / 4) + lane;      // of lanes below TM / 4
+        const int r = STACKED ? quad * 16 + (lane & 15) : tid;
+        const int r0 = quad * 16 + (lane >> 2), r1 = r0 + 8;   // stacked: the rows of this thread's fragments
         const uint32_t S = tmem + ((uint32_t)(quad * 32) << 16) + wg * 128;
         uint32_t cleans = 0;
         int n = 0;
         if (N) {
             TreeSeg g = start.g;
             do {
-                const bool valid = lane < TM / 4 && r < g.rows, live = quad * (TM / 4) < g.rows;
+                const bool valid = r < g.rows, live = quad * (STACKED ? 16 : 32) < g.rows;
                 const int hist = g.s.L - g.s.ns;
                 const int tok = g.s.s0 + (valid ? (g.rt * TW_ROWS + r) / a.nrep : 0);
                 // c > 0 (the scale's sign is in Q), and not 0: c x -inf has to stay -inf
                 const int64_t tile = ((int64_t)g.seq * a.row_tiles + g.rt) * a.hkv + g.kvh;
-                const int qexp = valid ? a.q_exps[tile * a.q_rows + r] : 0;
-                const float c = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + qexp) << 23), 1e-37f);
+                auto scale = [&](int row) {
+                    const int qexp = row < g.rows ? a.q_exps[tile * a.q_rows + row] : 0;
+                    return fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + qexp) << 23), 1e-37f);
+                };
+                const float c = scale(STACKED ? r0 : r), c1 = STACKED ? scale(r1) : c;
                 for (int t = 0; t < g.tiles && ok; t++, n++) {
                     if ((int)(n & 1) != wg) continue;
                     const uint32_t k = (uint32_t)(n >> 1);
@@ -674,7 +701,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         if (lane == 0) mbar_arrive(&C.cleaned[wg]);
                         ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
                         if (!ok) break;
-                        if (live) {
+                        if (live && !STACKED) {
 #pragma unroll 1
                             for (int w = 0; w < 4; w++) {
                                 const uint32_t vis = valid ? tree_bits(a, g.s, tok, kb + 32 * w) : 0u;   // keys this row sees
@@ -689,8 +716,89 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                             tmem_wait_st();
                         }
                     }
-                    float m = -INFINITY, sum = 0.0f;
-                    if (live) {
+                    float m = -INFINITY, sum = 0.0f, m1 = -INFINITY, sum1 = 0.0f;
+                    if (STACKED && live) {
+                        uint32_t vis[2];                   // lane i and i + 16: the first and last 64 keys of row i
+                        if (special) {
+#pragma unroll 1
+                            for (int w = 0; w < 2; w++) {
+                                const uint32_t v = valid ? tree_bits(a, g.s, tok, kb + 64 * (lane >> 4) + 32 * w) : 0u;
+                                if (w) vis[1] = v;
+                                else vis[0] = v;
+                            }
+                        }
+                        bool poison1 = false;
+                        float x[4][16];                    // the scores, then p
+                        uint32_t hi[2][16], lo[2][16];     // one is loaded while the other is worked on
+                        tmem_ld_frag(S, hi[0]);
+                        tmem_ld_frag(S + (16u << 16), lo[0]);
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            tmem_wait_ld();
+                            if (w < 3) {
+                                tmem_ld_frag(S + 32 * (w + 1), hi[(w + 1) & 1]);
+                                tmem_ld_frag(S + (16u << 16) + 32 * (w + 1), lo[(w + 1) & 1]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                unpack2(add2(pack2(__uint_as_float(hi[w & 1][i]), __uint_as_float(hi[w & 1][i + 1])),
+                                             pack2(__uint_as_float(lo[w & 1][i]), __uint_as_float(lo[w & 1][i + 1]))), x[w][i], x[w][i + 1]);
+                            if (special) {
+                                const int from = (lane >> 2) + 16 * (w >> 1);
+                                uint32_t v0 = __shfl_sync(0xffffffffu, vis[w & 1], from), v1 = __shfl_sync(0xffffffffu, vis[w & 1], from + 8);
+                                poison |= (v0 & C.bad[wg][w]) != 0;
+                                poison1 |= (v1 & C.bad[wg][w]) != 0;
+                                v0 >>= 2 * (lane & 3);
+                                v1 >>= 2 * (lane & 3);
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    if (!(((i & 2 ? v1 : v0) >> (8 * (i >> 2) + (i & 1))) & 1)) x[w][i] = -INFINITY;
+                            }
+                        }
+                        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int w = 0; w < 4; w++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) y[i & 3] = fmaxf(y[i & 3], x[w][i]);
+                        y[0] = fmaxf(y[0], y[1]);
+                        y[2] = fmaxf(y[2], y[3]);
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) {
+                            y[0] = fmaxf(y[0], __shfl_xor_sync(0xffffffffu, y[0], o));
+                            y[2] = fmaxf(y[2], __shfl_xor_sync(0xffffffffu, y[2], o));
+                        }
+                        m = y[0] * c;
+                        m1 = y[2] * c1;
+                        const float sh0 = TW_SHIFT - (m == -INFINITY ? 0.0f : m), sh1 = TW_SHIFT - (m1 == -INFINITY ? 0.0f : m1);
+                        const uint64_t k2[2] = {pack2(c, c), pack2(c1, c1)}, h2[2] = {pack2(sh0, sh0), pack2(sh1, sh1)};
+                        uint64_t sum2[2] = {0, 0};
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            uint32_t ph[8], pl[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                float p0, p1;
+                                unpack2(fma2(pack2(x[w][2 * i], x[w][2 * i + 1]), k2[i & 1], h2[i & 1]), p0, p1);
+                                p0 = ex2(p0);
+                                p1 = ex2(p1);
+                                sum2[i & 1] = add2(sum2[i & 1], pack2(p0, p1));
+                                cut_h2(p0, p1, ph[i], pl[i]);
+                            }
+                            tmem_st_frag(S + 16 * w, ph);
+                            tmem_st_frag(S + (16u << 16) + 16 * w, pl);
+                        }
+                        unpack2(sum2[0], y[0], y[1]);
+                        unpack2(sum2[1], y[2], y[3]);
+                        sum = y[0] + y[1];
+                        sum1 = y[2] + y[3];
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) {
+                            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                            sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
+                        }
+                        if (poison) sum = NAN;
+                        if (poison1) sum1 = NAN;
+                    } else if (live) {
                         // rolled loops: the two warpgroups' code has to stay in the instruction cache
                         float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
@@ -751,7 +859,11 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     }
                     if (k) ok = __all_sync(0xffffffffu, mbar_wait(&C.x_free[wg], (k - 1) & 1, &g_tree_error));
                     if (!ok) break;
-                    C.x[wg][tid] = make_float2(m, sum);
+                    if (!STACKED) C.x[wg][tid] = make_float2(m, sum);
+                    else if ((lane & 3) == 0) {
+                        C.x[wg][r0] = make_float2(m, sum);
+                        C.x[wg][r1] = make_float2(m1, sum1);
+                    }
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -760,15 +872,15 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             } while (ok && seg_next<TW_ROWS, TW_KEYS>(a, g));
         }
     } else {
-        // ---------------- the running output (thread = row) ----------------
+        // ---------------- the running output (thread = row, or half of it) ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TW_REGS_OUT));
-        const int quad = warp & 3, r = quad * (TM / 4) + lane;
+        const int quad = warp & 3, r = STACKED ? quad * 16 + (lane & 15) : quad * 32 + lane;
         const uint32_t O = tmem + ((uint32_t)(quad * 32) << 16) + 256;
         int n = 0;
         if (N) {
             TreeSeg g = start.g;
             do {
-                const bool valid = lane < TM / 4 && r < g.rows, live = quad * (TM / 4) < g.rows;
+                const bool valid = r < g.rows, live = quad * (STACKED ? 16 : 32) < g.rows;
                 const bool first = g.tile0 == 0;
                 uint64_t acc[64];
 #pragma unroll
@@ -780,7 +892,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     ok = __all_sync(0xffffffffu, mbar_wait(&C.o_full[b], k & 1, &g_tree_error));
                     if (!ok) break;
                     tc_fence_after();
-                    const float2 x = C.x[b][quad * 32 + lane];
+                    const float2 x = C.x[b][r];
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&C.x_free[b]);
                     if (live) {
@@ -813,6 +925,16 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 }
                 if (!ok) break;
                 const bool whole = g.tile0 == 0 && g.tiles == g.s.tiles;
+                // stacked: lane i ends with the sums of the first 64 dims, lane i + 16 with those of the last
+                constexpr int N2 = STACKED ? 32 : 64;
+                const int side = STACKED ? lane >> 4 : 0;
+                if (STACKED && live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const uint64_t other = __shfl_xor_sync(0xffffffffu, side ? acc[i] : acc[i + 32], 16);
+                        acc[i] = add2(side ? acc[i + 32] : acc[i], other);
+                    }
+                }
                 if (valid) {
                     const int R = g.rt * TW_ROWS + r;
                     const size_t part = ((size_t)blockIdx.x * 2 + (first ? 1 : 0)) * a.part_rows + r;
@@ -821,12 +943,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     if (whole) {
                         dst = a.out + ((int64_t)(g.s.s0 + R / a.nrep) * a.hq + g.kvh * a.nrep + R % a.nrep) * HD;
                         f = L != 0.0f ? 1.0f / L : 0.0f;
-                    } else {
+                    } else if (side == 0) {
                         *(float2*)(a.part_ml + part * 2) = make_float2(M, L);
                     }
+                    dst += side * 64;
                     const uint64_t f2 = pack2(f, f);
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
+                    for (int i = 0; i < N2; i += 2) {
                         float4 y;
                         unpack2(fma2(acc[i], f2, 0ull), y.x, y.y);
                         unpack2(fma2(acc[i + 1], f2, 0ull), y.z, y.w);
@@ -1297,7 +1420,7 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
     } else {
         p.G = num_sms();
         p.rows = (int)(rows < TW_ROWS ? rows : TW_ROWS);
-        p.q_rows = (p.rows + 7) / 8 * 8;
+        p.q_rows = p.rows <= TW_STACK ? (p.rows + 15) / 16 * 16 : (p.rows + 7) / 8 * 8;
         p.row_tiles = (int)((rows + TW_ROWS - 1) / TW_ROWS);
         parts = (size_t)2 * p.G;
         p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
@@ -1362,11 +1485,12 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     if (e == cudaSuccess) e = tree_map(&vm, varena, hkv, n_slots, p.few ? 2 : 1);
     if (e != cudaSuccess) return e;
     if (p.few) return p.rows <= 16 ? launch_few<1>(km, vm, a, p, st) : launch_few<2>(km, vm, a, p, st);
-    e = p.rows <= 64 ? DCG_SMEM_ATTR(tree_wide_kernel<64>, TW_SMEM) : DCG_SMEM_ATTR(tree_wide_kernel<128>, TW_SMEM);
+    const bool stacked = p.rows <= TW_STACK;
+    e = stacked ? DCG_SMEM_ATTR(tree_wide_kernel<true>, TW_SMEM) : DCG_SMEM_ATTR(tree_wide_kernel<false>, TW_SMEM);
     if (e != cudaSuccess) return e;
     e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(p.rows <= 64 ? tree_wide_kernel<64> : tree_wide_kernel<128>, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
+    e = launch_pdl(stacked ? tree_wide_kernel<true> : tree_wide_kernel<false>, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
     if (e != cudaSuccess) return e;
     return launch_pdl(tree_combine_kernel, dim3((unsigned)p.G, (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
                       dim3(TC_ROWS * 32), 0, st, a);
