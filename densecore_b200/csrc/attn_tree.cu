@@ -50,7 +50,7 @@ struct TreeArgs {
     float *part_o, *part_ml;     // [2 G][rows][128], [2 G][rows][2]
     struct TreeCut* cuts;        // [G]
     struct TreeStart* begins;    // [G]
-    int64_t* prefix;             // [2][n_seqs + 1]: costs and units before each sequence
+    int64_t* prefix;             // [2][n_seqs]: costs and units before each sequence
     int64_t* bounds;             // [G + 1]: first unit of each CTA
     int G;
     int part_rows;               // rows of the largest row tile
@@ -128,15 +128,18 @@ struct TreeStart {
     TreeSeg g;
 };
 
-// Every CTA's range, by one CTA of THREADS.  An item costs its units and EXTRA for its beginning, its
+// Every CTA's range, by one CTA of THREADS.  An item costs its units and `extra` for its beginning, its
 // masked last units and its output; the ranges cut the summed costs into equal parts, and a cut that
 // falls into an item's extra cost goes to its first unit.  (A CTA inside an item has a unit at least, so
 // an item's CTAs are consecutive.)
-template <int ROWS, int KEYS, int EXTRA, int THREADS>
-__device__ void tree_plan_ranges(const TreeArgs& a) {
-    __shared__ int64_t sums[2][THREADS / 32];
+// Up to THREADS sequences the search runs in shared memory (a chain of global loads cost 3 us).
+template <int ROWS, int KEYS, int THREADS>
+__device__ void tree_plan_ranges(const TreeArgs& a, int extra) {
+    __shared__ int64_t sums[2][THREADS / 32], s_cost[THREADS], s_units[THREADS];
+    __shared__ TreeSeq s_seq[THREADS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t *cost = a.prefix, *units = a.prefix + a.n_seqs + 1;
+    const bool small = a.n_seqs <= THREADS;
+    int64_t *cost = small ? s_cost : a.prefix, *units = small ? s_units : a.prefix + a.n_seqs;
     int64_t run = 0, run_u = 0;
     for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
         const int i = i0 + threadIdx.x;
@@ -145,8 +148,9 @@ __device__ void tree_plan_ranges(const TreeArgs& a) {
             const TreeSeq s = tree_seq<ROWS, KEYS>(a, i, true);
             items = s.tiles ? (int64_t)s.row_tiles * a.hkv : 0;
             u = s.tiles * items;
+            if (small) s_seq[i] = s;
         }
-        const int64_t c = u + EXTRA * items;
+        const int64_t c = u + extra * items;
         int64_t x = c, y = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -180,53 +184,54 @@ __device__ void tree_plan_ranges(const TreeArgs& a) {
     const int64_t V = run;
     const int G = (int)min((int64_t)a.G, V);      // no more ranges than cost: none is empty inside an item
     __syncthreads();
-    for (int c = threadIdx.x; c <= a.G; c += THREADS) {
-        int64_t u0 = run_u;
-        TreeStart b = {};
-        if (c < G) {
-            const int64_t v = sk_begin(c, V, G);
-            int lo = 0, hi = a.n_seqs;             // the last sequence that begins at or before v
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (cost[mid] <= v) lo = mid;
-                else hi = mid;
-            }
-            b.g.seq = lo;
-            b.g.s = tree_seq<ROWS, KEYS>(a, lo, false);
-            b.g.next = seq_or_none<ROWS, KEYS>(a, lo + 1);
-            const int off = (int)(v - cost[lo]), each = b.g.s.tiles + EXTRA, item = off / each;
-            b.g.tile0 = max(0, off - item * each - EXTRA);
-            b.g.kvh = item / b.g.s.row_tiles;
-            b.g.rt = item - b.g.kvh * b.g.s.row_tiles;
-            u0 = units[lo] + (int64_t)item * b.g.s.tiles + b.g.tile0;
+    auto seq_at = [&](int i) { return i >= a.n_seqs ? TreeSeq{0, 0, 0, 0, 0} : small ? s_seq[i] : tree_seq<ROWS, KEYS>(a, i, false); };
+    // range c's first unit; where that lies
+    auto begin = [&](int c, TreeSeg& g) -> int64_t {
+        if (c >= G) return run_u;
+        const int64_t v = sk_begin(c, V, G);
+        int lo = 0, hi = a.n_seqs;                 // the last sequence that begins at or before v
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (cost[mid] <= v) lo = mid;
+            else hi = mid;
         }
-        a.bounds[c] = b.u0 = u0;
+        g.seq = lo;
+        g.s = seq_at(lo);
+        const int off = (int)(v - cost[lo]), each = g.s.tiles + extra, item = off / each;
+        g.tile0 = max(0, off - item * each - extra);
+        g.kvh = item / g.s.row_tiles;
+        g.rt = item - g.kvh * g.s.row_tiles;
+        return units[lo] + (int64_t)item * g.s.tiles + g.tile0;
+    };
+    for (int c = threadIdx.x; c <= a.G; c += THREADS) {
+        TreeStart b = {};
+        a.bounds[c] = b.u0 = begin(c, b.g);
         if (c < a.G) {
+            TreeSeg end;
+            b.N = (int)(begin(c + 1, end) - b.u0);
+            b.g.left = b.N;
+            if (b.N) {
+                b.g.next = seq_at(b.g.seq + 1);
+                seg_shape<ROWS>(a, b.g);
+            }
             a.begins[c] = b;
             a.cuts[c].rows = 0;
         }
     }
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.G; c += THREADS) {
-        TreeStart& b = a.begins[c];
-        b.N = (int)(a.bounds[c + 1] - a.bounds[c]);
-        b.g.left = b.N;
-        if (b.N) seg_shape<ROWS>(a, b.g);
-    }
 }
 
-// mask bits of keys g0 .. g0 + 31 (as positions) for drafted token `tok` (row of q): history, then draft
-__device__ __forceinline__ uint32_t tree_bits(const TreeArgs& a, const TreeSeq& s, int tok, int g0) {
+// mask bits of keys g0 .. g0 + 31 (as positions) for the drafted token of mask row `m`, whose first word
+// is m0: history, then draft
+__device__ __forceinline__ uint32_t tree_bits(const TreeArgs& a, const TreeSeq& s, const uint64_t* m, uint64_t m0, int g0) {
     const int hist = s.L - s.ns, t0 = g0 - hist;
     if (t0 <= -32) return 0xFFFFFFFFu;
     if (g0 >= s.L) return 0u;
-    const uint64_t* m = (const uint64_t*)a.mask + (int64_t)tok * a.words;
     uint32_t v;
     if (t0 < 0) {
-        v = (uint32_t)(m[0] << -t0) | ((1u << -t0) - 1);
+        v = (uint32_t)(m0 << -t0) | ((1u << -t0) - 1);
     } else {
         const int w = t0 >> 6, b = t0 & 63;
-        v = (uint32_t)(m[w] >> b);
+        v = (uint32_t)((w ? m[w] : m0) >> b);
         if (b > 32 && w + 1 < a.words) v |= (uint32_t)(m[w + 1] << (64 - b));
     }
     const int n = s.L - g0;
@@ -279,7 +284,7 @@ constexpr int TW_OFF_RING = 2 * TW_BUF;           // Q hi, Q lo first
 constexpr int TW_OFF_CTRL = TW_OFF_RING + TW_RING * TW_BUF;
 constexpr int TW_CTRL = 3072;
 constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // all of it: 227 KB
-constexpr int TW_EXTRA = 2;                       // an item's fixed cost in units (7,000 cycles against 3,300 a unit)
+constexpr int TW_EXTRA = 4, TW_EXTRA_STACKED = 2; // an item's fixed cost in units (5.7 us against 1.4 us a unit; 2.4 and 1.1)
 constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^8: the small ones stay above fp16's least
 // registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128
 constexpr int TW_REGS_CTRL = 56, TW_REGS_SOFT = 128, TW_REGS_OUT = 200;
@@ -289,7 +294,7 @@ struct TwCtrl {
     uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_full[2], o_free[2], x_free[2], cleaned[2];
     uint64_t q_full[2], q_empty[2][2], mma_end[2], s_sent[2];   // q_empty: by MMA warp and buffer
     uint32_t tmem;
-    uint32_t bad[2][4];                           // per buffer: keys of its tile whose V is not finite
+    uint32_t bad[2][3][4];                        // per buffer, special tiles in turn: keys whose V is not finite
     float2 x[2][TW_ROWS];                         // a tile's row max and sum of p
 };
 static_assert(sizeof(TwCtrl) <= TW_CTRL, "control block");
@@ -370,6 +375,9 @@ __device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&v)
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory");
+}
 // ring position of the K and V tile of the range's n-th unit of N: K0 K1 V0 K2 V1 ... K(N-1) V(N-2) V(N-1)
 __device__ __forceinline__ uint32_t tw_k(int n) { return n ? 2 * n - 1 : 0; }
 __device__ __forceinline__ uint32_t tw_v(int n, int N) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; }
@@ -394,43 +402,69 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
 
 // Q as fp16 halves in the tiles that tree_wide_kernel copies: [hi, lo][half of 64 dims][q_rows][128 B], or
 // stacked [half of 64 dims][16 rows hi, the same lo, the next 16 hi, ...][128 B];
-// 128-byte swizzle, each row scaled by a power of two (its sign the scale's).  A warp is a row: CTA
-// (drafted token, sequence), heads in turn.  One CTA more plans the ranges.
-constexpr int TQ_WARPS = 8;
+// 128-byte swizzle, each row scaled by a power of two (its sign the scale's).  CTA (TQ_ROWS of a
+// sequence's rows, which lie one behind the other; sequence), 8 lanes a row.  One CTA more plans the ranges.
+constexpr int TQ_WARPS = 8, TQ_ROWS = 64;
 __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a) {
+    __shared__ __align__(128) float rows[TQ_ROWS * HD];
+    __shared__ uint64_t bar;
     pdl_wait();
     pdl_trigger();
     if (blockIdx.y == 0) {                        // first in the launch order
-        if (blockIdx.x == 0) tree_plan_ranges<TW_ROWS, TW_KEYS, TW_EXTRA, TQ_WARPS * 32>(a);
+        if (blockIdx.x == 0) tree_plan_ranges<TW_ROWS, TW_KEYS, TQ_WARPS * 32>(a, a.q_rows <= TW_STACK ? TW_EXTRA_STACKED : TW_EXTRA);
         return;
     }
     const int seq = blockIdx.y - 1;
     const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, seq, false);
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    if (t >= s.ns) return;
+    const int x0 = blockIdx.x * TQ_ROWS, n = min(TQ_ROWS, s.ns * a.hq - x0), lane = threadIdx.x & 31;
+    if (n <= 0) return;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar, 1);
+        fence_mbar_init();
+        mbar_arrive_expect_tx(&bar, (uint32_t)n * HD * 4);
+        bulk_g2s(rows, a.q + ((int64_t)s.s0 * a.hq + x0) * HD, (uint32_t)n * HD * 4, &bar);
+    }
+    __syncthreads();
     const bool stacked = a.q_rows <= TW_STACK;
     const int dims_half = a.q_rows * (stacked ? 256 : 128), to_lo = stacked ? 16 * 128 : a.q_rows * 256;
-    const float* q = a.q + (int64_t)(s.s0 + t) * a.hq * HD + 4 * lane;
-#pragma unroll 4
-    for (int h = threadIdx.x >> 5; h < a.hq; h += TQ_WARPS) {
-        const float4 x = *(const float4*)(q + h * HD);
+    if (!mbar_wait(&bar, 0, &g_tree_error)) return;
+#pragma unroll 1
+    for (int i0 = (threadIdx.x >> 5) * 4; i0 < n; i0 += TQ_WARPS * 4) {
+        const int i = min(i0 + (lane >> 3), n - 1), sub = lane & 7;   // (the last row by several alike)
+        float x[2][8], m = 0.0f;                  // dims 8 sub .. +7 of both halves
+#pragma unroll
+        for (int d = 0; d < 2; d++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const float4 y = *(const float4*)(rows + i * HD + 64 * d + 8 * sub + 4 * c);
+                x[d][4 * c] = y.x;
+                x[d][4 * c + 1] = y.y;
+                x[d][4 * c + 2] = y.z;
+                x[d][4 * c + 3] = y.w;
+                m = fmaxf(fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
+            }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int t = (x0 + i) / a.hq, h = x0 + i - t * a.hq;
         const int kvh = h / a.nrep, R = t * a.nrep + h - kvh * a.nrep, rt = R / TW_ROWS, r = R - rt * TW_ROWS;
         const int64_t tile = ((int64_t)seq * a.row_tiles + rt) * a.hkv + kvh;
-        const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
         // exponent of the row's largest value (0 rows and subnormal ones: the least)
-        int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(m)) >> 23) - 127;
+        int e = (int)(__float_as_uint(m) >> 23) - 127;
         e = e < -100 ? -100 : e > 120 ? 120 : e;
         const float f = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);   // 2^-e
-        uint32_t h0, l0, h1, l1;
-        cut_h2(x.x * f, x.y * f, h0, l0);
-        cut_h2(x.z * f, x.w * f, h1, l1);
-        // dims 4 lane .. +3: 8 bytes of 16-byte chunk (lane / 2) & 7 of its half
         const int at = stacked ? 2 * r - (r & 15) : r;
-        uint8_t* to = a.q_tiles + tile * a.q_rows * 512 + (lane >> 4) * dims_half + at * 128 +
-                      ((((lane >> 1) & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
-        *(uint2*)to = make_uint2(h0, h1);
-        *(uint2*)(to + to_lo) = make_uint2(l0, l1);
-        if (lane == 0) a.q_exps[tile * a.q_rows + r] = (int8_t)e;
+        uint8_t* to = a.q_tiles + tile * a.q_rows * 512 + at * 128 + ((sub ^ (r & 7)) << 4);
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            uint4 hi, lo;
+            cut_h2(x[d][0] * f, x[d][1] * f, hi.x, lo.x);
+            cut_h2(x[d][2] * f, x[d][3] * f, hi.y, lo.y);
+            cut_h2(x[d][4] * f, x[d][5] * f, hi.z, lo.z);
+            cut_h2(x[d][6] * f, x[d][7] * f, hi.w, lo.w);
+            *(uint4*)(to + d * dims_half) = hi;
+            *(uint4*)(to + d * dims_half + to_lo) = lo;
+        }
+        if (sub == 0) a.q_exps[tile * a.q_rows + r] = (int8_t)e;
     }
 }
 
@@ -468,11 +502,14 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         }
         fence_mbar_init();
     }
+    if (threadIdx.x < 24) (&C.bad[0][0][0])[threadIdx.x] = 0;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&C.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (threadIdx.x == 0 || threadIdx.x == 96) prefetch_tensormap(threadIdx.x ? &vmap : &kmap);
     pdl_wait();
+    pdl_trigger();                                // tree_combine_kernel's CTAs wait where this one's have ended
     const TreeStart& start = a.begins[blockIdx.x];
     const int N = start.N;
     tc_fence_before();
@@ -654,7 +691,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             do {
                 const bool valid = r < g.rows, live = quad * (STACKED ? 16 : 32) < g.rows;
                 const int hist = g.s.L - g.s.ns;
-                const int tok = g.s.s0 + (valid ? (g.rt * TW_ROWS + r) / a.nrep : 0);
+                const uint64_t* mask = (const uint64_t*)a.mask + (int64_t)(g.s.s0 + (valid ? (g.rt * TW_ROWS + r) / a.nrep : 0)) * a.words;
+                const uint64_t mask0 = *mask;
                 // c > 0 (the scale's sign is in Q), and not 0: c x -inf has to stay -inf
                 const int64_t tile = ((int64_t)g.seq * a.row_tiles + g.rt) * a.hkv + g.kvh;
                 auto scale = [&](int row) {
@@ -677,25 +715,28 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         const uint32_t lv = tw_v(n, N);
                         ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (lv / TW_RING) & 1, &g_tree_error));
                         if (!ok) break;
-                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + tid * 128;   // a key per thread
-                        const int key = kb + tid;
-                        bool odd = false;
-                        if (key >= hist && key < g.s.L) {
+                        // (pages past the sequence's last came as zeros).  A chunk of 16 bytes per lane, two keys
+                        // at a time, the warps in turn.
+                        uint32_t* bad = C.bad[wg][cleans % 3];
+                        if (tid < 4) C.bad[wg][(cleans + 1) % 3][tid] = 0;   // the last but one's: all have read it
+                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + ((lane >> 3) & 1) * TW_HALF + (lane & 7) * 16;
+                        const int end = min((g.s.L + KVB - 1) / KVB * KVB - kb, TW_KEYS);
 #pragma unroll 4
-                            for (int x = 0; x < 16; x++) {   // chunks in an order that spreads the lanes over the banks
-                                const uint4 w = *(const uint4*)(v + (x >> 3) * TW_HALF + ((x + lane) & 7) * 16);
+                        for (int i = max(hist - kb, 0) / 2 + quad; 2 * i < end; i += 4) {
+                            const int key = 2 * i + (lane >> 4);
+                            uint4* chunk = (uint4*)(v + key * 128);
+                            bool odd = false;
+                            if (kb + key >= hist && kb + key < g.s.L) {
+                                const uint4 w = *chunk;
                                 const uint32_t y[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    odd |= (y[i] & 0x7C00u) == 0x7C00u || (y[i] & 0x7C000000u) == 0x7C000000u;
+                                for (int e = 0; e < 4; e++)
+                                    odd |= (y[e] & 0x7C00u) == 0x7C00u || (y[e] & 0x7C000000u) == 0x7C000000u;
                             }
+                            const bool any = (__ballot_sync(0xffffffffu, odd) >> (lane & 16)) & 0xFFFFu;
+                            if (any || kb + key >= g.s.L) *chunk = make_uint4(0, 0, 0, 0);
+                            if (any && (lane & 15) == 0) atomicOr(&bad[key >> 5], 1u << (key & 31));
                         }
-                        if (odd || key >= g.s.L) {
-#pragma unroll 4
-                            for (int x = 0; x < 16; x++) *(uint4*)(v + (x >> 3) * TW_HALF + ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-                        if (lane == 0) C.bad[wg][quad] = odds;
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&C.cleaned[wg]);
@@ -704,8 +745,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         if (live && !STACKED) {
 #pragma unroll 1
                             for (int w = 0; w < 4; w++) {
-                                const uint32_t vis = valid ? tree_bits(a, g.s, tok, kb + 32 * w) : 0u;   // keys this row sees
-                                poison |= (vis & C.bad[wg][w]) != 0;
+                                const uint32_t vis = valid ? tree_bits(a, g.s, mask, mask0, kb + 32 * w) : 0u;   // keys this row sees
+                                poison |= (vis & C.bad[wg][(cleans + 2) % 3][w]) != 0;
                                 uint32_t s[32];
                                 tmem_ld32(S + 32 * w, s);
                                 tmem_wait_ld();
@@ -722,44 +763,47 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         if (special) {
 #pragma unroll 1
                             for (int w = 0; w < 2; w++) {
-                                const uint32_t v = valid ? tree_bits(a, g.s, tok, kb + 64 * (lane >> 4) + 32 * w) : 0u;
+                                const uint32_t v = valid ? tree_bits(a, g.s, mask, mask0, kb + 64 * (lane >> 4) + 32 * w) : 0u;
                                 if (w) vis[1] = v;
                                 else vis[0] = v;
                             }
                         }
                         bool poison1 = false;
-                        float x[4][16];                    // the scores, then p
-                        uint32_t hi[2][16], lo[2][16];     // one is loaded while the other is worked on
-                        tmem_ld_frag(S, hi[0]);
-                        tmem_ld_frag(S + (16u << 16), lo[0]);
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
+                        // rolled loops: the code of all the warps has to stay in the instruction cache
+                        uint32_t hi[16], lo[16];           // the next 32 scores, loaded while x is worked on
+                        float x[16];
+                        tmem_ld_frag(S, hi);
+                        tmem_ld_frag(S + (16u << 16), lo);
+                        auto scores = [&](int w, bool more) {
                             tmem_wait_ld();
-                            if (w < 3) {
-                                tmem_ld_frag(S + 32 * (w + 1), hi[(w + 1) & 1]);
-                                tmem_ld_frag(S + (16u << 16) + 32 * (w + 1), lo[(w + 1) & 1]);
-                            }
 #pragma unroll
                             for (int i = 0; i < 16; i += 2)
-                                unpack2(add2(pack2(__uint_as_float(hi[w & 1][i]), __uint_as_float(hi[w & 1][i + 1])),
-                                             pack2(__uint_as_float(lo[w & 1][i]), __uint_as_float(lo[w & 1][i + 1]))), x[w][i], x[w][i + 1]);
+                                unpack2(add2(pack2(__uint_as_float(hi[i]), __uint_as_float(hi[i + 1])),
+                                             pack2(__uint_as_float(lo[i]), __uint_as_float(lo[i + 1]))), x[i], x[i + 1]);
+                            if (more) {
+                                tmem_ld_frag(S + 32 * ((w + 1) & 3), hi);
+                                tmem_ld_frag(S + (16u << 16) + 32 * ((w + 1) & 3), lo);
+                            }
                             if (special) {
                                 const int from = (lane >> 2) + 16 * (w >> 1);
-                                uint32_t v0 = __shfl_sync(0xffffffffu, vis[w & 1], from), v1 = __shfl_sync(0xffffffffu, vis[w & 1], from + 8);
-                                poison |= (v0 & C.bad[wg][w]) != 0;
-                                poison1 |= (v1 & C.bad[wg][w]) != 0;
+                                const uint32_t v = w & 1 ? vis[1] : vis[0];
+                                uint32_t v0 = __shfl_sync(0xffffffffu, v, from), v1 = __shfl_sync(0xffffffffu, v, from + 8);
+                                poison |= (v0 & C.bad[wg][(cleans + 2) % 3][w]) != 0;
+                                poison1 |= (v1 & C.bad[wg][(cleans + 2) % 3][w]) != 0;
                                 v0 >>= 2 * (lane & 3);
                                 v1 >>= 2 * (lane & 3);
 #pragma unroll
                                 for (int i = 0; i < 16; i++)
-                                    if (!(((i & 2 ? v1 : v0) >> (8 * (i >> 2) + (i & 1))) & 1)) x[w][i] = -INFINITY;
+                                    if (!(((i & 2 ? v1 : v0) >> (8 * (i >> 2) + (i & 1))) & 1)) x[i] = -INFINITY;
                             }
-                        }
+                        };
                         float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                        for (int w = 0; w < 4; w++) {
+                            scores(w, true);
 #pragma unroll
-                        for (int w = 0; w < 4; w++)
-#pragma unroll
-                            for (int i = 0; i < 16; i++) y[i & 3] = fmaxf(y[i & 3], x[w][i]);
+                            for (int i = 0; i < 16; i++) y[i & 3] = fmaxf(y[i & 3], x[i]);
+                        }
                         y[0] = fmaxf(y[0], y[1]);
                         y[2] = fmaxf(y[2], y[3]);
 #pragma unroll
@@ -772,13 +816,14 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         const float sh0 = TW_SHIFT - (m == -INFINITY ? 0.0f : m), sh1 = TW_SHIFT - (m1 == -INFINITY ? 0.0f : m1);
                         const uint64_t k2[2] = {pack2(c, c), pack2(c1, c1)}, h2[2] = {pack2(sh0, sh0), pack2(sh1, sh1)};
                         uint64_t sum2[2] = {0, 0};
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
+#pragma unroll 1
+                        for (int w = 0; w < 4; w++) {      // P's columns lie behind the scores still to be read
+                            scores(w, w < 3);
                             uint32_t ph[8], pl[8];
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 float p0, p1;
-                                unpack2(fma2(pack2(x[w][2 * i], x[w][2 * i + 1]), k2[i & 1], h2[i & 1]), p0, p1);
+                                unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), k2[i & 1], h2[i & 1]), p0, p1);
                                 p0 = ex2(p0);
                                 p1 = ex2(p1);
                                 sum2[i & 1] = add2(sum2[i & 1], pack2(p0, p1));
@@ -976,7 +1021,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
-    pdl_trigger();
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1187,7 +1231,8 @@ __global__ void __launch_bounds__((TF_CONS + 1) * 32, 2) tree_few_kernel(
                 for (int t = 0; t < MT; t++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        vis[t][h] = tree_bits(a, s, tok[t][h], kb);
+                        const uint64_t* m = (const uint64_t*)a.mask + (int64_t)tok[t][h] * a.words;
+                        vis[t][h] = tree_bits(a, s, m, *m, kb);
                         if (vis[t][h] & bad) poison |= 1u << (2 * t + h);
                     }
             }
@@ -1314,15 +1359,26 @@ __global__ void __launch_bounds__((TF_CONS + 1) * 32, 2) tree_few_kernel(
 
 // The parts of a row, 32 at a time: m and l a lane each, then the outputs with all loads apart from the
 // sums (a lane 4 dims).  part(x): index of the x-th part.
-template <class F>
+// LOADS outputs are under way at a time: 16 where an item has many parts, 4 (and twice the warps) where few.
+template <int LOADS, class F>
 __device__ __forceinline__ void tree_join(const TreeArgs& a, int parts, F part, float* dst) {
     const int lane = threadIdx.x & 31;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int x0 = 0; x0 < parts; x0 += 32) {
-        const int64_t p = x0 + lane < parts ? part(x0 + lane) : -1;
+        const int n = min(32, parts - x0);
+        const int p = lane < n ? (int)part(x0 + lane) : 0;
+        float4 z[LOADS];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int q = __shfl_sync(0xffffffffu, p, i0 + i);
+                if (i0 + i < n) z[i] = *(const float4*)(a.part_o + (int64_t)q * HD + 4 * lane);
+            }
+        };
+        load(0);                                   // beside the maxima
         float2 y = make_float2(-INFINITY, 0.0f);
-        if (p >= 0) y = *(const float2*)(a.part_ml + p * 2);
+        if (lane < n) y = *(const float2*)(a.part_ml + (int64_t)p * 2);
         float m = fmaxf(M, y.x);
 #pragma unroll
         for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
@@ -1336,18 +1392,19 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, int parts, F part, 
         o.y *= f;
         o.z *= f;
         o.w *= f;
-        const int n = min(32, parts - x0);
-        const uint32_t used = __ballot_sync(0xffffffffu, y.y != 0.0f);   // others left nothing to read
-#pragma unroll 8
-        for (int i = 0; i < n; i++) {
-            if (!((used >> i) & 1)) continue;
-            const float v = __shfl_sync(0xffffffffu, w, i);
-            const int64_t q = __shfl_sync(0xffffffffu, p, i);
-            const float4 z = *(const float4*)(a.part_o + q * HD + 4 * lane);
-            o.x += z.x * v;
-            o.y += z.y * v;
-            o.z += z.z * v;
-            o.w += z.w * v;
+        const uint32_t used = __ballot_sync(0xffffffffu, y.y != 0.0f);   // the others' outputs were not written
+        for (int i0 = 0; i0 < n; i0 += LOADS) {
+            if (i0) load(i0);
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const float v = __shfl_sync(0xffffffffu, w, i0 + i);
+                if ((used >> (i0 + i)) & 1) {
+                    o.x += z[i].x * v;
+                    o.y += z[i].y * v;
+                    o.z += z[i].z * v;
+                    o.w += z[i].w * v;
+                }
+            }
         }
     }
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
@@ -1356,17 +1413,19 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, int parts, F part, 
 
 // tree_few_kernel's splits: a warp per row, CTA (sequence and kv head, 8 rows)
 constexpr int TC_ROWS = 8;
+template <int LOADS>
 __global__ void __launch_bounds__(TC_ROWS * 32) tree_join_kernel(const TreeArgs a, int splits) {
     pdl_wait();
     pdl_trigger();
     const int seq = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, r = blockIdx.y * TC_ROWS + (threadIdx.x >> 5);
     const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, seq, false);
     if (r >= s.ns * a.nrep) return;
-    tree_join(a, splits, [&](int x) { return ((int64_t)blockIdx.x * splits + x) * a.part_rows + r; },
+    tree_join<LOADS>(a, splits, [&](int x) { return ((int64_t)blockIdx.x * splits + x) * a.part_rows + r; },
               a.out + ((int64_t)(s.s0 + r / a.nrep) * a.hq + kvh * a.nrep + r % a.nrep) * HD);
 }
 
 // tree_wide_kernel's items that several CTAs worked on, in CTA order: CTA (CTA that began an item, 8 rows)
+template <int LOADS>
 __global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeArgs a) {
     pdl_wait();
     pdl_trigger();
@@ -1374,7 +1433,7 @@ __global__ void __launch_bounds__(TC_ROWS * 32) tree_combine_kernel(const TreeAr
     const TreeCut cut = a.cuts[c];
     if (r >= cut.rows) return;
     const int R = cut.row0 + r;
-    tree_join(a, cut.parts,
+    tree_join<LOADS>(a, cut.parts,
               [&](int x) { return ((int64_t)(c + x) * 2 + (x == 0 ? 1 : 0)) * a.part_rows + r; },
               a.out + ((int64_t)(cut.s0 + R / a.nrep) * a.hq + cut.kvh * a.nrep + R % a.nrep) * HD);
 }
@@ -1425,7 +1484,7 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
         parts = (size_t)2 * p.G;
         p.cut_bytes = align256((size_t)p.G * sizeof(TreeCut));
         p.start_bytes = align256((size_t)p.G * sizeof(TreeStart));
-        p.prefix_bytes = align256((size_t)(n_seqs + 1) * 2 * 8);
+        p.prefix_bytes = align256((size_t)n_seqs * 2 * 8);
         p.bound_bytes = align256((size_t)(p.G + 1) * 8);
         const size_t q = (size_t)n_seqs * p.row_tiles * hkv * p.q_rows;
         p.q_bytes = align256(q * 512);
@@ -1448,7 +1507,7 @@ static cudaError_t launch_few(const CUtensorMap& km, const CUtensorMap& vm, cons
     e = launch_pdl(tree_few_kernel<MT>, dim3((unsigned)(a.n_seqs * a.hkv), (unsigned)p.splits), dim3((TF_CONS + 1) * 32), smem,
                    st, km, vm, a, p.bps, p.splits);
     if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_pdl(tree_join_kernel, dim3((unsigned)(a.n_seqs * a.hkv), (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
+    return launch_pdl(p.splits > 8 ? tree_join_kernel<16> : tree_join_kernel<4>, dim3((unsigned)(a.n_seqs * a.hkv), (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
                       dim3(TC_ROWS * 32), 0, st, a, p.splits);
 }
 
@@ -1488,11 +1547,12 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     const bool stacked = p.rows <= TW_STACK;
     e = stacked ? DCG_SMEM_ATTR(tree_wide_kernel<true>, TW_SMEM) : DCG_SMEM_ATTR(tree_wide_kernel<false>, TW_SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(tree_q_kernel, dim3((unsigned)max_seq_tokens, (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
+    e = launch_pdl(tree_q_kernel, dim3((unsigned)(((int64_t)max_seq_tokens * hq + TQ_ROWS - 1) / TQ_ROWS), (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(stacked ? tree_wide_kernel<true> : tree_wide_kernel<false>, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
     if (e != cudaSuccess) return e;
-    return launch_pdl(tree_combine_kernel, dim3((unsigned)p.G, (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
+    const int64_t items = (int64_t)n_seqs * p.row_tiles * hkv;   // at most
+    return launch_pdl(items * 8 <= p.G ? tree_combine_kernel<16> : tree_combine_kernel<4>, dim3((unsigned)p.G, (unsigned)((p.rows + TC_ROWS - 1) / TC_ROWS)),
                       dim3(TC_ROWS * 32), 0, st, a);
 }
 
