@@ -286,13 +286,15 @@ constexpr int TW_CTRL = 3072;
 constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // all of it: 227 KB
 constexpr int TW_EXTRA = 4, TW_EXTRA_STACKED = 2; // an item's fixed cost in units (5.7 us against 1.4 us a unit; 2.4 and 1.1)
 constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^8: the small ones stay above fp16's least
-// registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128
-constexpr int TW_REGS_CTRL = 56, TW_REGS_SOFT = 128, TW_REGS_OUT = 200;
-static_assert(TW_REGS_CTRL + 2 * TW_REGS_SOFT + TW_REGS_OUT <= 512, "register split");
+// registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128,
+// as few spills as any split has
+constexpr int tw_regs_ctrl(bool stacked) { return stacked ? 56 : 80; }
+constexpr int TW_REGS_SOFT = 128;
+constexpr int tw_regs_out(bool stacked) { return 512 - 2 * TW_REGS_SOFT - tw_regs_ctrl(stacked); }
 
 struct TwCtrl {
     uint64_t full[TW_RING], empty[TW_RING], s_full[2], p_full[2], o_full[2], o_free[2], x_free[2], cleaned[2];
-    uint64_t q_full[2], q_empty[2][2], mma_end[2], s_sent[2];   // q_empty: by MMA warp and buffer
+    uint64_t q_full[2], q_empty[2][2], mma_end[2];   // q_empty: by MMA warp and buffer
     uint32_t tmem;
     uint32_t bad[2][3][4];                        // per buffer, special tiles in turn: keys whose V is not finite
     float2 x[2][TW_ROWS];                         // a tile's row max and sum of p
@@ -498,7 +500,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             mbar_init(&C.q_empty[0][b], 1);
             mbar_init(&C.q_empty[1][b], 1);
             mbar_init(&C.mma_end[b], 1);
-            mbar_init(&C.s_sent[b], 1);
         }
         fence_mbar_init();
     }
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     constexpr int q_bufs = STACKED ? 2 : 1;       // as many as there is room for
     const int q_bytes = a.q_rows * 512;
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TW_REGS_CTRL));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(tw_regs_ctrl(STACKED)));
         if (N == 0) {
         } else if (warp == 0 || warp == 3) {
             // ---------------- Q and K tiles (warp 0), V tiles (warp 3) ----------------
@@ -626,7 +627,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                             }
                         }
                     }
-                    mbar_arrive(&C.s_sent[b]);
                     tc_commit(&C.s_full[b]);
                     tc_commit(&C.empty[slot]);
                     if (n + 2 >= end) tc_commit(&q_empty[qb]);
@@ -636,8 +636,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             if (b < N) issue_s(b, false);
             for (int n = b; n < N && ok; n += 2) {  // O of unit n, then S of unit n + 2 into the same buffer
                 const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
-                // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit issued, others P.  (The third keeps
-                // the two streams apart: side by side, both softmaxes leave the tensor core idle.)
+                // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit, others P.  (The third keeps the
+                // two streams apart, and the tiles' order: a slot of the ring holds K and V in turn, and a producer
+                // that came a fill too early would not see it by the parity.)
                 uint64_t* bar = &C.p_full[b];
                 uint32_t parity = k & 1;
                 bool wait = true;
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     parity = (k - 1) & 1;
                     wait = k > 0;
                 } else if (lane == 2) {
-                    bar = &C.s_sent[b ^ 1];
+                    bar = &C.s_full[b ^ 1];
                     parity = ((uint32_t)(n + 1) >> 1) & 1;
                     wait = n + 1 < N;
                 }
@@ -918,7 +919,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         }
     } else {
         // ---------------- the running output (thread = row, or half of it) ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TW_REGS_OUT));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(tw_regs_out(STACKED)));
         const int quad = warp & 3, r = STACKED ? quad * 16 + (lane & 15) : quad * 32 + lane;
         const uint32_t O = tmem + ((uint32_t)(quad * 32) << 16) + 256;
         int n = 0;
@@ -1456,24 +1457,30 @@ static cudaError_t tree_map(CUtensorMap* map, const void* arena, int hkv, int64_
 }
 
 struct TreePlan {
-    bool few;                   // up to TF_ROWS rows per kv head: tree_few_kernel
+    bool few;                   // tree_few_kernel
     int rows;                   // of a part
     int splits, bps;            // few: splits of a sequence's blocks, blocks of one
     int G, q_rows, row_tiles;   // wide
     size_t o_bytes, ml_bytes, cut_bytes, start_bytes, prefix_bytes, bound_bytes, q_bytes, e_bytes;
 };
-constexpr int TF_ROWS = 32;
+constexpr int TF_MIN = 6;
 static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int max_ctx) {
     TreePlan p = {};
     const int64_t rows = (int64_t)max_seq_tokens * (hq / hkv);
-    p.few = rows <= TF_ROWS;
+    // few: a CTA for TF_MIN blocks at least, and all CTAs at once (two per SM).  Times in us of 1 / 4 / 16
+    // sequences with 8 kv heads and 16 rows, this plan against decode attention's two waves: 1,000
+    // tokens 7.6 / 10.3 / 19 against 14 / 14 / 30.
+    const int nblk = max_ctx > KVB ? (max_ctx - 1) / KVB + 1 : 1;
+    const int64_t fit = 2 * (int64_t)num_sms() / ((int64_t)n_seqs * hkv);
+    p.splits = (int)min((int64_t)(nblk - 1) / TF_MIN + 1, max(fit, (int64_t)1));
+    p.bps = (nblk - 1) / p.splits + 1;
+    p.splits = (nblk - 1) / p.bps + 1;
+    // Up to 16 rows few wins while its CTAs have up to 96 blocks, or as many each: 64 sequences of up to 1,024
+    // tokens 45 against wide's 53 us, of up to 4,096 140 against 117, one of 100,003 71 against 80.  Beyond 16
+    // rows, up to 32 blocks: one sequence of 4,000 tokens 16.3 against 17.5, of 20,000 33.2 against 31.8.
+    p.few = rows <= 16 ? p.bps <= 96 || n_seqs == 1 : rows <= 32 && p.bps <= 32;
     size_t parts;
     if (p.few) {
-        attn_plan(n_seqs, hkv, max_ctx, &p.splits, &p.bps);   // as many CTAs as decode attention
-        if (p.splits > 32768) {                               // a grid's second dimension
-            p.bps = (p.bps * p.splits + 32767) / 32768;
-            p.splits = 32768;
-        }
         p.rows = (int)rows;
         parts = p.splits > 1 ? (size_t)n_seqs * hkv * p.splits : 0;
     } else {
