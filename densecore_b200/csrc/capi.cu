@@ -350,7 +350,8 @@ int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena
     if (max_ctx < 0 || max_ctx > 16 * max_blocks_per_seq) return fail(DCG_EINVAL, "max_ctx exceeds the block table");
     if (mask_words <= 0 || max_seq_tokens > (int64_t)64 * mask_words)
         return fail(DCG_EINVAL, "tree_mask has too few words for max_seq_tokens");
-    if (n_seqs > 65535 || hq > 65535) return fail(DCG_EINVAL, "n_seqs and hq must be <= 65535");
+    if (n_seqs >= 65535 || hq >= 65535 || (int64_t)n_seqs * hkv > INT32_MAX)
+        return fail(DCG_EINVAL, "n_seqs and hq must be < 65535, n_seqs * hkv below 2^31");
     // rows, and the key tiles of a sequence's items, are counted in 32 bits
     if ((int64_t)max_seq_tokens * hq > INT32_MAX / 128 || ((int64_t)max_seq_tokens * hq / 16 + hkv) * (max_ctx / 16 + 1) > INT32_MAX)
         return fail(DCG_EINVAL, "max_seq_tokens * hq * max_ctx too large");

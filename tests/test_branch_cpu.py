@@ -28,6 +28,12 @@ def test_tree_refuses(kw, word):
     assert word in _lib.load().dcg_last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(n_seqs=65535), dict(hq=65535, hkv=1), dict(n_seqs=65534, hq=40000, hkv=40000)])
+def test_tree_refuses_what_a_grid_cannot_hold(kw):
+    assert tree(**kw) == EINVAL
+    assert b"65535" in _lib.load().dcg_last_error()
+
+
 def test_tree_without_work_is_ok():
     assert tree(n_seqs=0) == 0 and tree(n_tok=0) == 0 and tree(max_tok=0) == 0
 

@@ -117,6 +117,35 @@ def test_tree_many_sequences(ops):
     check_tree(ops, ns, ctx, 4, 2, n_layer=1, layer=0)
 
 
+@pytest.mark.parametrize("most", [12, 20])
+def test_tree_many_sequences_of_many_rows(ops, most):
+    """More sequences than the planning CTA has threads, some of them empty: up to 48 and 80 rows per kv head."""
+    rng = np.random.default_rng(most)
+    ns = rng.integers(0, most + 1, 300).tolist()
+    ns[0] = ns[299] = most
+    ctx = [n + int(c) for n, c in zip(ns, rng.integers(0, 40, 300))]
+    check_tree(ops, ns, ctx, 8, 2, n_layer=1, layer=0)
+
+
+@pytest.mark.parametrize("hq,hkv,most", [(32, 8, 16), (48, 8, 16), (16, 8, 8), (16, 8, 2)])
+def test_tree_ragged_batch(ops, hq, hkv, most):
+    """Items that begin and end within one CTA's range, several to a range."""
+    rng = np.random.default_rng(hq + most)
+    ns = rng.integers(1, most + 1, 24).tolist()
+    ns[0] = most
+    ctx = [n + int(c) for n, c in zip(ns, rng.integers(0, 600, 24))]
+    check_tree(ops, ns, ctx, hq, hkv, n_layer=1, layer=0)
+
+
+def test_tree_few_rows_some_long(ops):
+    """Few rows, but contexts too uneven for one CTA per sequence and kv head."""
+    rng = np.random.default_rng(11)
+    ns = rng.integers(1, 3, 40).tolist()
+    ctx = [n + int(c) for n, c in zip(ns, rng.integers(0, 50, 40))]
+    ctx[7], ctx[8], ctx[39] = 1700, 900, 1699
+    check_tree(ops, ns, ctx, 16, 8, n_layer=1, layer=0)
+
+
 @pytest.mark.parametrize("ns", [[3], [40]])
 def test_tree_long_context(ops, ns):
     check_tree(ops, ns, [5003], 8, 2, n_layer=1, layer=0)
