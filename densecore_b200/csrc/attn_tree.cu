@@ -370,6 +370,12 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&v)[16]) 
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st_frag32(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
 // and 16 lanes x 16 columns: of each 4 columns b row t / 4, column t % 4 in v[2 b] and row t / 4 + 8 in v[2 b + 1]
 __device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -708,68 +714,51 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     if (!ok) break;
                     tc_fence_after();
                     const int kb = (g.tile0 + t) * TW_KEYS;
-                    bool poison = false;
                     const bool special = kb + TW_KEYS > hist;
-                    if (special) {
-                        // V of slots past the context may be anything, and that of a drafted token that
-                        // this row does not see may be NaN: 0 x NaN is NaN, so such V become zeros
-                        const uint32_t lv = tw_v(n, N);
-                        ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (lv / TW_RING) & 1, &g_tree_error));
-                        if (!ok) break;
-                        // (pages past the sequence's last came as zeros).  A chunk of 16 bytes per lane, two keys
-                        // at a time, the warps in turn.
-                        uint32_t* bad = C.bad[wg][cleans % 3];
-                        if (tid < 4) C.bad[wg][(cleans + 1) % 3][tid] = 0;   // the last but one's: all have read it
-                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + ((lane >> 3) & 1) * TW_HALF + (lane & 7) * 16;
-                        const int end = min((g.s.L + KVB - 1) / KVB * KVB - kb, TW_KEYS);
-#pragma unroll 4
-                        for (int i = max(hist - kb, 0) / 2 + quad; 2 * i < end; i += 4) {
-                            const int key = 2 * i + (lane >> 4);
-                            uint4* chunk = (uint4*)(v + key * 128);
-                            bool odd = false;
-                            if (kb + key >= hist && kb + key < g.s.L) {
-                                const uint4 w = *chunk;
-                                const uint32_t y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    odd |= (y[e] & 0x7C00u) == 0x7C00u || (y[e] & 0x7C000000u) == 0x7C000000u;
-                            }
-                            const bool any = (__ballot_sync(0xffffffffu, odd) >> (lane & 16)) & 0xFFFFu;
-                            if (any || kb + key >= g.s.L) *chunk = make_uint4(0, 0, 0, 0);
-                            if (any && (lane & 15) == 0) atomicOr(&bad[key >> 5], 1u << (key & 31));
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&C.cleaned[wg]);
-                        ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
-                        if (!ok) break;
-                        if (live && !STACKED) {
-#pragma unroll 1
-                            for (int w = 0; w < 4; w++) {
-                                const uint32_t vis = valid ? tree_bits(a, g.s, mask, mask0, kb + 32 * w) : 0u;   // keys this row sees
-                                poison |= (vis & C.bad[wg][(cleans + 2) % 3][w]) != 0;
-                                uint32_t s[32];
-                                tmem_ld32(S + 32 * w, s);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; i++) s[i] = (vis >> i) & 1 ? s[i] : 0xFF800000u;
-                                tmem_st32(S + 32 * w, s);
-                            }
-                            tmem_wait_st();
-                        }
-                    }
-                    float m = -INFINITY, sum = 0.0f, m1 = -INFINITY, sum1 = 0.0f;
-                    if (STACKED && live) {
-                        uint32_t vis[2];                   // lane i and i + 16: the first and last 64 keys of row i
-                        if (special) {
+                    uint32_t vis[2];                       // stacked: lane i and i + 16 the first and last 64 keys of row i
+                    if (special && live) {                 // -inf for the keys that a row does not see
+                        auto bits = [&](int w) { return valid ? tree_bits(a, g.s, mask, mask0, kb + 32 * w) : 0u; };
+                        if (STACKED) {
 #pragma unroll 1
                             for (int w = 0; w < 2; w++) {
-                                const uint32_t v = valid ? tree_bits(a, g.s, mask, mask0, kb + 64 * (lane >> 4) + 32 * w) : 0u;
+                                const uint32_t v = bits(2 * (lane >> 4) + w);
                                 if (w) vis[1] = v;
                                 else vis[0] = v;
                             }
                         }
-                        bool poison1 = false;
+#pragma unroll 1
+                        for (int w = 0; w < 4; w++) {
+                            if (STACKED) {
+                                uint32_t hi[16], lo[16];
+                                tmem_ld_frag(S + 32 * w, hi);
+                                tmem_ld_frag(S + (16u << 16) + 32 * w, lo);
+                                const int from = (lane >> 2) + 16 * (w >> 1);
+                                const uint32_t v = w & 1 ? vis[1] : vis[0];
+                                const uint32_t v0 = __shfl_sync(0xffffffffu, v, from) >> (2 * (lane & 3));
+                                const uint32_t v1 = __shfl_sync(0xffffffffu, v, from + 8) >> (2 * (lane & 3));
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    if (!(((i & 2 ? v1 : v0) >> (8 * (i >> 2) + (i & 1))) & 1)) {
+                                        hi[i] = 0xFF800000u;
+                                        lo[i] = 0u;
+                                    }
+                                tmem_st_frag32(S + 32 * w, hi);
+                                tmem_st_frag32(S + (16u << 16) + 32 * w, lo);
+                            } else {
+                                const uint32_t v = bits(w);
+                                uint32_t s[32];
+                                tmem_ld32(S + 32 * w, s);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; i++) s[i] = (v >> i) & 1 ? s[i] : 0xFF800000u;
+                                tmem_st32(S + 32 * w, s);
+                            }
+                        }
+                        tmem_wait_st();
+                    }
+                    float m = -INFINITY, sum = 0.0f, m1 = -INFINITY, sum1 = 0.0f;
+                    if (STACKED && live) {
                         // rolled loops: the code of all the warps has to stay in the instruction cache
                         uint32_t hi[16], lo[16];           // the next 32 scores, loaded while x is worked on
                         float x[16];
@@ -784,18 +773,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                             if (more) {
                                 tmem_ld_frag(S + 32 * ((w + 1) & 3), hi);
                                 tmem_ld_frag(S + (16u << 16) + 32 * ((w + 1) & 3), lo);
-                            }
-                            if (special) {
-                                const int from = (lane >> 2) + 16 * (w >> 1);
-                                const uint32_t v = w & 1 ? vis[1] : vis[0];
-                                uint32_t v0 = __shfl_sync(0xffffffffu, v, from), v1 = __shfl_sync(0xffffffffu, v, from + 8);
-                                poison |= (v0 & C.bad[wg][(cleans + 2) % 3][w]) != 0;
-                                poison1 |= (v1 & C.bad[wg][(cleans + 2) % 3][w]) != 0;
-                                v0 >>= 2 * (lane & 3);
-                                v1 >>= 2 * (lane & 3);
-#pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    if (!(((i & 2 ? v1 : v0) >> (8 * (i >> 2) + (i & 1))) & 1)) x[i] = -INFINITY;
                             }
                         };
                         float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -842,8 +819,6 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                             sum += __shfl_xor_sync(0xffffffffu, sum, o);
                             sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
                         }
-                        if (poison) sum = NAN;
-                        if (poison1) sum1 = NAN;
                     } else if (live) {
                         // rolled loops: the two warpgroups' code has to stay in the instruction cache
                         float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -901,7 +876,55 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         }
                         float odd;
                         unpack2(sum2, sum, odd);
-                        sum = poison ? NAN : sum + odd;
+                        sum += odd;
+                    }
+                    if (special) {                         // behind the softmax, which V need not wait for
+                        // V of slots past the context may be anything, and that of a drafted token that
+                        // this row does not see may be NaN: 0 x NaN is NaN, so such V become zeros
+                        const uint32_t lv = tw_v(n, N);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&C.full[lv % TW_RING], (lv / TW_RING) & 1, &g_tree_error));
+                        if (!ok) break;
+                        // (pages past the sequence's last came as zeros).  A chunk of 16 bytes per lane, two keys
+                        // at a time, the warps in turn.
+                        uint32_t* bad = C.bad[wg][cleans % 3];
+                        if (tid < 4) C.bad[wg][(cleans + 1) % 3][tid] = 0;   // the last but one's: all have read it
+                        uint8_t* v = ring + (lv % TW_RING) * TW_BUF + ((lane >> 3) & 1) * TW_HALF + (lane & 7) * 16;
+                        const int end = min((g.s.L + KVB - 1) / KVB * KVB - kb, TW_KEYS);
+#pragma unroll 4
+                        for (int i = max(hist - kb, 0) / 2 + quad; 2 * i < end; i += 4) {
+                            const int key = 2 * i + (lane >> 4);
+                            uint4* chunk = (uint4*)(v + key * 128);
+                            bool odd = false;
+                            if (kb + key >= hist && kb + key < g.s.L) {
+                                const uint4 w = *chunk;
+                                const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    odd |= (y[e] & 0x7C00u) == 0x7C00u || (y[e] & 0x7C000000u) == 0x7C000000u;
+                            }
+                            const bool any = (__ballot_sync(0xffffffffu, odd) >> (lane & 16)) & 0xFFFFu;
+                            if (any || kb + key >= g.s.L) *chunk = make_uint4(0, 0, 0, 0);
+                            if (any && (lane & 15) == 0) atomicOr(&bad[key >> 5], 1u << (key & 31));
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&C.cleaned[wg]);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&C.cleaned[wg], cleans++ & 1, &g_tree_error));
+                        if (!ok) break;
+                        if (live) {                        // a row that sees a V which is not finite is NaN
+                            const uint32_t* seen = C.bad[wg][(cleans + 2) % 3];
+                            uint32_t hit = 0;
+                            if (STACKED) {
+                                hit = __ballot_sync(0xffffffffu, ((vis[0] & seen[2 * (lane >> 4)]) | (vis[1] & seen[2 * (lane >> 4) + 1])) != 0);
+                                hit |= hit >> 16;          // bit per row
+                                if ((hit >> (lane >> 2)) & 1) sum = NAN;
+                                if ((hit >> (8 + (lane >> 2))) & 1) sum1 = NAN;
+                            } else if (valid) {
+#pragma unroll 1
+                                for (int w = 0; w < 4; w++) hit |= seen[w] ? seen[w] & tree_bits(a, g.s, mask, mask0, kb + 32 * w) : 0u;
+                                if (hit) sum = NAN;
+                            }
+                        }
                     }
                     if (k) ok = __all_sync(0xffffffffu, mbar_wait(&C.x_free[wg], (k - 1) & 1, &g_tree_error));
                     if (!ok) break;
