@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         if (tid < 4) C.bad[wg][(cleans + 1) % 3][tid] = 0;   // the last but one's: all have read it
                         uint8_t* v = ring + (lv % TW_RING) * TW_BUF + ((lane >> 3) & 1) * TW_HALF + (lane & 7) * 16;
                         const int end = min((g.s.L + KVB - 1) / KVB * KVB - kb, TW_KEYS);
-#pragma unroll 4
+#pragma unroll 1
                         for (int i = max(hist - kb, 0) / 2 + quad; 2 * i < end; i += 4) {
                             const int key = 2 * i + (lane >> 4);
                             uint4* chunk = (uint4*)(v + key * 128);
