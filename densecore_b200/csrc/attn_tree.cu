@@ -255,23 +255,31 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 }
 
 // ------------------------------------------------------------------------------------------
-// tree_wide_kernel: tcgen05, 128 rows x 128 keys per unit.
+// tree_wide_kernel<STACKED>: tcgen05, one row tile x 128 keys per unit.
 //   S = Q K^T: Q as two fp16 halves (hi + lo) in shared memory, each row scaled by a power of two so
-//     that its largest value lies in [1, 2); K as it is in the cache; 16 MMAs of M128 N128 K16.
+//     that its largest value lies in [1, 2); K as it is in the cache.
 //   p = 2^(c s - m + 8), c = scale log2(e) / row scale, m the tile's own row max; cut into halves that
-//     overwrite S in tensor memory: k-step j's 8 + 8 columns lie where its 16 scores were.
-//   O = P V of this tile alone: A from tensor memory, V as it is in the cache (MN-major), 16 MMAs.
+//     overwrite S in tensor memory.
+//   O = P V of this tile alone: A from tensor memory, V as it is in the cache (MN-major).
 //   The tiles' O, m and sum of p are joined in registers, in fp32 rounded to nearest.
+// Up to 128 rows an item: both halves into one accumulator, 16 + 16 MMAs of M128 N128 K16 a unit; k-step
+// j's 8 + 8 columns of P lie where its 16 scores were.  STACKED, up to 64 rows: a row's halves are two rows
+// of the MMA (64-row MMAs take as long as 128-row ones), 8 + 8 MMAs a unit, and the softmax reads
+// fragments of 16 lanes, two halves added, 4 threads for 2 rows (98 -> 87 us for one sequence of 100,003
+// tokens and 52 rows against 64-row MMAs).
 // The tensor core cuts its sums off rather than rounding them, a bias of up to 2^-24 for each MMA that
 // adds to a large accumulator: hence the lo halves first, and no accumulator that lives for longer
-// than a tile (one that lived for a segment was 2-4 x 10^-6 off, this is 4-6 x 10^-7).
+// than a tile (one that lived for a segment was 2-4 x 10^-6 off, this is 4-8 x 10^-7).
 // Two S / P and two O buffers, used in turn.  Warps: 0 and 3 TMA producers of K (and each segment's Q,
 // up to 64 rows into a second buffer) and V (one ring of 5 x 32 KB, in the order the MMAs take them;
 // pages beyond the sequence load as zeros), 1 and 2 MMA issue for every other tile, 4-7 and 8-11 its
 // softmax, 12-15 the running output (128 registers of it per thread, thread = row).  tree_q_kernel has laid Q out
 // before: converting it here cost 20,000 cycles at every change of the item.
-// What bounds it: HBM up to 128 rows per item (64 KB per unit: 2800 cycles of an SM's share, against
-// 32 MMAs of 64 cycles); beyond, the tensor core.
+// What bounds it: a unit's chain S (700 cycles stacked, 1,470 not), softmax (2,500), O (650 / 1,250) in two
+// streams, 2,400 cycles a stacked unit while items are long, which is an SM's share of HBM (5.9 TB/s); at an
+// item's end 4,000 cycles more for masks, cleaning and the change.  Times with tree_q_kernel and
+// tree_combine_kernel: 1 x 13 tokens, 100,003 of context 83 us (410 MB, 4.9 TB/s); 32 x 16, up to 2,048
+// 49 us (163 MB); 16 x 64, 64 heads, up to 4,096 151 us (118 GFLOP with both halves, 780 TFLOP/s).
 // ------------------------------------------------------------------------------------------
 constexpr int TW_ROWS = 128;
 constexpr int TW_KEYS = 128;
@@ -1056,6 +1064,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
 // wide kernel; a block's P V starts from zero and is added to the running output in fp32 rounded to
 // nearest, because the tensor core cuts its sums off.  The warps merge in shared memory; splits leave
 // their parts for tree_join_kernel.
+// What bounds it: latency while contexts are short (8 tokens x 200: 7.8 us), HBM when they are long (8 x
+// 100,003: 71 us, 5.8 TB/s).
 // ------------------------------------------------------------------------------------------
 constexpr int TF_CONS = 3;
 constexpr int TF_STAGES = 9;

@@ -38,13 +38,15 @@ cudaError_t pages_device_error(int* out, bool clear) {
 //   apply   column strips of the table permuted through shared memory (every row's old entry is read
 //           before a new one is written), and the partial pages' slots copied.
 // When the plan finds bad input or too few pages, apply takes the deltas back and nothing changes.
-// What bounds it: the copied slots (HBM); a batch without copies is three launches' latency.
+// What bounds it: the copied slots (HBM), behind the plan's chain of loads and scans in one CTA (6 us);
+// a batch with few copies is that and the launches' latency.  8 rows, 28 layers: 10.2 us; 64 rows of
+// beam search, 36 layers, 73 MB read and written: 23 us (6.5 TB/s over the copies' own 11 us).
 // ------------------------------------------------------------------------------------------
 constexpr int FORK_MAX_ROWS = 4096;
 constexpr int FORK_THREADS = 256;
-constexpr int FORK_BATCH = 8;            // 16-byte loads in flight per thread of a copy
+constexpr int FORK_BATCH = 8;            // 16-byte loads in flight per thread of a copy (64 rows: 23.3 us; 4 or 16: 26.5)
 constexpr int PLAN_THREADS = 1024;
-constexpr int FORK_SMALL = 65536;       // table entries (64 x 1024: a few microseconds for one CTA)
+constexpr int FORK_SMALL = 65536;        // table entries a CTA counts itself (8 rows 10.2 us, in three launches 12.1)
 constexpr int PLAN_PER = 16;             // reference counts per thread and scan step
 constexpr int STRIP_INTS = 8192;         // 32 KB of table entries per strip
 
@@ -377,7 +379,9 @@ int kv_fork_max_rows() { return FORK_MAX_ROWS; }
 // path is strictly ascending, so path[j] >= j and a slot is read before or when it is written; each
 // thread owns one 16-byte column of one layer's K or V for the whole path, so the order within a
 // thread is the only order there is.  What bounds it: the moved bytes, 16 B loads with a batch of
-// COMPACT_BATCH in flight per thread before the first store.
+// COMPACT_BATCH in flight per thread before the first store.  32 paths of 64 tokens, 36 layers (171 MB
+// read and written): 31.1 us, 5.5 TB/s, of which the kernel's own 26 us are the rate of a copy; batches
+// of 4 31.7, of 16 32.5.  One path of 8: 2.5 us, a launch.
 // ------------------------------------------------------------------------------------------
 constexpr int COMPACT_THREADS = 256;
 constexpr int COMPACT_BATCH = 8;

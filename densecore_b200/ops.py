@@ -7,6 +7,11 @@ stream; all arithmetic runs in the sm_100a kernels.  Names follow the reference 
   QuantWeight                             a weight tensor resident on the device (the
                                           weight_tensor->data of cb_gemv_custom, uploaded once)
   HostContext                             the synchronous host-pointer boundary (dcg_ctx_*)
+  paged_attn_tree                         the attention selector (inference.cpp:1506-1573) for drafted
+                                          token trees, over the paged cache
+  kv_fork / kv_compact                    BlockManager's shared, copied-on-write blocks
+                                          (core/src/kv_cache.cpp:67-315), a batch at a time
+  beam_select                             the k best continuations of groups of beams
 """
 from __future__ import annotations
 
