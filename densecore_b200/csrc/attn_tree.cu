@@ -290,8 +290,8 @@ constexpr int TW_HALF = TW_BUF / 2;
 constexpr int TW_THREADS = 512;
 constexpr int TW_OFF_RING = 2 * TW_BUF;           // Q hi, Q lo first
 constexpr int TW_OFF_CTRL = TW_OFF_RING + TW_RING * TW_BUF;
-constexpr int TW_CTRL = 3072;
-constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // all of it: 227 KB
+constexpr int TW_CTRL = 2560;
+constexpr int TW_SMEM = TW_OFF_CTRL + TW_CTRL;    // of 227 KB
 constexpr int TW_EXTRA = 4, TW_EXTRA_STACKED = 2; // an item's fixed cost in units (5.7 us against 1.4 us a unit; 2.4 and 1.1)
 constexpr float TW_SHIFT = 8.0f;                  // p is at most 2^8: the small ones stay above fp16's least
 // registers per thread of the four warpgroups (control, 2 x softmax, output): 512 of a launch's 4 x 128,
