@@ -1069,6 +1069,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
 // ------------------------------------------------------------------------------------------
 constexpr int TF_CONS = 3;
 constexpr int TF_STAGES = 9;
+// A slot always belongs to the same consumer warp: one that another warp had not emptied yet would look
+// full by the parity of its phase.
+static_assert(TF_STAGES % TF_CONS == 0, "ring and consumers");
 constexpr int TF_TILE = KVB * HD * 2;             // 4 KB: [half of 64 dims][16 keys][128 B]
 constexpr int TF_STAGE = 2 * TF_TILE;             // K, V
 
