@@ -216,6 +216,27 @@ def test_tree_bad_values_stay_with_the_rows_that_see_them(ops, nodes):
                 assert (np.abs(out[i, h] - ref[i, h]) <= tol[i, h]).all()
 
 
+@pytest.mark.parametrize("nodes", [4, 12, 30])
+def test_tree_bad_values_in_many_sequences(ops, nodes):
+    """The same in every second sequence of a batch, at places all over the key tiles."""
+    rng = np.random.default_rng(nodes)
+    ctx = [nodes + int(c) for c in rng.integers(0, 300, 40)]
+    ka, va, bt, starts, q = make_tree(rng, [nodes] * 40, ctx, 8, 2, 1)
+    mask, seen = random_seen(rng, [nodes] * 40)
+    clean, at = va.copy(), rng.integers(0, nodes, 40)
+    for s in range(0, 40, 2):
+        p = ctx[s] - nodes + at[s]
+        va[bt[s, p // 16], p % 16, 1, 77] = np.nan if s % 4 else np.inf
+    out = run_tree(ops, q, ka, va, 1, 0, bt, starts, ctx, mask, 2, nodes).cpu().numpy()
+    ref, tol = R.tree_attention(q, ka, clean, 1, 0, bt, starts, ctx, seen, 2, 128 ** -0.5)
+    for s in range(40):
+        for i in range(nodes * s, nodes * (s + 1)):
+            bad = s % 2 == 0 and at[s] in seen[i]
+            assert np.isnan(out[i, 4:, 77]).all() if bad else np.isfinite(out[i, 4:]).all()
+            heads = slice(0, 4 if bad else 8)
+            assert (np.abs(out[i, heads] - ref[i, heads]) <= tol[i, heads]).all()
+
+
 @pytest.mark.parametrize("n", [1, 12, 50])
 def test_tree_chain_is_the_causal_prefill(ops, n):
     rng = np.random.default_rng(5)
@@ -331,6 +352,19 @@ def test_tree_captured_streams_and_repeats(ops, n):
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, eager) and torch.equal(out2, eager)
+
+
+@pytest.mark.parametrize("n", [9, 12, 16])
+def test_tree_rows_between_few_and_many(ops, n):
+    """The cases above with 36, 48 and 64 rows per kv head."""
+    test_tree_rows_that_see_nothing(ops, [n, n])
+    test_tree_ignores_what_nobody_sees(ops, [n, n - 1])
+    test_tree_bad_values_stay_with_the_rows_that_see_them(ops, n)
+    test_tree_empty_sequence(ops, n)
+    test_tree_bad_indexes_are_left_out(ops, n)
+    test_tree_captured_streams_and_repeats(ops, n)
+    for gain in (1e-6, 8.0, 3e4):
+        test_tree_query_magnitudes(ops, gain, [n])
 
 
 # ------------------------------------------------------------------------------------------- fork
