@@ -135,7 +135,7 @@ struct TreeStart {
 // Up to THREADS sequences the search runs in shared memory (a chain of global loads cost 3 us).
 template <int ROWS, int KEYS, int THREADS>
 __device__ void tree_plan_ranges(const TreeArgs& a, int extra) {
-    __shared__ int64_t sums[2][THREADS / 32], s_cost[THREADS], s_units[THREADS];
+    __shared__ int64_t sums[2][THREADS / 32], s_cost[THREADS], s_units[THREADS], s_begin[THREADS];
     __shared__ TreeSeq s_seq[THREADS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool small = a.n_seqs <= THREADS;
@@ -185,9 +185,11 @@ __device__ void tree_plan_ranges(const TreeArgs& a, int extra) {
     const int G = (int)min((int64_t)a.G, V);      // no more ranges than cost: none is empty inside an item
     __syncthreads();
     auto seq_at = [&](int i) { return i >= a.n_seqs ? TreeSeq{0, 0, 0, 0, 0} : small ? s_seq[i] : tree_seq<ROWS, KEYS>(a, i, false); };
-    // range c's first unit; where that lies
-    auto begin = [&](int c, TreeSeg& g) -> int64_t {
-        if (c >= G) return run_u;
+    // a range per thread: its first unit, and where that lies (a.G < THREADS)
+    const int c = threadIdx.x;
+    TreeStart b = {};
+    b.u0 = run_u;
+    if (c < G) {
         const int64_t v = sk_begin(c, V, G);
         int lo = 0, hi = a.n_seqs;                 // the last sequence that begins at or before v
         while (hi - lo > 1) {
@@ -195,29 +197,27 @@ __device__ void tree_plan_ranges(const TreeArgs& a, int extra) {
             if (cost[mid] <= v) lo = mid;
             else hi = mid;
         }
-        g.seq = lo;
-        g.s = seq_at(lo);
-        const int off = (int)(v - cost[lo]), each = g.s.tiles + extra, item = off / each;
-        g.tile0 = max(0, off - item * each - extra);
-        g.kvh = item / g.s.row_tiles;
-        g.rt = item - g.kvh * g.s.row_tiles;
-        return units[lo] + (int64_t)item * g.s.tiles + g.tile0;
-    };
-    for (int c = threadIdx.x; c <= a.G; c += THREADS) {
-        TreeStart b = {};
-        a.bounds[c] = b.u0 = begin(c, b.g);
-        if (c < a.G) {
-            TreeSeg end;
-            b.N = (int)(begin(c + 1, end) - b.u0);
-            b.g.left = b.N;
-            if (b.N) {
-                b.g.next = seq_at(b.g.seq + 1);
-                seg_shape<ROWS>(a, b.g);
-            }
-            a.begins[c] = b;
-            a.cuts[c].rows = 0;
-        }
+        b.g.seq = lo;
+        b.g.s = seq_at(lo);
+        const int off = (int)(v - cost[lo]), each = b.g.s.tiles + extra, item = off / each;
+        b.g.tile0 = max(0, off - item * each - extra);
+        b.g.kvh = item / b.g.s.row_tiles;
+        b.g.rt = item - b.g.kvh * b.g.s.row_tiles;
+        b.u0 = units[lo] + (int64_t)item * b.g.s.tiles + b.g.tile0;
     }
+    s_begin[c] = b.u0;
+    __syncthreads();
+    if (c > a.G) return;
+    a.bounds[c] = b.u0;
+    if (c == a.G) return;
+    b.N = (int)(s_begin[c + 1] - b.u0);
+    b.g.left = b.N;
+    if (b.N) {
+        b.g.next = seq_at(b.g.seq + 1);
+        seg_shape<ROWS>(a, b.g);
+    }
+    a.begins[c] = b;
+    a.cuts[c].rows = 0;
 }
 
 // mask bits of keys g0 .. g0 + 31 (as positions) for the drafted token of mask row `m`, whose first word
@@ -1523,7 +1523,7 @@ static TreePlan tree_plan(int n_seqs, int hq, int hkv, int max_seq_tokens, int m
         p.rows = (int)rows;
         parts = p.splits > 1 ? (size_t)n_seqs * hkv * p.splits : 0;
     } else {
-        p.G = num_sms();
+        p.G = min(num_sms(), TQ_WARPS * 32 - 1);               // a planning thread each
         p.rows = (int)(rows < TW_ROWS ? rows : TW_ROWS);
         p.q_rows = p.rows <= TW_STACK ? (p.rows + 15) / 16 * 16 : (p.rows + 7) / 8 * 8;
         p.row_tiles = (int)((rows + TW_ROWS - 1) / TW_ROWS);
