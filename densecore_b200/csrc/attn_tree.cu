@@ -433,8 +433,9 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
     const int seq = blockIdx.y - 1;
     const TreeSeq s = tree_seq<TW_ROWS, TW_KEYS>(a, seq, false);
     const int x0 = blockIdx.x * TQ_ROWS, n = min(TQ_ROWS, s.ns * a.hq - x0), lane = threadIdx.x & 31;
-    if (n <= 0) return;
-    if (threadIdx.x == 0) {
+    const int to = s.row_tiles ? (s.row_tiles - 1) * TW_ROWS + a.q_rows : 0;   // rows that tree_wide_kernel reads
+    if (x0 / a.hq * a.nrep >= to) return;
+    if (threadIdx.x == 0 && n > 0) {
         mbar_init(&bar, 1);
         fence_mbar_init();
         mbar_arrive_expect_tx(&bar, (uint32_t)n * HD * 4);
@@ -443,16 +444,19 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
     __syncthreads();
     const bool stacked = a.q_rows <= TW_STACK;
     const int dims_half = a.q_rows * (stacked ? 256 : 128), to_lo = stacked ? 16 * 128 : a.q_rows * 256;
-    if (!mbar_wait(&bar, 0, &g_tree_error)) return;
+    if (n > 0 && !mbar_wait(&bar, 0, &g_tree_error)) return;
 #pragma unroll 1
-    for (int i0 = (threadIdx.x >> 5) * 4; i0 < n; i0 += TQ_WARPS * 4) {
-        const int i = min(i0 + (lane >> 3), n - 1), sub = lane & 7;   // (the last row by several alike)
-        float x[2][8], m = 0.0f;                  // dims 8 sub .. +7 of both halves
+    for (int i0 = (threadIdx.x >> 5) * 4; i0 < TQ_ROWS; i0 += TQ_WARPS * 4) {
+        const int i = i0 + (lane >> 3), sub = lane & 7;
+        const int t = (x0 + i) / a.hq, h = x0 + i - t * a.hq;
+        const int kvh = h / a.nrep, R = t * a.nrep + h - kvh * a.nrep, rt = R / TW_ROWS, r = R - rt * TW_ROWS;
+        const int64_t tile = ((int64_t)seq * a.row_tiles + rt) * a.hkv + kvh;
+        float x[2][8], m = 0.0f;                  // dims 8 sub .. +7 of both halves; zeros behind the last query
 #pragma unroll
         for (int d = 0; d < 2; d++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const float4 y = *(const float4*)(rows + i * HD + 64 * d + 8 * sub + 4 * c);
+                const float4 y = i < n ? *(const float4*)(rows + i * HD + 64 * d + 8 * sub + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
                 x[d][4 * c] = y.x;
                 x[d][4 * c + 1] = y.y;
                 x[d][4 * c + 2] = y.z;
@@ -461,15 +465,13 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
             }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const int t = (x0 + i) / a.hq, h = x0 + i - t * a.hq;
-        const int kvh = h / a.nrep, R = t * a.nrep + h - kvh * a.nrep, rt = R / TW_ROWS, r = R - rt * TW_ROWS;
-        const int64_t tile = ((int64_t)seq * a.row_tiles + rt) * a.hkv + kvh;
+        if (R >= to) continue;
         // exponent of the row's largest value (0 rows and subnormal ones: the least)
         int e = (int)(__float_as_uint(m) >> 23) - 127;
         e = e < -100 ? -100 : e > 120 ? 120 : e;
         const float f = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);   // 2^-e
         const int at = stacked ? 2 * r - (r & 15) : r;
-        uint8_t* to = a.q_tiles + tile * a.q_rows * 512 + at * 128 + ((sub ^ (r & 7)) << 4);
+        uint8_t* dst = a.q_tiles + tile * a.q_rows * 512 + at * 128 + ((sub ^ (r & 7)) << 4);
 #pragma unroll
         for (int d = 0; d < 2; d++) {
             uint4 hi, lo;
@@ -477,8 +479,8 @@ __global__ void __launch_bounds__(TQ_WARPS * 32) tree_q_kernel(const TreeArgs a)
             cut_h2(x[d][2] * f, x[d][3] * f, hi.y, lo.y);
             cut_h2(x[d][4] * f, x[d][5] * f, hi.z, lo.z);
             cut_h2(x[d][6] * f, x[d][7] * f, hi.w, lo.w);
-            *(uint4*)(to + d * dims_half) = hi;
-            *(uint4*)(to + d * dims_half + to_lo) = lo;
+            *(uint4*)(dst + d * dims_half) = hi;
+            *(uint4*)(dst + d * dims_half + to_lo) = lo;
         }
         if (sub == 0) a.q_exps[tile * a.q_rows + r] = (int8_t)e;
     }
@@ -518,6 +520,10 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
         fence_mbar_init();
     }
     if (threadIdx.x < 24) (&C.bad[0][0][0])[threadIdx.x] = 0;
+    if (STACKED) {                                // rows without a query stay zeros: the tensor core's power is the limit
+        for (int i = threadIdx.x; i < 2 * TW_BUF / 16; i += TW_THREADS) ((uint4*)smem)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&C.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -534,7 +540,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
     bool ok = true;
 
     constexpr int q_bufs = STACKED ? 2 : 1;       // as many as there is room for
-    const int q_bytes = a.q_rows * 512;
+    const int q_bytes = a.q_rows * 512, q_buf = STACKED ? TW_BUF : q_bytes;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(tw_regs_ctrl(STACKED)));
         if (N == 0) {
@@ -565,7 +571,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     if (!ok) break;
                     if (lane == 0) {
                         mbar_arrive_expect_tx(&C.q_full[qb], (uint32_t)q_bytes);
-                        bulk_g2s(smem + qb * q_bytes, a.q_tiles + q_tile * q_bytes, (uint32_t)q_bytes, &C.q_full[qb]);
+                        for (int d = 0; d < (STACKED ? 2 : 1); d++)
+                            bulk_g2s(smem + qb * q_buf + d * TW_HALF, a.q_tiles + q_tile * q_bytes + d * (q_bytes / 2),
+                                     (uint32_t)(STACKED ? q_bytes / 2 : q_bytes), &C.q_full[qb]);
                     }
                     seg++;
                 }
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             // Each in step, one elected thread issuing.  A warp's polls, and its waits for the tensor core to
             // take its last operands, leave the core with the other's work.
             constexpr uint32_t id_s = idesc_f16(TW_ROWS, TW_KEYS, false), id_o = idesc_f16(TW_ROWS, HD, true);
-            const uint32_t qs = smem_u32(smem), rg = qs + TW_OFF_RING, q_half = a.q_rows * (STACKED ? 256 : 128);
+            const uint32_t qs = smem_u32(smem), rg = qs + TW_OFF_RING, q_half = STACKED ? TW_HALF : a.q_rows * 128;
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const bool leader = elect_one();
             const int b = warp - 1;
@@ -627,7 +635,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                     tc_fence_after();
                 }
                 if (leader) {
-                    const uint32_t q = qs + qb * q_bytes;
+                    const uint32_t q = qs + qb * q_buf;
                     const uint64_t kd = umma_desc_sw128(rg + slot * TW_BUF);
 #pragma unroll
                     for (int h = STACKED ? 0 : 1; h >= 0; h--) {   // the lo half first
@@ -799,7 +807,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                         }
                         m = y[0] * c;
                         m1 = y[2] * c1;
-                        const float sh0 = TW_SHIFT - (m == -INFINITY ? 0.0f : m), sh1 = TW_SHIFT - (m1 == -INFINITY ? 0.0f : m1);
+                        // (rows without a query: p = 0)
+                        const float sh0 = r0 < g.rows ? TW_SHIFT - (m == -INFINITY ? 0.0f : m) : -INFINITY;
+                        const float sh1 = r1 < g.rows ? TW_SHIFT - (m1 == -INFINITY ? 0.0f : m1) : -INFINITY;
                         const uint64_t k2[2] = {pack2(c, c), pack2(c1, c1)}, h2[2] = {pack2(sh0, sh0), pack2(sh1, sh1)};
                         uint64_t sum2[2] = {0, 0};
 #pragma unroll 1
@@ -1593,7 +1603,9 @@ cudaError_t launch_paged_attn_tree(const float* q, const void* karena, const voi
     const bool stacked = p.rows <= TW_STACK;
     e = stacked ? DCG_SMEM_ATTR(tree_wide_kernel<true>, TW_SMEM) : DCG_SMEM_ATTR(tree_wide_kernel<false>, TW_SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(tree_q_kernel, dim3((unsigned)(((int64_t)max_seq_tokens * hq + TQ_ROWS - 1) / TQ_ROWS), (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
+    // tokens with those behind a sequence's last whose rows belong to its last tile
+    const int64_t q_tokens = ((int64_t)(p.row_tiles - 1) * TW_ROWS + p.q_rows + a.nrep - 1) / a.nrep;
+    e = launch_pdl(tree_q_kernel, dim3((unsigned)((q_tokens * hq + TQ_ROWS - 1) / TQ_ROWS), (unsigned)n_seqs + 1), dim3(TQ_WARPS * 32), 0, st, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(stacked ? tree_wide_kernel<true> : tree_wide_kernel<false>, dim3((unsigned)p.G), dim3(TW_THREADS), (size_t)TW_SMEM, st, km, vm, a);
     if (e != cudaSuccess) return e;
