@@ -278,8 +278,9 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // What bounds it: a unit's chain S (700 cycles stacked, 1,470 not), softmax (2,500), O (650 / 1,250) in two
 // streams, 2,400 cycles a stacked unit while items are long, which is an SM's share of HBM (5.9 TB/s); at an
 // item's end 4,000 cycles more for masks, cleaning and the change.  Times with tree_q_kernel and
-// tree_combine_kernel: 1 x 13 tokens, 100,003 of context 83 us (410 MB, 4.9 TB/s); 32 x 16, up to 2,048
-// 49 us (163 MB); 16 x 64, 64 heads, up to 4,096 151 us (118 GFLOP with both halves, 780 TFLOP/s).
+// tree_combine_kernel: 1 x 13 tokens, 100,003 of context 81 us (410 MB, 5.1 TB/s); 32 x 16, up to 2,048
+// 49 us (163 MB); 16 x 64, 64 heads, up to 4,096 148 us (118 GFLOP with both halves, 800 TFLOP/s); sustained, at
+// the power limit's clock, 99, 52 and 180 us.
 // ------------------------------------------------------------------------------------------
 constexpr int TW_ROWS = 128;
 constexpr int TW_KEYS = 128;
