@@ -11,8 +11,8 @@
 // CTA whatever row they lie in.  Per part of a row that a CTA meets it leaves the part's k largest
 // logits, and per tile and warp the max and the sum of exp(x - max) over the others: sums that do not
 // depend on how the rows were cut, so that rows with the same logits tie exactly.  beam_merge_kernel, one CTA per group, joins them.
-// What bounds it: HBM in the pass over many rows (512 beams of 128,256 logits: 70 us with the merge's
-// 12, 4.5 TB/s in the pass), the two launches' latency over few (4 beams of 151,936: 10.4 us).
+// What bounds it: HBM in the pass over many rows (512 beams of 128,256 logits: 69 us with the merge's
+// 11, 4.5 TB/s in the pass), the two launches' latency over few (4 beams of 151,936: 9.4 us).
 #include <math.h>
 
 #include "../../include/dcgpu.h"
@@ -329,6 +329,7 @@ __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
 }
 
 constexpr int MERGE_PER = 4;
+constexpr int MERGE_SUMS = 8;                            // a thread's tile sums under way (35 beams: 16.8 us, with 4 or 6 17.1, with 16 19)
 constexpr int MERGE_TILE = BEAM_THREADS * MERGE_PER;
 
 // one CTA per group; candidate c = (rank c / lists in part-list c % lists): the heads come first
@@ -355,14 +356,26 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
         const float2* p = sums + (row0 + b) * tpr * BEAM_WARPS;
         const int np = tpr * BEAM_WARPS;
         float M = -INFINITY;
-#pragma unroll 4
-        for (int i = lane; i < np; i += 32) M = fmaxf(M, p[i].x);
-        M = warp_max(M);
         double s = 0.0;
-#pragma unroll 4
-        for (int i = lane; i < np; i += 32) {
-            const float2 q = p[i];
-            if (q.x > -INFINITY || q.y != 0.0f) s += (1.0 + (double)q.y) * (double)ex2((q.x - M) * LOG2E);
+#pragma unroll 1
+        for (int i0 = 0; i0 < np; i0 += 32 * MERGE_SUMS) {
+            float2 q[MERGE_SUMS];                 // loaded once
+#pragma unroll
+            for (int i = 0; i < MERGE_SUMS; i++) {
+                const int at = i0 + 32 * i + lane;
+                q[i] = at < np ? p[at] : make_float2(-INFINITY, 0.0f);
+            }
+            float m = q[0].x;
+#pragma unroll
+            for (int i = 1; i < MERGE_SUMS; i++) m = fmaxf(m, q[i].x);
+            m = warp_max(m);
+            if (m > M) {
+                s *= (double)ex2((M - m) * LOG2E);
+                M = m;
+            }
+#pragma unroll
+            for (int i = 0; i < MERGE_SUMS; i++)
+                if (q[i].x > -INFINITY || q[i].y != 0.0f) s += (1.0 + (double)q[i].y) * (double)ex2((q[i].x - M) * LOG2E);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
