@@ -39,14 +39,14 @@ cudaError_t pages_device_error(int* out, bool clear) {
 //           before a new one is written), and the partial pages' slots copied.
 // When the plan finds bad input or too few pages, apply takes the deltas back and nothing changes.
 // What bounds it: the copied slots (HBM), behind the plan's chain of loads and scans in one CTA (6 us);
-// a batch with few copies is that and the launches' latency.  8 rows, 28 layers: 10.2 us; 64 rows of
-// beam search, 36 layers, 73 MB read and written: 23 us (6.5 TB/s over the copies' own 11 us).
+// a batch with few copies is that and the launches' latency.  8 rows, 28 layers: 9.6 us; 64 rows of
+// beam search, 36 layers, 73 MB read and written: 22.7 us (the copies alone 11).
 // ------------------------------------------------------------------------------------------
 constexpr int FORK_MAX_ROWS = 4096;
 constexpr int FORK_THREADS = 256;
 constexpr int FORK_BATCH = 8;            // 16-byte loads in flight per thread of a copy (64 rows: 23.3 us; 4 or 16: 26.5)
 constexpr int PLAN_THREADS = 1024;
-constexpr int FORK_SMALL = 65536;        // table entries a CTA counts itself (8 rows 10.2 us, in three launches 12.1)
+constexpr int FORK_SMALL = 65536;        // table entries a CTA counts itself (8 rows 10.2 us where three launches took 12.1)
 constexpr int PLAN_PER = 16;             // reference counts per thread and scan step
 constexpr int STRIP_INTS = 8192;         // 32 KB of table entries per strip
 
@@ -147,7 +147,8 @@ __device__ int block_scan(int v, int* warp_sums, int* sum) {
 template <bool SMALL>
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs a) {
     __shared__ int s_src[FORK_MAX_ROWS];     // partly filled last page of each new row, or -1
-    __shared__ int s_par[SMALL ? PLAN_THREADS : 1], s_len[SMALL ? PLAN_THREADS : 1], s_kids[SMALL ? PLAN_THREADS : 1];
+    // SMALL: read once, all loads together
+    __shared__ int s_par[SMALL ? PLAN_THREADS : 1], s_len[SMALL ? PLAN_THREADS : 1], s_held[SMALL ? PLAN_THREADS : 1], s_kids[SMALL ? PLAN_THREADS : 1];
     __shared__ int warp_sums[32];
     __shared__ int s_copies;
     pdl_wait();
@@ -155,19 +156,22 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs 
     const int t = threadIdx.x;
     if (t == 0) s_copies = 0;
     bool bad = false;
+    int my_reserve = 0, my_now = 0, my_used = 0, my_held = 0;   // SMALL: of row t
     if (SMALL) {
         int p = -1;
         s_kids[t] = 0;
         if (t < a.n) {
             s_par[t] = p = a.parents[t];
             s_len[t] = a.lens[t];
+            s_held[t] = my_held = a.held[t];
+            my_reserve = a.reserve ? a.reserve[t] : 0;
             bad = p < -1 || p >= a.n;
         }
         __syncthreads();
         if (p >= 0 && !bad) atomicAdd(&s_kids[p], 1);
         __syncthreads();
         for (int r = t >> 5; r < a.n; r += PLAN_THREADS / 32) {
-            const OldRow row = sized_row(a, s_par[r], s_len[r], a.held[r], s_kids[r]);
+            const OldRow row = sized_row(a, s_par[r], s_len[r], s_held[r], s_kids[r]);
             bad |= row.bad;
             bad |= add_deltas(a, r, row, 1, t & 31, 32);
         }
@@ -183,14 +187,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs 
     for (int i = t; i < a.n; i += PLAN_THREADS) {
         const int p = SMALL ? s_par[i] : a.parents[i];
         const int len = p < 0 ? 0 : SMALL ? s_len[p] : a.lens[p];
-        const int64_t need = p >= 0 ? (int64_t)len + (a.reserve ? a.reserve[i] : 0) : 0;
+        const int more = SMALL ? my_reserve : a.reserve ? a.reserve[i] : 0;
+        const int64_t need = p >= 0 ? (int64_t)len + more : 0;
         const int used = (len + KVB - 1) / KVB;
         const int64_t total = (need + KVB - 1) / KVB;
-        bad |= p >= 0 && ((a.reserve && a.reserve[i] < 0) || total > a.mbs);
+        bad |= p >= 0 && (more < 0 || total > a.mbs);
         s_src[i] = len % KVB ? a.bt[(int64_t)p * a.mbs + used - 1] : -1;
         a.new_len[i] = len;
-        a.new_held[i] = (int)(total > a.mbs ? a.mbs : total);
-        a.old_held[i] = a.held[i];
+        my_now = (int)(total > a.mbs ? a.mbs : total);
+        my_used = used;
+        if (!SMALL) my_held = a.held[i];
+        a.new_held[i] = my_now;
+        a.old_held[i] = my_held;
         a.used[i] = used;
     }
     bad = __syncthreads_or(bad);
@@ -211,11 +219,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const ForkArgs 
                 for (int j = 0; j < i; j++) rank += s_src[j] == b;
                 copy = held - rank > 1;
             }
-            const int now = a.new_held[i];
-            want = copy + now - a.used[i];
+            const int now = SMALL ? my_now : a.new_held[i];
+            want = copy + now - (SMALL ? my_used : a.used[i]);
             a.src[i] = copy ? b : -1;
             if (copy) a.copies[atomicAdd(&s_copies, 1)] = i;
-            columns = max(columns, max(now, a.old_held[i]));
+            columns = max(columns, max(now, SMALL ? my_held : a.old_held[i]));
         }
         int sum;
         const int at = block_scan(want, warp_sums, &sum);
