@@ -12,7 +12,7 @@
 // logits, and per tile and warp the max and the sum of exp(x - max) over the others: sums that do not
 // depend on how the rows were cut, so that rows with the same logits tie exactly.  beam_merge_kernel, one CTA per group, joins them.
 // What bounds it: HBM in the pass over many rows (512 beams of 128,256 logits: 69 us with the merge's
-// 11, 4.5 TB/s in the pass), the two launches' latency over few (4 beams of 151,936: 9.4 us).
+// 11, 4.5 TB/s in the pass), the two launches' latency over few (4 beams of 151,936: 9.5 us).
 #include <math.h>
 
 #include "../../include/dcgpu.h"
@@ -332,8 +332,9 @@ constexpr int MERGE_PER = 4;
 constexpr int MERGE_SUMS = 8;                            // a thread's tile sums under way (35 beams: 16.8 us, with 4 or 6 17.1, with 16 19)
 constexpr int MERGE_TILE = BEAM_THREADS * MERGE_PER;
 
-// one CTA per group; candidate c = (rank c / lists in part-list c % lists): the heads come first
-__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
+// one CTA per group; candidate c = (rank c / lists in part-list c % lists): the heads come first.  (One CTA per SM
+// in the bounds and rolled loops: held to 64 registers, it spilled and took 2 us more.)
+__global__ void __launch_bounds__(BEAM_THREADS, 1) beam_merge_kernel(
     const uint64_t* __restrict__ keys, const float2* __restrict__ sums, int tpr, int64_t T, int G, int max_parts,
     const float* __restrict__ scores, const uint8_t* __restrict__ finished, int eos, int n_beams, int k,
     float* __restrict__ out_scores, int* __restrict__ out_rows, int* __restrict__ out_tokens) {
@@ -348,10 +349,12 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t row0 = (int64_t)blockIdx.x * n_beams;
     const int lists = n_beams * max_parts, N = lists * k;   // max_parts <= G: below 2^31
+#pragma unroll 1
     for (int b = t; b < n_beams; b += BEAM_THREADS) {
         const int64_t u = (row0 + b) * tpr;
         n_parts[b] = finished && finished[row0 + b] ? 0 : (int)(beam_owner(u + tpr - 1, T, G) - beam_owner(u, T, G)) + 1;
     }
+#pragma unroll 1
     for (int b = warp; b < n_beams; b += BEAM_WARPS) {
         const float2* p = sums + (row0 + b) * tpr * BEAM_WARPS;
         const int np = tpr * BEAM_WARPS;
@@ -390,7 +393,9 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
     bool full = false;                     // list[k - 1] bounds what may still enter
     Cand bound = {-INFINITY, 0, 0};
     uint32_t th = 0;
-    for (int c0 = 0; c0 < N; c0 += MERGE_TILE) {
+    int quiet = 0;                         // candidates since the last that came in
+#pragma unroll 1
+    for (int c0 = 0; c0 < N && quiet < lists; c0 += MERGE_TILE) {
         Cand v[MERGE_PER];
         uint32_t best = 0;
 #pragma unroll
@@ -411,24 +416,34 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
         }
         // scores rounded down keep their order
         if (c0 == 0) th = block_threshold(best, k, S.sh);
-        bool over = false;
+        bool over = false, came = false;
 #pragma unroll
         for (int j = 0; j < MERGE_PER; j++)
             if (v[j].row >= 0 && (full ? better(v[j], bound) : float_key(__double2float_rd(v[j].score)) >= th)) {
                 const int slot = atomicAdd(&S.count, 1);
                 list[slot] = v[j];
                 over |= slot >= BEAM_RANK;
+                came = true;
             }
-        if (__syncthreads_or(over || c0 + MERGE_TILE >= N)) {
+        // the lists descend: once none of a whole rank comes in, nothing behind does (16 beams of 119,088 logits
+        // in one group, k 32: 48 us without this)
+        bool last = c0 + MERGE_TILE >= N;
+        if (!last) {
+            quiet = __syncthreads_or(came) ? 0 : quiet + MERGE_TILE;
+            last = quiet >= lists;
+        }
+        if (__syncthreads_or(over || last)) {
             n = S.count;
             const int keep = n < k ? n : k;
             int m = n;
             const Cand* from = list;
             if (n > BEAM_FEW) {            // as prune_keys, by score alone
                 uint32_t top = 0;
+#pragma unroll 1
                 for (int i = t; i < n; i += BEAM_THREADS) top = max(top, float_key(__double2float_rd(list[i].score)));
                 if (t == 0) S.kept = 0;
                 const uint32_t reach = block_threshold(top, k, S.sh);
+#pragma unroll 1
                 for (int i = t; i < n; i += BEAM_THREADS)
                     if (float_key(__double2float_rd(list[i].score)) >= reach) {
                         const int slot = atomicAdd(&S.kept, 1);
@@ -450,13 +465,15 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
                 if (t < m && rank < keep) list[rank] = mine;
             } else {
                 Cand found = {0, 0, 0}, below = {INFINITY, 0, 0};
+#pragma unroll 1
                 for (int r = 0; r < keep; r++) {
                     Cand b = {-INFINITY, 0, INT32_MAX};
+#pragma unroll 1
                     for (int i = t; i < n; i += BEAM_THREADS) {
                         const Cand x = list[i];
                         if (better(below, x) && better(x, b)) b = x;
                     }
-#pragma unroll
+#pragma unroll 1
                     for (int o = 16; o; o >>= 1) {
                         Cand w;
                         w.score = __shfl_xor_sync(0xffffffffu, b.score, o);
@@ -467,7 +484,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(
                     if (lane == 0) best_of[warp] = b;
                     __syncthreads();
                     b = best_of[0];
-#pragma unroll
+#pragma unroll 1
                     for (int w = 1; w < BEAM_WARPS; w++)
                         if (better(best_of[w], b)) b = best_of[w];
                     __syncthreads();

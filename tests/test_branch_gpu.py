@@ -616,6 +616,22 @@ def test_beam_random(ops, groups, n_beams, vocab, k):
     check_beam(ops, x, -rng.random(groups * n_beams).astype(np.float32) * 5, n_beams, k)
 
 
+@pytest.mark.parametrize("groups,n_beams,vocab,k", [(1, 16, 60007, 32), (2, 40, 30011, 64), (1, 200, 9001, 8)])
+@pytest.mark.parametrize("spread", [False, True])
+def test_beam_many_lists_of_one_group(ops, groups, n_beams, vocab, k, spread):
+    """Few groups of many parts: more candidates than the merge looks at in one go, the best of them in a
+    few of the parts or (spread) one in each."""
+    rng = np.random.default_rng(vocab + spread)
+    x = rng.standard_normal((groups * n_beams, vocab)).astype(np.float32)
+    scores = (rng.standard_normal(groups * n_beams) * (0.01 if spread else 3)).astype(np.float32)
+    if spread:
+        x = np.minimum(x, 3)
+        for r in range(len(x)):
+            x[r, rng.integers(0, 4096, vocab // 4096) + 4096 * np.arange(vocab // 4096)] = 8 + rng.random(vocab // 4096)
+    check_beam(ops, x, scores, n_beams, k)
+
+
+
 def test_beam_strided_rows(ops):
     """Rows that are part of wider ones, at every alignment."""
     rng = np.random.default_rng(2)
