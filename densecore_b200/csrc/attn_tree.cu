@@ -616,10 +616,16 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             int seg = 0, end = g.tiles;            // the segment's end among the range's units
             bool begins = true;                    // its Q not waited for yet
             uint64_t* q_empty = C.q_empty[b];
-            // S of unit n
+            // S of unit n.  Each MMA warp sees every segment's Q land, also where it has no unit of the segment: the
+            // parity that it waits for at the next Q in the same buffer is that of a barrier without a phase behind
+            // it as well, so a Q not waited for would leave the next one's wait without effect.
             auto issue_s = [&](int n, bool have_k) {
-                while (n >= end) {                 // (a segment that has no unit of this warp: given back at once)
-                    if (begins && leader) tc_commit(&q_empty[seg % q_bufs]);
+                while (n >= end) {
+                    if (begins) {                  // (no unit of this warp: given back at once)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&C.q_full[seg % q_bufs], (uint32_t)((seg / q_bufs) & 1), &g_tree_error));
+                        if (!ok) return;
+                        if (leader) tc_commit(&q_empty[seg % q_bufs]);
+                    }
                     seg_next<TW_ROWS, TW_KEYS>(a, g);
                     seg++;
                     end += g.tiles;
