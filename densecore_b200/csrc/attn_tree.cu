@@ -663,6 +663,10 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 __syncwarp();
             };
             if (b < N) issue_s(b, false);
+            // The second warp sees S of unit 0 too.  Its first poll below is for S of unit 2, and the parity of that
+            // phase is also that of a barrier which has ended none: unit 1 would go on, and the ring with it, while
+            // K of unit 0 were still on its way.
+            if (b && b < N && ok) ok = __all_sync(0xffffffffu, mbar_wait(&C.s_full[0], 0, &g_tree_error));
             for (int n = b; n < N && ok; n += 2) {  // O of unit n, then S of unit n + 2 into the same buffer
                 const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
                 // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit, others P.  (The third keeps the

@@ -46,3 +46,10 @@ def test_tree_ranges_that_begin_on_an_items_last_tile(ops, hq, hkv, most):  # no
     rng = np.random.default_rng(most + 1)
     ns = rng.integers(most // 2 + 1, most + 1, 130).tolist()
     repeat_tree(ops, rng, ns, [n + int(c) for n, c in zip(ns, rng.integers(129, 480, 130))], hq, hkv)
+
+
+@pytest.mark.parametrize("hq,hkv,nodes,seqs,ctx", [(16, 8, 12, 1, 30000), (16, 2, 16, 74, 500), (8, 1, 5, 140, 400)])
+def test_tree_first_units_of_a_range(ops, hq, hkv, nodes, seqs, ctx):  # noqa: F811
+    """Three to 13 units a range, the first of them from memory: the order of a CTA's first tiles."""
+    rng = np.random.default_rng(seqs)
+    repeat_tree(ops, rng, [nodes] * seqs, [ctx + int(c) for c in rng.integers(0, 100, seqs)], hq, hkv, times=40)
