@@ -248,9 +248,10 @@ __device__ bool read_part(const float* __restrict__ p, int64_t u0, int64_t u1, i
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         float r1 = s - 1.0f;               // the sum without the largest logit's own 1
-        if (s < 1.015625f || !(fabsf(me) < 1e38f)) {
-            // one logit far above the rest (lse - max would be lost next to 1), or me c overflows: the
-            // rest alone.  +inf makes it NaN, as a NaN does
+        if (!(s >= 1.015625f && fabsf(me) < 16777216.0f)) {
+            // one logit far above the rest (lse - max would be lost next to 1), or me so large that l, up to half a
+            // step of h (1 at |me| = 2^24, beyond 126 from 5 x 10^9 on), takes the two factors out of fp32's range:
+            // the rest alone, from v - me.  +inf makes it NaN, as a NaN does
             bool skip = lane == __ffs(__ballot_sync(0xffffffffu, mt == mw)) - 1;
             r1 = me == INFINITY ? NAN : 0.0f;
 #pragma unroll

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import branch_ref as R
-from test_branch_gpu import check_tree, dev, device_error, make_tree, ops, random_seen, run_tree  # noqa: F401
+from test_branch_gpu import check_beam, dev, device_error, make_tree, ops, random_seen  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,38 @@ def test_tree_first_units_of_a_range(ops, hq, hkv, nodes, seqs, ctx):  # noqa: F
     """Three to 13 units a range, the first of them from memory: the order of a CTA's first tiles."""
     rng = np.random.default_rng(seqs)
     repeat_tree(ops, rng, [nodes] * seqs, [ctx + int(c) for c in rng.integers(0, 100, seqs)], hq, hkv, times=40)
+
+
+# ------------------------------------------------------------------------------------------- beam
+# The bound of check_beam (2^-19.3 + 2^-22 + 8 2^-24 = 2.3 10^-6 of 2^-18 = 3.8 10^-6) holds at any offset M.  Up to
+# |M| = 2^24 the one factor more, 2^-l with |l| <= 1, is off by 2^-22, and l adds 2^-24 to the arguments' rounding: 0.3 10^-6.
+# From 2^24 on logits that differ do so by 1 at least, x - max is exact and the sums are those of the first case; from
+# 2^28 on (steps of 32) only equal logits count, whose sum is exact, and 64-bit lse and score are rounded by 2^-25 |M| 2^-28
+# at most on each side: 10^-6 at 2^33, beyond which log(vocab) itself is lost on both sides alike.
+@pytest.mark.parametrize("big", [2.0 ** 23, 16777214.0, 2.0 ** 24, 1e9, 5e9, 6e9, 1e10, 1e12, 1e20, 1e30, 9.9e37, 1.1e38, 3e38])
+@pytest.mark.parametrize("k", [4, 40])
+def test_beam_masked_and_offset_logits(ops, big, k):  # noqa: F811
+    """Logits masked with a large finite number (all but a few, whole tiles, the padding of a vocabulary),
+    and rows that lie around it."""
+    rng = np.random.default_rng(int(np.log2(big)))
+    x = (rng.standard_normal((8, 20011)) * 3).astype(np.float32)
+    x[0, rng.permutation(20011)[5:]] = -big
+    x[1, -267:] = -big
+    x[2, 4096:8192] = -big
+    x[3, 511:] = -big
+    x[4] += np.float32(big)
+    x[5] -= np.float32(big)
+    x[6, 1:] = -big
+    x[7] = np.float32(big) * (1 + rng.integers(0, 3, 20011).astype(np.float32) / 64) * (1 if big < 3e38 else 0.9)
+    scores = -rng.random(8).astype(np.float32) * 4
+    check_beam(ops, x, scores, 4, k)
+    check_beam(ops, x, scores, 1, k)
+    check_beam(ops, x, scores, 8, k)
+
+
+@pytest.mark.parametrize("big", [1e10, 1e20, 3.4028235e38])
+def test_beam_padded_vocabulary(ops, big):  # noqa: F811
+    rng = np.random.default_rng(13)
+    x = (rng.standard_normal((8, 151936)) * 3).astype(np.float32)
+    x[:, -267:] = -big
+    check_beam(ops, x, -rng.random(8).astype(np.float32) * 4, 4, 8)
