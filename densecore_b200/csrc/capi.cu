@@ -368,6 +368,10 @@ int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena
     return DCG_OK;
 }
 
+static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
 static int pages_common(const void* k_arena, const void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv,
                         int head_dim, int max_blocks_per_seq) {
     if (n_layer <= 0 || hkv <= 0 || head_dim <= 0 || n_arena_blocks <= 0 || max_blocks_per_seq <= 0)
@@ -423,8 +427,11 @@ int dcg_kv_compact(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_l
     if (rc) return rc;
     if (max_path <= 0 || max_path > dcg::kv_compact_max_path())
         return fail(DCG_EINVAL, "max_path must be in 1 .. " + std::to_string(dcg::kv_compact_max_path()));
-    if (ctx_lens < base_lens + n_seqs && base_lens < ctx_lens + n_seqs)
-        return fail(DCG_EINVAL, "ctx_lens must not overlap base_lens");
+    // one CTA of a row writes ctx_lens while others may still read the row
+    const size_t row = (size_t)n_seqs * sizeof(int32_t);
+    if (overlap(ctx_lens, row, base_lens, row) || overlap(ctx_lens, row, path_lens, row) || overlap(ctx_lens, row, path, row * max_path) ||
+        overlap(ctx_lens, row, block_tables, row * max_blocks_per_seq))
+        return fail(DCG_EINVAL, "ctx_lens must not overlap base_lens, path, path_lens or block_tables");
     DCG_CUDA(dcg::launch_kv_compact(k_arena, v_arena, n_arena_blocks, n_layer, (int64_t)hkv * head_dim * 2,
                                     block_tables, max_blocks_per_seq, base_lens, path, max_path, path_lens, n_seqs,
                                     ctx_lens, (cudaStream_t)stream), "kv_compact");

@@ -220,8 +220,9 @@ int dcg_kv_fork(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_laye
  * base_lens[s] + path_lens[s].  path [n_seqs][max_path] must ascend strictly within path_lens[s]
  * (ancestors are drafted before their descendants).  Blocks that are written must not be shared
  * with other rows (dcg_kv_fork gives every row its own last blocks); blocks past the new length stay
- * held until the next dcg_kv_fork.  ctx_lens must not overlap base_lens.  A row with a bad path,
- * length or block id is left as it was (DCG_DEVERR_INDEX).  max_path <= 1024, n_seqs <= 65535;
+ * held until the next dcg_kv_fork.  ctx_lens must not overlap base_lens, path, path_lens or
+ * block_tables.  A row with a bad path, length or block id is left as it was (DCG_DEVERR_INDEX).
+ * max_path <= 1024, n_seqs <= 65535;
  * hkv * head_dim a multiple of 8; arenas 16-B aligned. */
 int dcg_kv_compact(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv, int head_dim,
                    const int32_t* block_tables, int max_blocks_per_seq, const int32_t* base_lens,
