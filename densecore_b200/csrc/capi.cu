@@ -408,6 +408,12 @@ int dcg_kv_fork(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_laye
     const size_t need = dcg::kv_fork_scratch_bytes(n_seqs, max_blocks_per_seq, n_arena_blocks);
     if (scratch_bytes < need) return fail(DCG_ESCRATCH, "kv_fork scratch needs " + std::to_string(need) + " bytes");
     if (!aligned(scratch, 256)) return fail(DCG_EINVAL, "scratch must be 256-byte aligned");
+    // parents are read by every launch, reserve while the counts change
+    const size_t row = (size_t)n_seqs * sizeof(int32_t), counts = (size_t)n_arena_blocks * sizeof(int32_t);
+    if (overlap(parents, row, block_tables, row * max_blocks_per_seq) || overlap(parents, row, ctx_lens, row) || overlap(parents, row, n_pages, row) ||
+        overlap(parents, row, ref_counts, counts) || overlap(parents, row, status, sizeof(int32_t)))
+        return fail(DCG_EINVAL, "parents must not overlap block_tables, ctx_lens, n_pages, ref_counts or status");
+    if (reserve && overlap(reserve, row, ref_counts, counts)) return fail(DCG_EINVAL, "reserve must not overlap ref_counts");
     DCG_CUDA(dcg::launch_kv_fork(k_arena, v_arena, n_arena_blocks, n_layer, (int64_t)hkv * head_dim * 2, block_tables,
                                  max_blocks_per_seq, ctx_lens, n_pages, ref_counts, parents, reserve, n_seqs,
                                  fill_block, status, scratch, (cudaStream_t)stream), "kv_fork");

@@ -206,7 +206,8 @@ int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena
  * parents[i] = i for all i grows, and frees what lies past the lengths.  Entries of a row from its
  * new to its old n_pages are set to fill_block, which should hold a reference of its own.
  * *status (device) is 0; > 0: so many blocks were missing; < 0: a parent, length, block count or
- * block id was out of range.  In the last two cases nothing is changed.  n_seqs <= 4096;
+ * block id was out of range.  In the last two cases nothing is changed.  parents must not overlap an
+ * array that the call updates, reserve not ref_counts.  n_seqs <= 4096;
  * hkv * head_dim a multiple of 8; arenas 16-B aligned; scratch: dcg_kv_fork_scratch_size bytes,
  * 256-B aligned, not shared by calls that may overlap. */
 size_t dcg_kv_fork_scratch_size(int n_seqs, int max_blocks_per_seq, int64_t n_arena_blocks);
