@@ -468,6 +468,13 @@ int dcg_beam_select(const float* logits, int64_t ld, int n_groups, int n_beams, 
     if (scratch_bytes < need || !scratch)
         return fail(DCG_ESCRATCH, "beam_select scratch needs " + std::to_string(need) + " bytes");
     if (!aligned(scratch, 256)) return fail(DCG_EINVAL, "scratch must be 256-byte aligned");
+    // a group's CTA reads its beams' scores and flags before it writes its own k results
+    const size_t rows = (size_t)n_groups * n_beams, res = (size_t)n_groups * k * 4;
+    const bool in_place = (const float*)out_scores == scores && k == n_beams;
+    if ((overlap(scores, rows * 4, out_scores, res) && !in_place) || overlap(scores, rows * 4, out_rows, res) || overlap(scores, rows * 4, out_tokens, res))
+        return fail(DCG_EINVAL, "results must not overlap scores (out_scores may be scores itself when k = n_beams)");
+    if (finished && (overlap(finished, rows, out_scores, res) || overlap(finished, rows, out_rows, res) || overlap(finished, rows, out_tokens, res)))
+        return fail(DCG_EINVAL, "results must not overlap finished");
     DCG_CUDA(dcg::launch_beam_select(logits, ld, n_groups, n_beams, vocab, scores, finished, eos, k, out_scores,
                                      out_rows, out_tokens, scratch, (cudaStream_t)stream), "beam_select");
     return DCG_OK;

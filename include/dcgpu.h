@@ -237,7 +237,8 @@ int dcg_kv_compact(void* k_arena, void* v_arena, int64_t n_arena_blocks, int n_l
  * the lower row, in a row to the larger logit, then to the lower token.  A row with finished[row]
  * != 0 (finished may be NULL) offers one candidate, token eos at its own score.  -inf logits are no
  * candidates; a row whose score is not finite, or whose logits hold a NaN or +inf or are all -inf,
- * offers none.  Places without a candidate get score -inf, row -1 and token -1.  k <= 64;
+ * offers none.  Places without a candidate get score -inf, row -1 and token -1.  The results must not
+ * overlap scores or finished; out_scores may be scores itself when k = n_beams.  k <= 64;
  * n_beams <= 512; vocab <= 2^30; scratch: dcg_beam_select_scratch_size bytes, 256-B aligned, not shared by calls
  * that may overlap. */
 size_t dcg_beam_select_scratch_size(int n_groups, int n_beams, int64_t vocab, int k);

@@ -88,3 +88,14 @@ def test_beam_padded_vocabulary(ops, big):  # noqa: F811
     x = (rng.standard_normal((8, 151936)) * 3).astype(np.float32)
     x[:, -267:] = -big
     check_beam(ops, x, -rng.random(8).astype(np.float32) * 4, 4, 8)
+
+
+def test_beam_scores_in_place(ops):  # noqa: F811
+    """out_scores may be scores itself when there are as many results as beams."""
+    rng = np.random.default_rng(14)
+    x = dev((rng.standard_normal((40, 9001)) * 3).astype(np.float32))
+    scores = dev(-rng.random(40).astype(np.float32) * 4)
+    want = ops.beam_select(x, scores, 4, 4)
+    out = (scores, torch.empty_like(want[1]), torch.empty_like(want[2]))
+    ops.beam_select(x, scores, 4, 4, out=out)
+    assert torch.equal(scores.view(10, 4), want[0]) and torch.equal(out[1], want[1]) and torch.equal(out[2], want[2])
