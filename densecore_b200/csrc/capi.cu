@@ -326,6 +326,10 @@ int dcg_paged_attn_prefill(const float* q, const void* k_arena, const void* v_ar
     return DCG_OK;
 }
 
+static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
 size_t dcg_paged_attn_tree_scratch_size(int n_seqs, int hq, int hkv, int head_dim, int max_seq_tokens, int max_ctx) {
     if (n_seqs <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || head_dim != 128 || max_seq_tokens <= 0 || max_ctx < 0) return 0;
     return dcg::tree_scratch_bytes(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
@@ -357,6 +361,9 @@ int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena
         return fail(DCG_EINVAL, "max_seq_tokens * hq * max_ctx too large");
     if (!aligned(k_arena, 16) || !aligned(v_arena, 16) || !aligned(q, 16) || !aligned(out, 16) || !aligned(tree_mask, 8))
         return fail(DCG_EINVAL, "q, out and the arenas must be 16-byte aligned, tree_mask 8-byte");
+    // (token, head) rows are read by the CTA that writes them, or by an earlier launch: out may be q, but not lie across it
+    const size_t rows_bytes = (size_t)n_tok * hq * head_dim * sizeof(float);
+    if (out != q && overlap(out, rows_bytes, q, rows_bytes)) return fail(DCG_EINVAL, "out must be q itself or not overlap it");
     const size_t need = dcg::tree_scratch_bytes(n_seqs, hq, hkv, max_seq_tokens, max_ctx);
     if (scratch_bytes < need || (need && !scratch))
         return fail(DCG_ESCRATCH, "tree attention scratch needs " + std::to_string(need) + " bytes");
@@ -366,10 +373,6 @@ int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena
                                          n_seqs, max_seq_tokens, hq, hkv, max_ctx, scale, out, scratch,
                                          (cudaStream_t)stream), "paged_attn_tree");
     return DCG_OK;
-}
-
-static bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
 }
 
 static int pages_common(const void* k_arena, const void* v_arena, int64_t n_arena_blocks, int n_layer, int hkv,

@@ -184,7 +184,8 @@ int dcg_paged_attn_prefill(const float* q, const void* k_arena, const void* v_ar
  * other; slots at and past ctx_lens[s] may hold anything.  Rows of q outside all sequences are
  * neither read nor written.  Each n_s must be <= max_seq_tokens and <= 64 * mask_words, each
  * ctx_lens[s] in [n_s, max_ctx] (else the sequence's rows are left as they were, DCG_DEVERR_INDEX).
- * hq / hkv: any whole number.  n_seqs and hq < 65535.  head_dim must be 128.  scratch:
+ * hq / hkv: any whole number.  n_seqs and hq < 65535.  head_dim must be 128.  out may be q itself, but
+ * must not overlap it otherwise.  scratch:
  * dcg_paged_attn_tree_scratch_size bytes, 256-B aligned, not shared by calls that may overlap. */
 size_t dcg_paged_attn_tree_scratch_size(int n_seqs, int hq, int hkv, int head_dim, int max_seq_tokens, int max_ctx);
 int dcg_paged_attn_tree(const float* q, const void* k_arena, const void* v_arena, int64_t n_arena_blocks,

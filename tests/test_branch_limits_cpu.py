@@ -2,7 +2,7 @@
 import pytest
 
 from densecore_b200 import _lib
-from test_branch_cpu import EINVAL, P, beam, compact, fork
+from test_branch_cpu import EINVAL, P, beam, compact, fork, tree
 
 
 # base_lens, path_lens 8 bytes, path and block_tables 32 at P
@@ -30,4 +30,10 @@ def test_fork_refuses_parents_that_it_would_write(kw):
 def test_beam_refuses_results_over_what_it_reads(kw):
     apart = dict(scores=2 * P, finished=3 * P, s=4 * P, r=5 * P, t=6 * P)
     assert beam(**{**apart, **kw}) == EINVAL
+    assert b"overlap" in _lib.load().dcg_last_error()
+
+
+@pytest.mark.parametrize("off", [16, -16, 4 * 16 * 512 - 16])      # 4 tokens of 16 heads
+def test_tree_refuses_an_output_across_q(off):
+    assert tree(q=1 << 20, out=(1 << 20) + off) == EINVAL
     assert b"overlap" in _lib.load().dcg_last_error()

@@ -55,6 +55,22 @@ def test_tree_first_units_of_a_range(ops, hq, hkv, nodes, seqs, ctx):  # noqa: F
     repeat_tree(ops, rng, [nodes] * seqs, [ctx + int(c) for c in rng.integers(0, 100, seqs)], hq, hkv, times=40)
 
 
+@pytest.mark.parametrize("hq,hkv,ns,ctx", [(16, 8, [5, 8, 1], [60, 200, 30]), (16, 8, [5, 8], [2000, 700]), (32, 8, [12, 3], [900, 77]),
+                                           (32, 4, [40, 9, 40], [300, 64, 1000])])
+def test_tree_in_place(ops, hq, hkv, ns, ctx):  # noqa: F811
+    """out = q, in every form of the kernel: bit for bit what it is in a buffer of its own."""
+    rng = np.random.default_rng(hq + ns[0])
+    ka, va, bt, starts, q = make_tree(rng, ns, ctx, hq, hkv, 1)
+    mask, _ = random_seen(rng, ns)
+    a = [dev(x) for x in (ka, va, bt, starts, np.array(ctx, np.int32), mask)]
+    x = dev(q)
+    want = ops.paged_attn_tree(x, a[0], a[1], 1, 0, *a[2:], hkv, max(ns), max(ctx))
+    for _ in range(5):
+        y = x.clone()
+        assert ops.paged_attn_tree(y, a[0], a[1], 1, 0, *a[2:], hkv, max(ns), max(ctx), out=y) is y
+        assert torch.equal(y, want)
+
+
 # ------------------------------------------------------------------------------------------- beam
 # The bound of check_beam (2^-19.3 + 2^-22 + 8 2^-24 = 2.3 10^-6 of 2^-18 = 3.8 10^-6) holds at any offset M.  Up to
 # |M| = 2^24 the one factor more, 2^-l with |l| <= 1, is off by 2^-22, and l adds 2^-24 to the arguments' rounding: 0.3 10^-6.
