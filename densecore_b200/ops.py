@@ -309,6 +309,9 @@ def paged_attn_tree(q: torch.Tensor, k_arena: torch.Tensor, v_arena: torch.Tenso
         raise ValueError("seq_starts needs one entry more than block_tables has rows, ctx_lens as many")
     if words[0] != n_tok:
         raise ValueError("tree_mask needs a row for each row of q")
+    for arena in (k_arena.shape, v_arena.shape):   # another form than dcg_kv_fork's is taken by its size
+        if len(arena) == 4 and arena[1] == 16 and (arena[2] != hkv or arena[3] != hd):
+            raise ValueError(f"arenas of {arena[2]} kv heads x {arena[3]}, called with {hkv} x {hd}")
     per_block = 16 * hkv * hd * n_layer
     elements = k_arena.numel()
     if per_block <= 0 or elements % per_block or v_arena.numel() != elements:

@@ -71,6 +71,22 @@ def test_tree_in_place(ops, hq, hkv, ns, ctx):  # noqa: F811
         assert torch.equal(y, want)
 
 
+def test_tree_refuses_another_head_layout(ops):  # noqa: F811
+    """kv heads or a head size that the arenas do not have, although the sizes divide."""
+    h = torch.zeros((4, 16, 8, 128), dtype=torch.float16, device="cuda")
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    m = torch.zeros((1, 1), dtype=torch.int64, device="cuda")
+    q = torch.zeros((1, 8, 128), device="cuda")
+
+    def call(k, v, hkv, q=q):
+        return ops.paged_attn_tree(q, k, v, 1, 0, i(1, 4), i(2), i(1), m, hkv, 1, 16)
+    for k, v, hkv in ((h, h, 4), (h, h, 1), (h.view(8, 16, 4, 128), h, 4), (h, h.view(2, 16, 16, 128), 8), (h.view(4, 16, 16, 64), h, 8)):
+        with pytest.raises(ValueError, match="kv heads"):
+            call(k, v, hkv)
+    call(h, h, 8)
+    call(h.flatten(), h.view(64, 8, 128), 8)     # another form of the same layout
+
+
 # ------------------------------------------------------------------------------------------- beam
 # The bound of check_beam (2^-19.3 + 2^-22 + 8 2^-24 = 2.3 10^-6 of 2^-18 = 3.8 10^-6) holds at any offset M.  Up to
 # |M| = 2^24 the one factor more, 2^-l with |l| <= 1, is off by 2^-22, and l adds 2^-24 to the arguments' rounding: 0.3 10^-6.
