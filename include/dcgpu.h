@@ -181,7 +181,10 @@ int dcg_paged_attn_prefill(const float* q, const void* k_arena, const void* v_ar
  * drafted token t of its own sequence when bit t % 64 of tree_mask[i * mask_words + t / 64] is set
  * (i: row of q).  A token that sees no key gets zeros.  K may hold anything in slots that no token
  * sees; a non-finite V of a drafted token makes NaN of the rows (token, head) that see it and of no
- * other; slots at and past ctx_lens[s] may hold anything.  Rows of q outside all sequences are
+ * other; slots at and past ctx_lens[s] may hold anything.  Q and the weights enter the products as two
+ * fp16 halves, and a half that is 0 makes NaN of an infinity: a row that sees a non-finite K, or a
+ * non-finite V of the history, is NaN or what the formula gives, rows that do not see it are what
+ * they are without it.  Rows of q outside all sequences are
  * neither read nor written.  Each n_s must be <= max_seq_tokens and <= 64 * mask_words, each
  * ctx_lens[s] in [n_s, max_ctx] (else the sequence's rows are left as they were, DCG_DEVERR_INDEX).
  * hq / hkv: any whole number.  n_seqs and hq < 65535.  head_dim must be 128.  out may be q itself, but

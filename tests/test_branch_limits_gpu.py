@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import branch_ref as R
-from test_branch_gpu import check_beam, dev, device_error, make_tree, ops, random_seen  # noqa: F401
+from test_branch_gpu import check_beam, dev, device_error, make_tree, ops, random_seen, run_tree  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -85,6 +85,31 @@ def test_tree_refuses_another_head_layout(ops):  # noqa: F811
             call(k, v, hkv)
     call(h, h, 8)
     call(h.flatten(), h.view(64, 8, 128), 8)     # another form of the same layout
+
+
+@pytest.mark.parametrize("hq,hkv,nodes", [(8, 2, 3), (8, 2, 7), (8, 2, 12), (16, 2, 12), (32, 2, 30)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_tree_infinities_stay_with_the_rows_that_see_them(ops, hq, hkv, nodes, bad):  # noqa: F811
+    """Infinities in K and V of the history reach the rows of their kv head and sequence, one in a drafted K the
+    rows that see it; all others are right, in every form of the kernel."""
+    rng = np.random.default_rng(nodes)
+    ns, ctx = [nodes] * 4, [nodes + 300, nodes + 40, nodes + 140, nodes + 260]
+    ka, va, bt, starts, q = make_tree(rng, ns, ctx, hq, hkv, 1)
+    mask, seen = random_seen(rng, ns)
+    k0, v0 = ka.copy(), va.copy()
+    ka[bt[0, 3], 5, 1, 17] = bad                 # history of sequence 0, kv head 1
+    va[bt[2, 0], 2, 0, 99] = bad                 # history of sequence 2, kv head 0
+    p = ctx[3] - nodes + 1                       # drafted token 1 of sequence 3, kv head 0
+    ka[bt[3, p // 16], p % 16, 0, 3] = bad
+    out = run_tree(ops, q, ka, va, 1, 0, bt, starts, ctx, mask, hkv, nodes).cpu().numpy()
+    ref, tol = R.tree_attention(q, k0, v0, 1, 0, bt, starts, ctx, seen, hkv, 128 ** -0.5)
+    half, checked = hq // 2, 0
+    for i in range(len(q)):
+        s = i // nodes
+        heads = slice(0, half) if s == 0 else slice(half, hq) if s == 2 or (s == 3 and 1 in seen[i]) else slice(0, hq)
+        assert (np.abs(out[i, heads] - ref[i, heads]) <= tol[i, heads]).all()
+        checked += s == 3 and heads == slice(0, hq)
+    assert checked and device_error() == 0
 
 
 # ------------------------------------------------------------------------------------------- beam
