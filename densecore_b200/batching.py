@@ -177,7 +177,7 @@ class PagePool:
         self.refs[0] = 1
         self.tables.zero_()
         self.identity = torch.arange(dec.batch, dtype=i32, device=dev)
-        self.short = torch.zeros((), dtype=i32, device=dev)             # worst status so far (0: all went well)
+        self.short = torch.zeros((), dtype=i32, device=dev)             # first status that was not 0
         self._status = torch.zeros((), dtype=i32, device=dev)
         self._scratch = torch.empty(ops.kv_fork_scratch_size(dec.batch, self.tables.shape[1], dec.n_blocks),
                                     dtype=torch.uint8, device=dev)
@@ -188,7 +188,7 @@ class PagePool:
         ops.kv_fork(d.k_arena, d.v_arena, d.cfg.n_layer, self.tables, self.lens, self.pages, self.refs,
                     self.identity if parents is None else parents, reserve=reserve, fill_page=0,
                     status=self._status, scratch=self._scratch)
-        self.short = torch.maximum(self.short, self._status.abs())
+        self.short = torch.where(self.short == 0, self._status, self.short)
 
     def compact(self, base: torch.Tensor, path: torch.Tensor, path_lens: torch.Tensor):
         """Keep the accepted branches: base tokens before the draft, path in drafted tokens."""
@@ -196,8 +196,11 @@ class PagePool:
         ops.kv_compact(d.k_arena, d.v_arena, d.cfg.n_layer, self.tables, base, path, path_lens, self.lens)
 
     def check(self):
-        """Raise if a fork so far found too few blocks (it then changed nothing)."""
+        """Raise if a fork so far found too few blocks or bad input (it then changed nothing): what the
+        first such fork said."""
         n = int(self.short)
+        if n < 0:
+            raise ValueError("a fork met a parent, length or block that is out of range")
         if n:
             raise MemoryError(f"the KV arena is {n} blocks short")
 
