@@ -12,7 +12,8 @@ point at one reserved block and run a harmless one-token step.
 
 Sequences that branch: BeamSearcher (beam search over groups of decoder rows) and TreeSpeculator
 (greedy decoding that scores drafted token trees) keep the blocks on the device, shared between rows
-and counted (PagePool).  Each takes the whole decoder's cache while it runs.
+and counted (PagePool).  Each takes the whole decoder's cache while it runs: what the cache held is
+gone afterwards, the decoder's block table is as it was.
 """
 from __future__ import annotations
 
@@ -165,7 +166,8 @@ class PagePool:
     """The decoder's KV blocks as pages shared between rows, kept on the device: the block table, how
     many tokens and blocks each row holds, and how often each block is held.  fork and compact are
     kv_fork and kv_compact on all rows at once; block 0 is the idle block that unused entries point
-    at.  Nothing waits for the host except `check`."""
+    at.  Nothing waits for the host except `check`.  The table is the decoder's own; `close` (or the end
+    of a with block) puts back what it held before."""
 
     def __init__(self, dec: Decoder):
         self.dec = dec
@@ -175,12 +177,23 @@ class PagePool:
         self.pages = torch.zeros(dec.batch, dtype=i32, device=dev)
         self.refs = torch.zeros(dec.n_blocks, dtype=i32, device=dev)
         self.refs[0] = 1
+        self._before = self.tables.clone()
         self.tables.zero_()
         self.identity = torch.arange(dec.batch, dtype=i32, device=dev)
         self.short = torch.zeros((), dtype=i32, device=dev)             # first status that was not 0
         self._status = torch.zeros((), dtype=i32, device=dev)
         self._scratch = torch.empty(ops.kv_fork_scratch_size(dec.batch, self.tables.shape[1], dec.n_blocks),
                                     dtype=torch.uint8, device=dev)
+
+    def close(self):
+        """Give the decoder its block table back; the pool is not used after it."""
+        self.tables.copy_(self._before)
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
 
     def fork(self, parents: torch.Tensor | None = None, reserve: torch.Tensor | None = None):
         """Rows become children of `parents` (default: themselves) with room for `reserve` more tokens."""
@@ -220,12 +233,17 @@ class BeamSearcher:
         sum of the tokens' log-probabilities; a continuation ends at eos (included) or max_new tokens.
         Fewer, if the logits allow fewer."""
         dec, nb = self.dec, self.n_beams
-        G, B, dev, i32 = len(prompts), dec.batch, dec.device, torch.int32
+        G, B = len(prompts), dec.batch
         if not 0 < G <= B // nb:
             raise ValueError(f"1 to {B // nb} prompts fit")
         if max_new < 1 or any(not p or len(p) + max_new > dec.max_ctx for p in prompts):
             raise ValueError(f"need non-empty prompts, max_new >= 1 and at most {dec.max_ctx} positions")
-        pool = PagePool(dec)
+        with PagePool(dec) as pool:
+            return self._search(pool, prompts, max_new)
+
+    def _search(self, pool, prompts, max_new):
+        dec, nb = self.dec, self.n_beams
+        G, B, dev, i32 = len(prompts), dec.batch, dec.device, torch.int32
         first = torch.arange(G, dtype=i32, device=dev) * nb
         room = torch.zeros(B, dtype=i32, device=dev)
         room[first.long()] = torch.tensor([len(p) for p in prompts], dtype=i32, device=dev)
@@ -333,13 +351,17 @@ class TreeSpeculator:
     def generate(self, prompts, max_new: int, eos: int | None = None):
         """The greedy continuation of each prompt (at most max_new tokens, up to eos included)."""
         dec = self.dec
-        B, dev, i32 = dec.batch, dec.device, torch.int32
-        n = len(prompts)
+        n, B = len(prompts), dec.batch
         if not 0 < n <= B:
             raise ValueError(f"1 to {B} prompts fit")
         if max_new < 1 or any(not p or len(p) + max_new > dec.max_ctx for p in prompts):
             raise ValueError(f"need non-empty prompts, max_new >= 1 and at most {dec.max_ctx} positions")
-        pool = PagePool(dec)
+        with PagePool(dec) as pool:
+            return self._generate(pool, prompts, max_new, eos)
+
+    def _generate(self, pool, prompts, max_new, eos):
+        dec, n = self.dec, len(prompts)
+        B, dev, i32 = dec.batch, dec.device, torch.int32
 
         def per_row(values):
             return torch.tensor(list(values) + [0] * (B - n), dtype=i32).to(dev)

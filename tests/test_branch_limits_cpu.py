@@ -137,3 +137,21 @@ def test_pool_tells_bad_input_from_too_few_blocks(on_cpu):
     pool.fork(i32(5, 0))                     # the first thing that went wrong is what is told
     with pytest.raises(MemoryError, match="3 blocks"):
         pool.check()
+
+
+def test_pool_gives_the_table_back(on_cpu):
+    dec = FakeDecoder(2, 64)
+    before = dec.block_tables.clone()
+    prompts = [[1, 2, 3] * 7, [4] * 18]
+    assert batching.TreeSpeculator(dec).generate(prompts, 20) == [greedy(p, 20) for p in prompts]
+    assert torch.equal(dec.block_tables, before)
+    with batching.PagePool(dec) as pool:
+        pool.fork(reserve=torch.full((2,), 17, dtype=torch.int32))
+        assert not torch.equal(dec.block_tables, before)
+    assert torch.equal(dec.block_tables, before)
+
+    def broken(history):
+        raise RuntimeError("no draft")
+    with pytest.raises(RuntimeError):
+        batching.TreeSpeculator(dec, broken).generate(prompts, 20)
+    assert torch.equal(dec.block_tables, before)

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import branch_ref as R
+from test_branching_gpu import greedy, make
 from test_branch_gpu import check_beam, dev, device_error, make_tree, ops, random_seen, run_tree  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -156,3 +157,24 @@ def test_beam_scores_in_place(ops):  # noqa: F811
     out = (scores, torch.empty_like(want[1]), torch.empty_like(want[2]))
     ops.beam_select(x, scores, 4, 4, out=out)
     assert torch.equal(scores.view(10, 4), want[0]) and torch.equal(out[1], want[1]) and torch.equal(out[2], want[2])
+
+
+# ---------------------------------------------------------------------------------- the decode loops
+@pytest.mark.parametrize("loop", ["speculator", "beams"])
+def test_loops_give_the_decoder_back(loop):
+    """A decoder that a loop has used serves direct calls as one that it has not."""
+    from densecore_b200.batching import BeamSearcher, TreeSpeculator
+    used, fresh = make("q8_0", 4, 96), make("q8_0", 4, 96)
+    prompts = [[7, 300, 11] * 6, [42] * 5]
+    if loop == "speculator":
+        TreeSpeculator(used).generate(prompts, 20)
+    else:
+        BeamSearcher(used, 2).search(prompts, 20)
+    assert torch.equal(used.block_tables, fresh.block_tables)
+    texts = [[int(t) for t in np.random.default_rng(i).integers(0, 400, 20 + i)] for i in range(4)]
+    for d in (used, fresh):
+        nxt, d.seen = d.prefill(range(4), texts)
+        d.tokens.copy_(nxt)
+        d.ctx_lens.copy_(torch.tensor([len(t) + 1 for t in texts], dtype=torch.int32))
+        d.replay()
+    assert torch.equal(used.seen, fresh.seen) and torch.equal(used.logits, fresh.logits)
