@@ -97,7 +97,9 @@ class Decoder:
         all-gather of the logits over tp_group (NCCL).  shard_init = "slice": every rank draws the
         full random weights and keeps its slice (bitwise the tp_size = 1 model); "local": each rank
         draws only its shard (faster; a different random model).  seq_tokens: per-sequence token
-        capacity; the arena then holds exactly those blocks (default: max_ctx for every sequence).
+        capacity; the arena then holds exactly those blocks (default: max_ctx for every sequence), and
+        one more that no table row starts with: whoever hands out blocks needs an idle one, and the
+        sequences still get all of their own (batching.py).
         weights: GGUF-named tensors (gguf_file.decoder_weights) instead of random ones."""
         self.cfg, self.batch, self.max_ctx = cfg, batch, max_ctx
         self.tp_rank, self.tp_size, self.tp_group = tp_rank, tp_size, tp_group
@@ -283,12 +285,14 @@ class Decoder:
             nblk = [self.blocks_per_seq] * batch
         else:
             nblk = [(int(t) + KV_BLOCK - 1) // KV_BLOCK for t in seq_tokens]
-        self.n_blocks = sum(nblk)
+        self.n_blocks = sum(nblk) + 1
         shape = (self.n_blocks * cfg.n_layer, KV_BLOCK, self.hkv, D)
         self.k_arena = torch.empty(shape, dtype=torch.float16, device=dev)
         self.v_arena = torch.empty(shape, dtype=torch.float16, device=dev)
-        # each sequence owns a shuffled set of physical blocks
-        perm = torch.randperm(self.n_blocks, generator=torch.Generator().manual_seed(self.seed + 1))
+        for arena in (self.k_arena, self.v_arena):
+            arena[-cfg.n_layer:].zero_()
+        # each sequence owns a shuffled set of physical blocks (all but the last)
+        perm = torch.randperm(self.n_blocks - 1, generator=torch.Generator().manual_seed(self.seed + 1))
         bt = torch.zeros((batch, self.blocks_per_seq), dtype=torch.int32)
         o = 0
         for i, nb in enumerate(nblk):
@@ -637,8 +641,8 @@ class Decoder:
         """Seeded random history for every slot (stands in for prefill when timing decode)."""
         g = torch.Generator(device=self.device)
         g.manual_seed(seed)
-        self.k_arena.normal_(0.0, 1.0, generator=g)
-        self.v_arena.normal_(0.0, 1.0, generator=g)
+        for arena in (self.k_arena, self.v_arena):
+            arena[:-self.cfg.n_layer].normal_(0.0, 1.0, generator=g)
 
     # bytes one decode step must read at least (weights + KV history), for the roofline
     def step_bytes(self, ctx_lens) -> int:

@@ -178,3 +178,34 @@ def test_loops_give_the_decoder_back(loop):
         d.ctx_lens.copy_(torch.tensor([len(t) + 1 for t in texts], dtype=torch.int32))
         d.replay()
     assert torch.equal(used.seen, fresh.seen) and torch.equal(used.logits, fresh.logits)
+
+
+def test_full_caches():
+    """Requests that fill the decoder's cache to its last slot, in every loop that hands out blocks."""
+    from densecore_b200.batching import BeamSearcher, ContinuousBatcher, TreeSpeculator
+    prompts = [[7, 300, 11, 5] * 10, [42, 43] * 20]
+    want = greedy("q8_0", prompts, 24)
+    assert TreeSpeculator(make("q8_0", 2, 64)).generate(prompts, 24) == want
+    b = ContinuousBatcher(make("q8_0", 2, 64))
+    hs = [b.submit(p, 24) for p in prompts]
+    b.run(200)
+    assert [h.out for h in hs] == want and len(b.alloc.free) == b.alloc.n_blocks - 1
+    assert [x[0][1] for x in BeamSearcher(make("q8_0", 2, 64), 1).search(prompts, 24)] == want
+    # four beams that have nothing but their first token in common
+    beams = BeamSearcher(make("q8_0", 4, 48), 4).search([[300]], 47)[0]
+    assert len(beams) == 4 and len({tuple(t) for _, t in beams}) == 4 and all(len(t) == 47 for _, t in beams)
+
+
+def test_decoder_tables_and_history_with_the_idle_block():
+    """The idle block lies behind the sequences' own: no table row starts with it, and the random history of
+    the others is the one that a seed gives an arena of their size."""
+    dec = make("q8_0", 2, 40, seq_tokens=[40, 17])
+    assert dec.n_blocks == 3 + 2 + 1 and dec.k_arena.shape[0] == dec.n_blocks * dec.cfg.n_layer
+    held = dec.block_tables.cpu()
+    assert sorted(held[0].tolist() + held[1, :2].tolist()) == list(range(5))
+    dec.fill_kv_random(3)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    for arena in (dec.k_arena, dec.v_arena):
+        own = arena[:5 * dec.cfg.n_layer]
+        assert torch.equal(own, torch.empty_like(own).normal_(0.0, 1.0, generator=g)) and not arena[5 * dec.cfg.n_layer:].any()
