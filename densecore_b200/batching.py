@@ -363,8 +363,11 @@ class TreeSpeculator:
         dec, n = self.dec, len(prompts)
         B, dev, i32 = dec.batch, dec.device, torch.int32
 
-        def per_row(values):
-            return torch.tensor(list(values) + [0] * (B - n), dtype=i32).to(dev)
+        def per_row(values, other=0):
+            return torch.tensor(list(values) + [other] * (B - n), dtype=i32).to(dev)
+
+        def blocks(tokens):
+            return -(-tokens // KV_BLOCK)
 
         pool.fork(reserve=per_row(len(p) for p in prompts))
         pool.check()
@@ -380,19 +383,34 @@ class TreeSpeculator:
             live = [i for i in range(n) if not done(i)]
             if not live:
                 return out
-            trees = {}
+            # No row shares blocks, so the host knows how many are free once the finished rows have given theirs
+            # back.  Every row's known token comes first (a row without a block for it waits for others to finish),
+            # the drafts share what is left.
+            free = dec.n_blocks - 1 - sum(blocks(cached[i]) for i in live)
+            going = []
             for i in live:
+                need = blocks(cached[i] + 1) - blocks(cached[i])
+                if need <= free:
+                    going.append(i)
+                    free -= need
+            if not going:
+                raise MemoryError(f"no block of the KV arena is free for any of {len(live)} sequences")
+            trees = {}
+            for i in going:
                 t, p = self.draft(list(prompts[i]) + out[i])
                 # token 0 is the one just chosen; every drafted token takes a slot of the cache
-                room = min(self.max_nodes, dec.max_ctx - cached[i]) - 1
+                least = blocks(cached[i] + 1)
+                room = min(self.max_nodes, dec.max_ctx - cached[i], (least + free) * KV_BLOCK - cached[i]) - 1
                 trees[i] = ([out[i][-1]] + list(t)[:room], [-1] + [q + 1 for q in list(p)[:room]])
-            pool.fork(reserve=per_row(len(trees[i][0]) if i in trees else 0 for i in range(n)))
+                free -= blocks(cached[i] + len(trees[i][0])) - least
+            pool.fork(per_row((i if i in live else -1 for i in range(n)), -1),
+                      reserve=per_row(len(trees[i][0]) if i in trees else 0 for i in range(n)))
             pool.check()
-            greedy, _ = dec.verify_tree(live, [trees[i] for i in live], [cached[i] for i in live])
+            greedy, _ = dec.verify_tree(going, [trees[i] for i in going], [cached[i] for i in going])
             greedy = greedy.tolist()
             paths, at = [[] for _ in range(n)], 0
-            base = list(cached)
-            for i in live:
+            base = [cached[i] if i in live else 0 for i in range(n)]
+            for i in going:
                 t, p = trees[i]
                 g = greedy[at:at + len(t)]
                 at += len(t)

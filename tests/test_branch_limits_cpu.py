@@ -1,4 +1,5 @@
 """Further refusals and host logic of the branching operators, decided without a GPU."""
+import random
 import types
 
 import pytest
@@ -155,3 +156,59 @@ def test_pool_gives_the_table_back(on_cpu):
     with pytest.raises(RuntimeError):
         batching.TreeSpeculator(dec, broken).generate(prompts, 20)
     assert torch.equal(dec.block_tables, before)
+
+
+def wild(history):
+    """Forty guesses, nearly all of them wrong."""
+    rng = random.Random(len(history))
+    return [rng.randrange(VOCAB) for _ in range(40)], [rng.randrange(-1, i) if i else -1 for i in range(40)]
+
+
+class Watched(batching.PagePool):
+    """A pool that looks at its books after every fork: what a row holds is what it needs, every block's count is
+    the number of rows that hold it."""
+
+    forks = 0
+
+    def fork(self, parents=None, reserve=None):
+        super().fork(parents, reserve)
+        type(self).forks += 1
+        room = self.lens + (reserve if reserve is not None else 0)
+        assert torch.equal(self.pages, torch.where(self.lens + (parents if parents is not None else 0) < 0, 0, -(-room // 16)))
+        held = [0] * self.dec.n_blocks
+        held[0] = 1
+        for row, n in zip(self.tables.tolist(), self.pages.tolist()):
+            for b in row[:n]:
+                held[b] += 1
+        assert self.refs.tolist() == held and max(held) == 1
+
+
+@pytest.mark.parametrize("draft", [wild, batching.ngram_draft])
+def test_speculator_in_a_tight_arena(on_cpu, monkeypatch, draft):
+    """Drafts never take a block that the text needs: an arena that holds the finished texts is enough."""
+    monkeypatch.setattr(batching, "PagePool", Watched)
+    prompts = [[1] * 30, [2] * 30, [3] * 7]
+    need = sum(-(-(len(p) + 34) // 16) for p in prompts)      # the last token is not in the cache
+    dec = FakeDecoder(4, 96, need + 1)
+    assert batching.TreeSpeculator(dec, draft).generate(prompts, 35) == [greedy(p, 35) for p in prompts]
+    # one block short of that: nothing is lost if a text ends early enough, and another waits for it
+    eos = greedy(prompts[0], 35)[3]
+    want = [greedy(p, 35, eos) for p in prompts]
+    assert len(want[0]) == 4 and batching.TreeSpeculator(FakeDecoder(4, 96, need), draft).generate(prompts, 35, eos) == want
+    before = dec.block_tables.clone()
+    with pytest.raises(MemoryError):
+        batching.TreeSpeculator(FakeDecoder(1, 96, 4), draft).generate([[1] * 30], 35)
+    assert torch.equal(dec.block_tables, before) and Watched.forks
+
+
+def test_speculator_rows_wait_for_blocks(on_cpu, monkeypatch):
+    """Two texts that do not fit side by side: the second goes on when the first has ended."""
+    monkeypatch.setattr(batching, "PagePool", Watched)
+    eos = greedy([1] * 15, 17)[16]
+    long = next([t] * 32 for t in range(VOCAB) if eos not in greedy([t] * 32, 40))
+    prompts = [[1] * 15, long]
+    want = [greedy(p, 40, eos) for p in prompts]
+    assert len(want[0]) == 17 and len(want[1]) == 40
+    # idle, two blocks each, one more for the second
+    for n_blocks in (5, 6):
+        assert batching.TreeSpeculator(FakeDecoder(2, 96, n_blocks + 1), wild).generate(prompts, 40, eos) == want

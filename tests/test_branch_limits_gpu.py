@@ -209,3 +209,17 @@ def test_decoder_tables_and_history_with_the_idle_block():
     for arena in (dec.k_arena, dec.v_arena):
         own = arena[:5 * dec.cfg.n_layer]
         assert torch.equal(own, torch.empty_like(own).normal_(0.0, 1.0, generator=g)) and not arena[5 * dec.cfg.n_layer:].any()
+
+
+def test_speculator_in_a_tight_arena():
+    """An arena that holds the finished texts is enough, whatever is drafted."""
+    from densecore_b200.batching import TreeSpeculator
+    rng = np.random.default_rng(0)
+
+    def wild(history):
+        return [int(x) for x in rng.integers(0, 400, 40)], [int(rng.integers(-1, i)) if i else -1 for i in range(40)]
+    prompts = [[7, 300, 11] * 5, [42] * 17, [500, 1, 2]]
+    dec = make("q8_0", 3, 96, seq_tokens=[len(p) + 29 for p in prompts])
+    spec = TreeSpeculator(dec, wild)
+    assert spec.generate(prompts, 30) == greedy("q8_0", prompts, 30)
+    assert device_error() == 0
