@@ -201,6 +201,24 @@ def test_speculator_in_a_tight_arena(on_cpu, monkeypatch, draft):
     assert torch.equal(dec.block_tables, before) and Watched.forks
 
 
+def test_speculator_gives_every_block_back(on_cpu, monkeypatch):
+    """Rejected drafts, rows that end at different times and at eos: no block stays held."""
+    pools = []
+
+    class Kept(Watched):
+        def close(self):
+            self.fork(torch.full((self.dec.batch,), -1, dtype=torch.int32))
+            pools.append(self.refs.tolist())
+            super().close()
+    monkeypatch.setattr(batching, "PagePool", Kept)
+    prompts = [[7, 8, 9], [5] * 40, [6] * 16]
+    eos = greedy(prompts[2], 30)[11]
+    for e in (None, eos):
+        dec = FakeDecoder(4, 96)
+        assert batching.TreeSpeculator(dec, wild).generate(prompts, 30, e) == [greedy(p, 30, e) for p in prompts]
+    assert pools == [[1] + [0] * (dec.n_blocks - 1)] * 2
+
+
 def test_speculator_rows_wait_for_blocks(on_cpu, monkeypatch):
     """Two texts that do not fit side by side: the second goes on when the first has ended."""
     monkeypatch.setattr(batching, "PagePool", Watched)
