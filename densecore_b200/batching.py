@@ -23,7 +23,7 @@ import dataclasses
 import torch
 
 from . import ops
-from .decoder import KV_BLOCK, Decoder
+from .decoder import KV_BLOCK, Decoder, check_tokens
 
 
 class BlockAllocator:
@@ -238,6 +238,7 @@ class BeamSearcher:
             raise ValueError(f"1 to {B // nb} prompts fit")
         if max_new < 1 or any(not p or len(p) + max_new > dec.max_ctx for p in prompts):
             raise ValueError(f"need non-empty prompts, max_new >= 1 and at most {dec.max_ctx} positions")
+        check_tokens(prompts, dec.cfg.vocab)
         with PagePool(dec) as pool:
             return self._search(pool, prompts, max_new)
 
@@ -356,6 +357,7 @@ class TreeSpeculator:
             raise ValueError(f"1 to {B} prompts fit")
         if max_new < 1 or any(not p or len(p) + max_new > dec.max_ctx for p in prompts):
             raise ValueError(f"need non-empty prompts, max_new >= 1 and at most {dec.max_ctx} positions")
+        check_tokens(prompts, dec.cfg.vocab)
         with PagePool(dec) as pool:
             return self._generate(pool, prompts, max_new, eos)
 

@@ -86,6 +86,13 @@ def _wtype(cfg: DecoderConfig, layer: int, name: str) -> int:
     return cfg.wtype
 
 
+def check_tokens(texts, vocab: int):
+    """Raise unless every token of the texts is one of the vocabulary."""
+    for t in texts:
+        if t and not 0 <= min(t) <= max(t) < vocab:
+            raise ValueError(f"tokens must be in 0 .. {vocab - 1}")
+
+
 class Decoder:
     """Weights, paged KV cache and the captured decode step for `batch` sequences."""
 
@@ -483,6 +490,12 @@ class Decoder:
             raise ValueError("every drafted token needs a parent")
         if len(trees) != len(seqs) or len(start) != len(seqs):
             raise ValueError("seqs, trees and start differ in length")
+        # (a lookup on the device would meet a fault instead, or another row's cache)
+        if len(set(seqs)) != len(seqs) or any(not 0 <= s < self.batch for s in seqs):
+            raise ValueError(f"seqs must be different rows, 0 .. {self.batch - 1}")
+        if any(n < 0 for n in start):
+            raise ValueError("start must not be negative")
+        check_tokens(tokens, self.cfg.vocab)
         if self.tp_size == 1:
             return self._prefill(seqs, tokens, start, parents)
         lib = ops._lib.load()

@@ -230,3 +230,25 @@ def test_speculator_rows_wait_for_blocks(on_cpu, monkeypatch):
     # idle, two blocks each, one more for the second
     for n_blocks in (5, 6):
         assert batching.TreeSpeculator(FakeDecoder(2, 96, n_blocks + 1), wild).generate(prompts, 40, eos) == want
+
+
+@pytest.mark.parametrize("seqs,trees,start,word", [
+    ([0, 0], [([1], [-1])] * 2, [5, 5], "different rows"), ([0, 3], [([1], [-1])] * 2, [5, 5], "different rows"),
+    ([-1], [([1], [-1])], [5], "different rows"), ([1], [([1], [-1])], [-1], "start"), ([1], [([1, 50], [-1, 0])], [5], "tokens"),
+    ([1], [([1, -1], [-1, 0])], [5], "tokens"), ([1], [([1, 2], [-1])], [5], "parent"), ([1], [([1], [-1])], [5, 6], "length")])
+def test_verify_tree_refuses(seqs, trees, start, word):
+    """On the host, before anything is looked up on the device."""
+    from densecore_b200.decoder import Decoder
+    dec = Decoder.__new__(Decoder)
+    dec.batch, dec.tp_size, dec.cfg = 3, 1, types.SimpleNamespace(vocab=VOCAB)
+    with pytest.raises(ValueError, match=word):
+        dec.verify_tree(seqs, trees, start)
+
+
+@pytest.mark.parametrize("bad", [-1, VOCAB])
+def test_loops_refuse_tokens_beyond_the_vocabulary(on_cpu, bad):
+    dec = FakeDecoder(2, 64)
+    with pytest.raises(ValueError, match="tokens"):
+        batching.TreeSpeculator(dec).generate([[1, 2], [3, bad]], 5)
+    with pytest.raises(ValueError, match="tokens"):
+        batching.BeamSearcher(dec, 1).search([[1, 2], [bad]], 5)
