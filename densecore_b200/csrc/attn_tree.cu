@@ -616,16 +616,10 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
             int seg = 0, end = g.tiles;            // the segment's end among the range's units
             bool begins = true;                    // its Q not waited for yet
             uint64_t* q_empty = C.q_empty[b];
-            // S of unit n.  Each MMA warp sees every segment's Q land, also where it has no unit of the segment: the
-            // parity that it waits for at the next Q in the same buffer is that of a barrier without a phase behind
-            // it as well, so a Q not waited for would leave the next one's wait without effect.
+            // S of unit n
             auto issue_s = [&](int n, bool have_k) {
-                while (n >= end) {
-                    if (begins) {                  // (no unit of this warp: given back at once)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&C.q_full[seg % q_bufs], (uint32_t)((seg / q_bufs) & 1), &g_tree_error));
-                        if (!ok) return;
-                        if (leader) tc_commit(&q_empty[seg % q_bufs]);
-                    }
+                while (n >= end) {                 // (a segment that has no unit of this warp: given back at once)
+                    if (begins && leader) tc_commit(&q_empty[seg % q_bufs]);
                     seg_next<TW_ROWS, TW_KEYS>(a, g);
                     seg++;
                     end += g.tiles;
@@ -662,11 +656,11 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
                 }
                 __syncwarp();
             };
-            if (b < N) issue_s(b, false);
-            // The second warp sees S of unit 0 too.  Its first poll below is for S of unit 2, and the parity of that
-            // phase is also that of a barrier which has ended none: unit 1 would go on, and the ring with it, while
-            // K of unit 0 were still on its way.
-            if (b && b < N && ok) ok = __all_sync(0xffffffffu, mbar_wait(&C.s_full[0], 0, &g_tree_error));
+            // No S is issued before the one ahead of it has ended (below, by lane 2's wait).  So every Q up to then, and
+            // every K, has landed, also of segments and units that are the other warp's: a barrier that has ended no
+            // phase passes a wait for its second one, which has the same parity.
+            if (b && b < N) ok = __all_sync(0xffffffffu, mbar_wait(&C.s_full[0], 0, &g_tree_error));
+            if (b < N && ok) issue_s(b, false);
             for (int n = b; n < N && ok; n += 2) {  // O of unit n, then S of unit n + 2 into the same buffer
                 const uint32_t k = (uint32_t)n >> 1, l = tw_v(n, N), slot = l % TW_RING;
                 // one poll for all: lane 0 V, 1 O's buffer, 2 S of the next unit, others P.  (The third keeps the
