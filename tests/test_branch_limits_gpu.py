@@ -223,3 +223,57 @@ def test_speculator_in_a_tight_arena():
     spec = TreeSpeculator(dec, wild)
     assert spec.generate(prompts, 30) == greedy("q8_0", prompts, 30)
     assert device_error() == 0
+
+
+def test_verify_tree_on_two_shards(monkeypatch):
+    """The tensor-parallel pass: two shards of a model on this GPU, a thread each, with sums and gathers that
+    the host makes (no kernel waits for another), against the whole model."""
+    import threading
+
+    import torch.distributed as dist
+    from densecore_b200 import _lib
+    from densecore_b200.decoder import Decoder
+    from test_tp_gpu import _config
+    cfg, batch, _, max_ctx = _config("tiny")
+    whole = Decoder(cfg, batch=batch, max_ctx=max_ctx, seed=7)
+    shards = [Decoder(cfg, batch=batch, max_ctx=max_ctx, seed=7, tp_rank=r, tp_size=2) for r in range(2)]
+    meet, given, me = threading.Barrier(2, timeout=60), [None, None], threading.local()
+
+    def exchange(x):
+        given[me.rank] = x.clone()
+        meet.wait()
+        both = [t.clone() for t in given]
+        meet.wait()
+        return both
+    monkeypatch.setattr(dist, "all_reduce", lambda y, group=None: y.copy_(sum(exchange(y))))
+    monkeypatch.setattr(dist, "all_gather_into_tensor", lambda out, x, group=None: out.copy_(torch.stack(exchange(x))))
+    prompts = [[7, 300, 11, 5, 9, 100, 200, 301, 4, 4, 4, 17, 18], [42, 43]]
+    trees = [([1, 2, 3, 2, 9, 8, 7], [-1, 0, 0, 1, 2, 3, 2]), ([5, 6, 7], [-1, 0, 0])]
+
+    def run(dec):
+        dec.prefill([0, 1], prompts)
+        return dec.verify_tree([0, 1], trees, [len(p) for p in prompts])
+    got = [None, None]
+
+    def work(r):
+        me.rank = r
+        try:
+            got[r] = run(shards[r])
+        except BaseException as e:   # noqa: BLE001 -- told below; the other thread's barrier runs out
+            meet.abort()
+            got[r] = e
+    prev = _lib.load().dcg_set_programmatic_launch(1)
+    threads = [threading.Thread(target=work, args=(r,)) for r in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    _lib.load().dcg_set_programmatic_launch(prev)        # the threads' own saving of it may have crossed
+    for g in got:
+        if isinstance(g, BaseException):
+            raise g
+    _, want = run(whole)
+    for nxt, logits in got:
+        assert torch.equal(logits, got[0][1]) and torch.equal(nxt, logits.argmax(-1))
+        x, y = logits.double(), want.double()
+        assert bool(((x - y).norm(dim=-1) / y.norm(dim=-1) < 2e-3).all())      # the bar of shards against the whole
