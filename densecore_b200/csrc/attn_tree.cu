@@ -276,11 +276,12 @@ __device__ __forceinline__ void cut_h2(float x0, float x1, uint32_t& hi, uint32_
 // softmax, 12-15 the running output (128 registers of it per thread, thread = row).  tree_q_kernel has laid Q out
 // before: converting it here cost 20,000 cycles at every change of the item.
 // What bounds it: a unit's chain S (700 cycles stacked, 1,470 not), softmax (2,500), O (650 / 1,250) in two
-// streams, 2,400 cycles a stacked unit while items are long, which is an SM's share of HBM (5.9 TB/s); at an
-// item's end 4,000 cycles more for masks, cleaning and the change.  Times with tree_q_kernel and
-// tree_combine_kernel: 1 x 13 tokens, 100,003 of context 81 us (410 MB, 5.1 TB/s); 32 x 16, up to 2,048
-// 49 us (163 MB); 16 x 64, 64 heads, up to 4,096 148 us (118 GFLOP with both halves, 800 TFLOP/s); sustained, at
-// the power limit's clock, 99, 52 and 180 us.
+// streams, 2,400 cycles a stacked unit while items are long: 1.2 us at the full clock, where an SM's share of HBM is
+// the limit (64 KB, 1.5 us), and 1.6 us at the 1.5 GHz of long runs, where the chain is; at an item's end
+// 4,000 cycles more for masks, cleaning and the change.  Times with tree_q_kernel and
+// tree_combine_kernel: 1 x 13 tokens, 100,003 of context 83 us (410 MB, 4.9 TB/s); 32 x 16, up to 2,048
+// 49 us (163 MB); 16 x 64, 64 heads, up to 4,096 151 us (118 GFLOP with both halves, 780 TFLOP/s); sustained, at
+// the power limit's clock, 100, 52 and 181 us.
 // ------------------------------------------------------------------------------------------
 constexpr int TW_ROWS = 128;
 constexpr int TW_KEYS = 128;
@@ -1079,7 +1080,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tree_wide_kernel(
 // wide kernel; a block's P V starts from zero and is added to the running output in fp32 rounded to
 // nearest, because the tensor core cuts its sums off.  The warps merge in shared memory; splits leave
 // their parts for tree_join_kernel.
-// What bounds it: latency while contexts are short (8 tokens x 200: 7.8 us), HBM when they are long (8 x
+// What bounds it: latency while contexts are short (8 tokens x 200: 7.9 us), HBM when they are long (8 x
 // 100,003: 71 us, 5.8 TB/s).
 // ------------------------------------------------------------------------------------------
 constexpr int TF_CONS = 3;
