@@ -491,6 +491,7 @@ class Decoder:
         if len(trees) != len(seqs) or len(start) != len(seqs):
             raise ValueError("seqs, trees and start differ in length")
         # (a lookup on the device would meet a fault instead, or another row's cache)
+        seqs, start = [int(s) for s in seqs], [int(n) for n in start]
         if len(set(seqs)) != len(seqs) or any(not 0 <= s < self.batch for s in seqs):
             raise ValueError(f"seqs must be different rows, 0 .. {self.batch - 1}")
         if any(n < 0 for n in start):

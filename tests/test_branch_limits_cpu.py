@@ -195,10 +195,11 @@ def test_speculator_in_a_tight_arena(on_cpu, monkeypatch, draft):
     eos = greedy(prompts[0], 35)[3]
     want = [greedy(p, 35, eos) for p in prompts]
     assert len(want[0]) == 4 and batching.TreeSpeculator(FakeDecoder(4, 96, need), draft).generate(prompts, 35, eos) == want
-    before = dec.block_tables.clone()
+    small = FakeDecoder(1, 96, 4)
+    before = small.block_tables.clone()
     with pytest.raises(MemoryError):
-        batching.TreeSpeculator(FakeDecoder(1, 96, 4), draft).generate([[1] * 30], 35)
-    assert torch.equal(dec.block_tables, before) and Watched.forks
+        batching.TreeSpeculator(small, draft).generate([[1] * 30], 35)
+    assert torch.equal(small.block_tables, before) and Watched.forks
 
 
 def test_speculator_gives_every_block_back(on_cpu, monkeypatch):
@@ -233,7 +234,8 @@ def test_speculator_rows_wait_for_blocks(on_cpu, monkeypatch):
 
 
 @pytest.mark.parametrize("seqs,trees,start,word", [
-    ([0, 0], [([1], [-1])] * 2, [5, 5], "different rows"), ([0, 3], [([1], [-1])] * 2, [5, 5], "different rows"),
+    ([0, 0], [([1], [-1])] * 2, [5, 5], "different rows"), (torch.tensor([2, 2]), [([1], [-1])] * 2, [5, 5], "different rows"),
+    ([0, 3], [([1], [-1])] * 2, [5, 5], "different rows"),
     ([-1], [([1], [-1])], [5], "different rows"), ([1], [([1], [-1])], [-1], "start"), ([1], [([1, 50], [-1, 0])], [5], "tokens"),
     ([1], [([1, -1], [-1, 0])], [5], "tokens"), ([1], [([1, 2], [-1])], [5], "parent"), ([1], [([1], [-1])], [5, 6], "length")])
 def test_verify_tree_refuses(seqs, trees, start, word):
